@@ -4,7 +4,7 @@ There is no fallback: if the library cannot be loaded every operator raises.
 """
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_void_p
+from ctypes import POINTER, Structure, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_void_p
 
 from .build import LIB
 
@@ -25,6 +25,16 @@ class LBSGrads(Structure):
 class AdamTensor(Structure):
     _fields_ = [("param", _vp), ("grad", _vp), ("exp_avg", _vp), ("exp_avg_sq", _vp), ("M", c_int32),
                 ("lr", c_float), ("eps", c_float)]
+
+
+class AdamWTensor(Structure):
+    _fields_ = [("param", _vp), ("grad", _vp), ("exp_avg", _vp), ("exp_avg_sq", _vp), ("exp_avg_scale", _vp),
+                ("exp_avg_sq_scale", _vp), ("master", _vp), ("step", _vp), ("numel", c_int64), ("lr", c_float),
+                ("weight_decay", c_float)]
+
+
+class NormTensor(Structure):
+    _fields_ = [("data", _vp), ("numel", c_int64), ("type", c_int32)]
 
 
 class RowTensor(Structure):
@@ -120,6 +130,9 @@ SYMBOLS = {
     "fsgs_adam_masked": (c_int, [_vp, _vp, _vp, _vp, _vp, c_float, c_float, c_float, c_float, c_int64, c_int64, _vp]),
     "fsgs_adam_masked_multi": (c_int, [c_int, POINTER(AdamTensor), _vp, c_int64, c_float, c_float, _vp]),
     "fsgs_adam_masked_multi_fmask": (c_int, [c_int, POINTER(AdamTensor), _vp, c_int64, c_float, c_float, _vp]),
+    "fsgs_adamw_multi": (c_int, [c_int, _vp, c_int, c_int, c_int, c_double, c_double, c_float, _vp, _vp, _vp, _vp]),
+    "fsgs_grad_norm_workspace_bytes": (c_size_t, []),
+    "fsgs_grad_norm": (c_int, [c_int, _vp, c_float, _vp, c_size_t, _vp, _vp]),
     "fsgs_view_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int64, c_int, c_int]),
     "fsgs_motion_param_count": (c_int64, [POINTER(MotionCfg)]),
     "fsgs_motion_param_offsets": (c_int, [POINTER(MotionCfg), POINTER(c_int64), POINTER(c_int32)]),

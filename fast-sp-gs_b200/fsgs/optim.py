@@ -1,12 +1,16 @@
 """``SparseGaussianAdam``: the reference's visibility-masked Adam (``fast_2d_gs/sparse_gaussian_adam.py:10-49``)
-with every parameter group updated by ONE kernel launch instead of one launch per group."""
+with every parameter group updated by ONE kernel launch instead of one launch per group; ``DenseAdam`` for dense
+parameters through the same kernel; ``AdamW`` over many dense tensors with moments in 32 or in 8 bits, clipping by the
+norm of all gradients (``grad_norm``) and a step count on the device."""
 import ctypes
+import operator
 
+import numpy as np
 import torch
 
 from . import _lib
 from ._lib import lib, check
-from .ops import _ptr, _stream
+from .ops import _need, _on_device, _ptr, _stream
 
 
 class SparseGaussianAdam(torch.optim.Adam):
@@ -131,3 +135,316 @@ def masked_adam_step(batch, visibility, N, b1=0.9, b2=0.999):
             arr[k].param, arr[k].grad, arr[k].exp_avg, arr[k].exp_avg_sq = p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr()
             arr[k].M, arr[k].lr, arr[k].eps = p.numel() // N, lr, eps
         check(launch(len(chunk), arr, _ptr(vis), int(N), b1, b2, _stream()), "fsgs_adam_masked_multi")
+
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # FSGS_F32, FSGS_BF16, FSGS_F16
+_BLOCK = 256                                                        # FSGS_ADAMW_BLOCK
+_data_ptr, _numel, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_table_type = np.dtype([(n, np.float32 if t is ctypes.c_float else np.int64) for n, t in _lib.AdamWTensor._fields_])
+_norm_type = np.dtype([("data", np.int64), ("numel", np.int64), ("type", np.int64)])
+assert _table_type.itemsize == ctypes.sizeof(_lib.AdamWTensor) and _norm_type.itemsize == ctypes.sizeof(_lib.NormTensor)
+
+
+def _norm_workspace(device):
+    return torch.zeros(int(lib().fsgs_grad_norm_workspace_bytes()), dtype=torch.uint8, device=device)
+
+
+def _launch_norm(data, numel, types, max_norm, workspace, out):
+    table = np.empty(len(data), _norm_type)
+    table["data"], table["numel"], table["type"] = data, numel, types
+    check(lib().fsgs_grad_norm(len(data), table.ctypes.data, max_norm, _ptr(workspace), workspace.numel(), _ptr(out),
+                               _stream()), "fsgs_grad_norm")
+
+
+def grad_norm(tensors, max_norm=None):
+    """``(norm, factor)``: the 2-norm of all elements of all ``tensors`` (float32, bfloat16 or float16, on one device)
+    and ``min(1, max_norm / (norm + 1e-6))``, the factor that clips them to ``max_norm`` -- 1 without ``max_norm``, 0
+    where the norm is not finite.  Two float32 device scalars, one launch (per 256 tensors) and no synchronisation; the
+    factor can be given to ``AdamW.step(grad_scale=...)``.  Summed in a fixed order: the same gradients give the same
+    bits."""
+    tensors = [t.detach() for t in tensors]
+    _need(len(tensors) > 0, "grad_norm: no tensors")
+    _need(max_norm is None or max_norm > 0, "grad_norm: max_norm must be positive")
+    device = tensors[0].device
+    for t in tensors:
+        _need(t.is_cuda and t.device == device and t.dtype in _TYPES and t.layout == torch.strided,
+              "grad_norm: dense float32, bfloat16 or float16 CUDA tensors on one device")
+    tensors = [t.contiguous() for t in tensors]
+    with _on_device(device):
+        out = torch.empty(2, device=device)
+        _launch_norm(list(map(_data_ptr, tensors)), list(map(_numel, tensors)), [_TYPES[t.dtype] for t in tensors],
+                     float("inf") if max_norm is None else float(max_norm), _norm_workspace(device), out)
+    return out[0], out[1]
+
+
+class _Launch:
+    """The tensors of one ``fsgs_adamw_multi`` call: those that share their types, betas and eps."""
+
+    def __init__(self, rows, whole, param_type, grad_type, betas, eps):
+        self.rows, self.whole = rows, whole     # places in the plan's lists; whether they are all of them
+        self.table = np.zeros(len(rows), _table_type)
+        self.head = (len(rows), self.table.ctypes.data, param_type, grad_type)
+        self.scalars = (float(betas[0]), float(betas[1]), float(eps))
+
+
+class _Plan:
+    """The argument tables of a step for one list of parameters.  ``matches`` reads every address and length anew: a
+    plan is used only while the parameters, their state tensors and their places are what it was made from."""
+
+    def __init__(self, opt, params):
+        self.params, self.device = params, params[0].device
+        group_of = {id(p): k for k, g in enumerate(opt.param_groups) for p in g["params"]}
+        self.groups = [group_of[id(p)] for p in params]
+        for p in params:
+            _need(p.is_cuda and p.device == self.device, "AdamW: CUDA parameters on one device")
+            _need(p.is_contiguous() and p.dtype in _TYPES, "AdamW: contiguous float32, bfloat16 or float16 parameters")
+            _need(p.grad.layout == torch.strided and (p.grad.dtype == p.dtype or p.grad.dtype == torch.float32),
+                  "AdamW: a dense gradient of its parameter's type or float32")
+        self.numel = list(map(_numel, params))
+        self.grad_dtypes = [p.grad.dtype for p in params]
+        self.grad_types = [_TYPES[t] for t in self.grad_dtypes]
+        self.states = [opt._state_of(p) for p in params]
+        self.names = [opt._names(p) for p in params]
+        self.read = [operator.itemgetter(*n) for n in self.names]
+        for p, st, names in zip(params, self.states, self.names):
+            for name in names:
+                _need(name in st, f"AdamW: a parameter's state has no {name}")
+                t = st[name]
+                want = (p.numel() + _BLOCK - 1) // _BLOCK if name.endswith("_scale") else 1 if name == "step" else p.numel()
+                kind = torch.float8_e4m3fn if opt.state_bits == 8 and name in ("exp_avg", "exp_avg_sq_root") else torch.float32
+                _need(t.device == self.device and t.dtype == kind and t.numel() == want and t.is_contiguous(),
+                      f"AdamW: the state {name} must be a contiguous {kind} tensor of {want} elements on {self.device}")
+        self.settings_key = self._settings(opt)
+        self.addresses = self._addresses(params)
+        kinds = {}
+        for i, (p, k) in enumerate(zip(params, self.groups)):
+            g = opt.param_groups[k]
+            key = (_TYPES[p.dtype], self.grad_types[i], "master" in self.names[i], tuple(g["betas"]), g["eps"])
+            kinds.setdefault(key, []).append(i)
+        self.launches = []
+        for (param_type, grad_type, _, betas, eps), rows in kinds.items():
+            launch = _Launch(rows, len(rows) == len(params), param_type, grad_type, betas, eps)
+            t = launch.table
+            pick = lambda name: [self.states[i][name].data_ptr() if name in self.names[i] else 0 for i in rows]  # noqa: E731
+            t["param"], t["numel"] = [params[i].data_ptr() for i in rows], [self.numel[i] for i in rows]
+            t["step"], t["exp_avg"], t["master"] = pick("step"), pick("exp_avg"), pick("master")
+            t["exp_avg_sq"] = pick("exp_avg_sq" if opt.state_bits == 32 else "exp_avg_sq_root")
+            t["exp_avg_scale"], t["exp_avg_sq_scale"] = pick("exp_avg_scale"), pick("exp_avg_sq_root_scale")
+            self.launches.append(launch)
+        self._rates(opt)
+
+    @staticmethod
+    def _settings(opt):
+        return [(len(g["params"]), tuple(g["betas"]), g["eps"], float(g["lr"]), g["weight_decay"]) for g in opt.param_groups]
+
+    def _rates(self, opt):
+        lr, wd = ([float(g[k]) for g in opt.param_groups] for k in ("lr", "weight_decay"))
+        for launch in self.launches:
+            launch.table["lr"] = [lr[self.groups[i]] for i in launch.rows]
+            launch.table["weight_decay"] = [wd[self.groups[i]] for i in launch.rows]
+
+    def _addresses(self, params):
+        out = list(map(_data_ptr, params))
+        for read, st in zip(self.read, self.states):
+            out.extend(map(_data_ptr, read(st)))
+        return out
+
+    def matches(self, opt, params):
+        if len(params) != len(self.params) or not all(map(operator.is_, params, self.params)):
+            return False
+        if not all(map(operator.is_, map(opt.state.get, params), self.states)):
+            return False
+        try:
+            if self._addresses(params) != self.addresses or list(map(_numel, params)) != self.numel:
+                return False
+        except KeyError:
+            return False
+        settings = self._settings(opt)
+        if settings != self.settings_key:
+            if [s[:3] for s in settings] != [s[:3] for s in self.settings_key]:
+                return False
+            self.settings_key = settings
+            self._rates(opt)
+        return True
+
+    def gradients(self, grads):
+        """Addresses of the gradients, contiguous (``self.kept`` holds copies until the next step)."""
+        self.kept = None
+        if not all(map(_is_contiguous, grads)):
+            grads = self.kept = [g.contiguous() for g in grads]
+        _need(list(map(_numel, grads)) == self.numel, "AdamW: a gradient has another size than its parameter")
+        return list(map(_data_ptr, grads))
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) over any number of dense tensors, one launch for all that share their types:
+
+        ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
+        ``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)``.
+
+    Parameters are contiguous CUDA tensors of float32, bfloat16 or float16 on one device, gradients of the parameter's
+    type or (``param.grad_dtype``) float32.  ``lr``, ``betas``, ``eps`` and ``weight_decay`` are per group and may be
+    changed between steps.
+
+    * ``state_bits=32``: state ``step`` (float32 device scalar), ``exp_avg``, ``exp_avg_sq`` (float32): the layout of
+      ``torch.optim.AdamW``, whose ``state_dict`` loads.
+    * ``state_bits=8``: 2.03 bytes per element instead of 8.  ``exp_avg`` and ``exp_avg_sq_root`` = sqrt(v) are
+      ``torch.float8_e4m3fn`` tensors, each with a float32 scale per 256 elements (``..._scale``): value = element *
+      scale.  The rounding is to nearest: second moments of elements that move against their block by less than a
+      sixteenth per step stay where they are.  A gradient that is not finite spoils its block of 256.
+    * ``master_weights=True``: 16-bit parameters are updated through a float32 copy in the state (``master``); without
+      it an update below half a unit of the parameter's last place is lost.
+    * ``max_grad_norm``: every step is preceded by the norm of all its gradients and clips by it; ``self.grad_norm``
+      is the last norm (a device scalar, overwritten by the next step).  A step whose norm is not finite is dropped.
+
+    A dropped step -- that, or a closed ``gate`` -- leaves parameters, moments and step counts as they were; the decision
+    is taken on the device.  Nothing synchronises.  A step can be captured into a CUDA graph once the state exists (after
+    a step, or ``init_state()``): the step counts advance with every replay, while learning rates and the other numbers
+    are those of the capture, and gradients are read where they lay then.  Steps of one optimiser have to follow one
+    another on their stream."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
+                 master_weights=False, max_grad_norm=None):
+        _need(state_bits in (8, 32), "AdamW: state_bits is 8 or 32")
+        _need(max_grad_norm is None or max_grad_norm > 0, "AdamW: max_grad_norm must be positive")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.master_weights, self.max_grad_norm = state_bits, bool(master_weights), max_grad_norm
+        self._plan = self._ticket = self._norm = None
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        _need(float(g["lr"]) >= 0 and g["eps"] >= 0 and g["weight_decay"] >= 0 and
+              all(0 <= b < 1 for b in g["betas"]), "AdamW: lr, eps, weight_decay >= 0 and 0 <= beta < 1")
+        for p in g["params"]:
+            _need(p.dtype in _TYPES and p.layout == torch.strided, "AdamW: dense float32, bfloat16 or float16 parameters")
+
+    @property
+    def grad_norm(self):
+        """Norm of all gradients of the last step (``max_grad_norm``), before clipping; a device scalar."""
+        return None if self._norm is None else self._norm[0][0]
+
+    # ---- state --------------------------------------------------------------------------------------------------
+    def _names(self, param):
+        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else \
+            ("exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale")
+        return ("step",) + names + (("master",) if self.master_weights and param.dtype != torch.float32 else ())
+
+    def _fresh(self, p, name):
+        if name == "step":
+            return torch.zeros((), dtype=torch.float32, device=p.device)
+        if name == "master":
+            return p.detach().float().contiguous()
+        if name.endswith("_scale"):
+            return torch.zeros((p.numel() + _BLOCK - 1) // _BLOCK, dtype=torch.float32, device=p.device)
+        return torch.zeros(p.shape, dtype=torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn, device=p.device)
+
+    @torch.no_grad()
+    def init_state(self):
+        """Create the state of every parameter that has none yet (a step does that for those with a gradient)."""
+        for group in self.param_groups:
+            for p in group["params"]:
+                _need(p.is_cuda, "AdamW: CUDA parameters on one device")
+                self._state_of(p)
+                with _on_device(p.device):
+                    self._workspaces(p.device)
+
+    def _state_of(self, p):
+        st = self.state[p]
+        if len(st) == 0:
+            _need(not (p.is_cuda and torch.cuda.is_current_stream_capturing()),
+                  "AdamW: the state has to exist before a step is captured (take a step, or call init_state())")
+            for name in self._names(p):
+                st[name] = self._fresh(p, name)
+        return st
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """As ``torch.optim.Optimizer.load_state_dict``, with every state tensor kept in its own type (the base class
+        casts them to the parameter's) and copied to the parameter's device.  A state in another number of bits, or
+        without the master copy that this optimiser keeps, is refused."""
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        own = [p for g in self.param_groups for p in g["params"]]
+        _need(len(ids) == len(own), "AdamW: the loaded state has another number of parameters")
+        loaded = {}
+        for i, p in zip(ids, own):
+            st = state_dict["state"].get(i)
+            if not st:
+                continue
+            for name in self._names(p):
+                _need(name in st, f"AdamW: the loaded state has no {name} (state_bits={self.state_bits}, "
+                                  f"master_weights={self.master_weights})")
+                fresh, value = self._fresh(p, name), torch.as_tensor(st[name])
+                _need(value.numel() == fresh.numel() and (value.dtype == fresh.dtype or name == "step"),
+                      f"AdamW: the loaded {name} has another size or type")
+                loaded.setdefault(p, {})[name] = fresh.copy_(value.reshape(fresh.shape))
+        before = {p: self.state[p] for p in own if p in self.state}
+        super().load_state_dict(dict(state_dict, state={}))
+        for p, new in loaded.items():
+            st = before.get(p, {})
+            if set(st) == set(new) and all(st[n].shape == t.shape and st[n].dtype == t.dtype and st[n].device == t.device
+                                           for n, t in new.items()):
+                for n, t in new.items():   # into the tensors that are there: a captured step goes on using them
+                    st[n].copy_(t)
+                new = st
+            self.state[p] = new
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), state_bits=self.state_bits, master_weights=self.master_weights,
+                    max_grad_norm=self.max_grad_norm)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plan = None
+        self.__dict__.setdefault("_ticket", None)
+        self.__dict__.setdefault("_norm", None)
+
+    # ---- the step -----------------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, gate=None, grad_scale=None):
+        """``gate``: a one-element float32 device tensor; the step is applied where it is > 0.  ``grad_scale``: a
+        one-element float32 device tensor that multiplies every gradient; the step is dropped where it is not positive
+        and finite (not together with ``max_grad_norm``, which makes its own)."""
+        self.step_gated(gate, grad_scale)
+
+    def step_gated(self, gate=None, grad_scale=None):
+        """The body of ``step`` without the hook layers that ``torch.optim.Optimizer`` wraps around it."""
+        params, grads = [], []
+        for group in self.param_groups:
+            for p in group["params"]:
+                g = p.grad
+                if g is not None:
+                    params.append(p)
+                    grads.append(g)
+        if not params:
+            return
+        _need(grad_scale is None or self.max_grad_norm is None, "AdamW: grad_scale together with max_grad_norm")
+        plan = self._plan
+        if plan is None or [g.dtype for g in grads] != plan.grad_dtypes or not plan.matches(self, params):
+            plan = self._plan = _Plan(self, params)
+        device = plan.device
+        for t in (gate, grad_scale):
+            _need(t is None or (t.device == device and t.numel() == 1 and t.dtype == torch.float32),
+                  "AdamW: gate and grad_scale are one-element float32 tensors on the parameters' device")
+        with _on_device(device):
+            self._workspaces(device)
+            data = plan.gradients(grads)
+            if self.max_grad_norm is not None:
+                _launch_norm(data, plan.numel, plan.grad_types, self.max_grad_norm, self._norm[1], self._norm[0])
+                grad_scale = self._norm[0][1:]
+            tail = (_ptr(grad_scale), _ptr(gate), _ptr(self._ticket[0]), _stream())
+            for launch in plan.launches:
+                launch.table["grad"] = data if launch.whole else [data[i] for i in launch.rows]
+                check(lib().fsgs_adamw_multi(*launch.head, self.state_bits, *launch.scalars, *tail), "fsgs_adamw_multi")
+
+    def _workspaces(self, device):
+        """Created once, zeroed once: the kernels leave their counters at zero.  Never replaced on the same device: a
+        captured step goes on using them."""
+        for name, wanted, make in (("_ticket", True, lambda: (torch.zeros(1, dtype=torch.int32, device=device),)),
+                                   ("_norm", self.max_grad_norm is not None,
+                                    lambda: (torch.zeros(2, device=device), _norm_workspace(device)))):
+            have = getattr(self, name)
+            if wanted and (have is None or have[0].device != device):
+                _need(not torch.cuda.is_current_stream_capturing(),
+                      "AdamW: take a step, or call init_state(), before a step is captured")
+                setattr(self, name, make())

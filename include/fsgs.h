@@ -104,6 +104,65 @@ int fsgs_adam_masked_multi_fmask(int n_tensors, const fsgs_adam_tensor *tensors 
     int64_t N, float b1, float b2, fsgs_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * AdamW over many tensors, and the norm of all gradients.  Additive: the reference trains its dense parameters with
+ * torch.optim.Adam (fast_2d_gs/network.py:296-305); this is the same update with decoupled weight decay, clipping, a
+ * step count on the device and moments in float32 or in 8 bits.
+ *
+ *   g' = c g ; m' = b1 m + (1 - b1) g' ; v' = b2 v + (1 - b2) g'^2 ; t = *step + 1
+ *   p' = p (1 - lr weight_decay) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+ *
+ * state_bits 32: exp_avg and exp_avg_sq hold m and v as floats.  state_bits 8: they hold m and sqrt(v) as e4m3 bytes
+ * with one scale per FSGS_ADAMW_BLOCK consecutive elements (exp_avg_scale / exp_avg_sq_scale,
+ * [ceil(numel / FSGS_ADAMW_BLOCK)]): value = byte * scale, scale = largest magnitude of the block / 448; a positive
+ * sqrt(v) is held as no less than the smallest positive byte; a block whose largest magnitude is below 2^-110 is held
+ * as zeros.  A gradient that is not finite spoils its element (32 bits) or its block (8 bits).
+ * param_type: FSGS_F32, FSGS_BF16 or FSGS_F16; grad_type: FSGS_F32 or the same as param_type.  master (16-bit
+ * parameters; for all tensors of a call or for none): the float32 parameter that is updated, param receives it rounded.
+ * grad_scale (device, optional): c; gate (device, optional).  A call with *gate <= 0, or with *grad_scale <= 0 or not
+ * finite, changes nothing, the step counts included.
+ * step: one float per tensor, advanced by the call.  ticket: one int32 in device memory, zero before its first call;
+ * calls leave it zero.  Calls that may run at the same time need tickets of their own.
+ * Tensors are contiguous; any alignment of the element type works, 16 bytes is the fast one.
+ * ---------------------------------------------------------------------------------------------- */
+#define FSGS_F32 0
+#define FSGS_BF16 1
+#define FSGS_F16 2
+#define FSGS_ADAMW_BLOCK 256
+
+typedef struct fsgs_adamw_tensor {
+  void *param;
+  const void *grad;
+  void *exp_avg;
+  void *exp_avg_sq;
+  float *exp_avg_scale;    /* state_bits 8, else NULL */
+  float *exp_avg_sq_scale;
+  float *master;           /* or NULL */
+  float *step;             /* [1] */
+  int64_t numel;
+  float lr;
+  float weight_decay;
+} fsgs_adamw_tensor;
+
+int fsgs_adamw_multi(int n_tensors, const fsgs_adamw_tensor *tensors /* host */, int param_type, int grad_type,
+    int state_bits, double beta1, double beta2, float eps, const float *grad_scale, const float *gate, int32_t *ticket,
+    fsgs_stream_t stream);
+
+/* out[0] = sqrt(sum of the squares of all elements of all tensors), out[1] = min(1, max_norm / (out[0] + 1e-6)), or 0
+ * where the norm is not finite: the grad_scale of fsgs_adamw_multi.  Summed in a fixed order: the same gradients give
+ * the same bits.  workspace: 16-byte aligned; its first four bytes zero before its first call, calls leave them zero;
+ * calls that may run at the same time need workspaces of their own. */
+typedef struct fsgs_norm_tensor {
+  const void *data;
+  int64_t numel;
+  int32_t type;
+} fsgs_norm_tensor;
+
+#define FSGS_GRAD_NORM_SLOTS 1184
+size_t fsgs_grad_norm_workspace_bytes(void);
+int fsgs_grad_norm(int n_tensors, const fsgs_norm_tensor *tensors /* host */, float max_norm, void *workspace,
+    size_t workspace_bytes, float *out, fsgs_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Splat -> screen matrix, standalone.
  * Replaces gs_2d_fast_compute_transmat_forward / gs_2d_fast_compute_trans_mat_backward
  * (src/gaussian_splatting/gs_2d_fast_preprocess.cu:871-909, 923-958).

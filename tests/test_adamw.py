@@ -1,0 +1,97 @@
+"""AdamW on the CPU: what it refuses, and what its state dictionary keeps."""
+import copy
+
+import pytest
+import torch
+
+from fsgs.optim import AdamW, grad_norm
+
+
+def _with_state(opt):
+    """State as a step would have left it, filled with values that survive no cast unnoticed."""
+    for k, p in enumerate(p for g in opt.param_groups for p in g["params"]):
+        st = opt._state_of(p)
+        for name, t in st.items():
+            if t.dtype == torch.float8_e4m3fn:
+                t.copy_((torch.arange(t.numel()).reshape(t.shape) % 13 - 6.0).to(torch.float8_e4m3fn))
+            else:
+                t.copy_(torch.linspace(1.00001, 2.00001, t.numel()).reshape(t.shape) * (k + 1))
+    return opt
+
+
+def _params(dtype=torch.float32):
+    return [torch.nn.Parameter(torch.randn(n, dtype=torch.float32).to(dtype)) for n in (5, 300)]
+
+
+@pytest.mark.parametrize("kw", [dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(betas=(-0.1, 0.9)),
+                                dict(eps=-1e-8), dict(weight_decay=-0.1), dict(max_grad_norm=0.0), dict(max_grad_norm=-1.0)])
+def test_refused_settings(kw):
+    with pytest.raises(RuntimeError):
+        AdamW(_params(), **kw)
+
+
+def test_refused_parameters():
+    with pytest.raises(RuntimeError):
+        AdamW([torch.nn.Parameter(torch.zeros(3, dtype=torch.float64))])
+    p = _params()
+    p[0].grad = torch.ones(5)
+    for opt in (AdamW(p), AdamW(p, state_bits=8, max_grad_norm=1.0)):
+        with pytest.raises(RuntimeError):
+            opt.step()                         # no CPU path
+        with pytest.raises(RuntimeError):
+            opt.init_state()
+    AdamW(_params()).step()                    # nothing has a gradient: nothing to do
+    for bad in ([], [torch.zeros(3)]):
+        with pytest.raises(RuntimeError):
+            grad_norm(bad)
+
+
+@pytest.mark.parametrize("bits,dtype,master", [(32, torch.float32, False), (8, torch.float32, False),
+                                               (32, torch.bfloat16, True), (8, torch.float16, True), (8, torch.bfloat16, False)])
+def test_state_dict_keeps_types_and_bits(bits, dtype, master, tmp_path):
+    a = _with_state(AdamW(_params(dtype), lr=3e-4, state_bits=bits, master_weights=master))
+    torch.save(a.state_dict(), tmp_path / "s.pt")
+    sd = torch.load(tmp_path / "s.pt")
+    b = AdamW(_params(dtype), state_bits=bits, master_weights=master)
+    for _ in range(2):                         # into an optimiser without state, and into one with it
+        before = {p: dict(st) for p, st in b.state.items()}
+        b.load_state_dict(sd)
+        assert b.param_groups[0]["lr"] == 3e-4
+        for p, q in zip(a.param_groups[0]["params"], b.param_groups[0]["params"]):
+            assert set(a.state[p]) == set(b.state[q]) == set(a._names(p))
+            for name, t in a.state[p].items():
+                u = b.state[q][name]
+                assert u.dtype == t.dtype and u.shape == t.shape and torch.equal(u.float(), t.float()), name
+                assert q not in before or before[q][name] is u, "state tensors that are there are written, not replaced"
+
+
+def test_state_dicts_that_do_not_fit_are_refused():
+    sd32 = _with_state(AdamW(_params())).state_dict()
+    sd8 = _with_state(AdamW(_params(), state_bits=8)).state_dict()
+    for opt, sd in ((AdamW(_params(), state_bits=8), sd32), (AdamW(_params()), sd8),
+                    (AdamW(_params(torch.bfloat16), master_weights=True), sd32),
+                    (AdamW(_params()[:1]), sd32), (AdamW(_params()[::-1]), sd32)):
+        with pytest.raises(RuntimeError):
+            opt.load_state_dict(sd)
+        assert len(opt.state) == 0
+
+
+def test_state_of_torchs_adamw_loads():
+    p = _params()
+    ref = torch.optim.AdamW(p, lr=1e-2)
+    for q in p:
+        q.grad = torch.randn_like(q)
+    ref.step()
+    opt = AdamW(p, lr=1.0)
+    opt.load_state_dict(ref.state_dict())
+    for q in p:
+        assert float(opt.state[q]["step"]) == 1.0
+        assert torch.equal(opt.state[q]["exp_avg"], ref.state[q]["exp_avg"])
+        assert torch.equal(opt.state[q]["exp_avg_sq"], ref.state[q]["exp_avg_sq"])
+
+
+def test_copies_keep_their_settings():
+    a = _with_state(AdamW(_params(torch.bfloat16), state_bits=8, master_weights=True, max_grad_norm=2.0))
+    b = copy.deepcopy(a)
+    assert (b.state_bits, b.master_weights, b.max_grad_norm) == (8, True, 2.0) and b.grad_norm is None
+    assert {len(s) for s in b.state.values()} == {6}

@@ -1,0 +1,369 @@
+"""The AdamW step and the gradient norm against the formulas evaluated in float64, one step at a time from the state
+that the step before left.
+
+Tolerances, e = 2^-24 (half a unit of float32).  With g' = c g (c: the clip factor, 6 e off: the norm 3, its inverse and
+product 3) and M = |b1 m| + |(1 - b1) g'|: the first moment is 12 e M off (8-bit states add a product: e), the second 20 e
+relative, so its root 11 e, the denominator 15 e; the quotient is the device's approximate one (2 units: 4 e), the factor
+lr / (1 - b1^t) and its product 2 e.  The update U = lr / (1 - b1^t) M / (sqrt(v) / sqrt(1 - b2^t) + eps) is thus at
+most 34 e U off and the parameter, with its own product, sum and rounded constant, 4 e |p| more; 40 e U + 4 e |p| is
+asked for, and half a unit of the parameter's type on top where that has 16 bits.  A moment in 8 bits is off by half a
+step of its format, 2^-4 relative or 2^-10 of its scale where the format is denormal; sqrt(v) by a whole smallest step,
+2^-9 of its scale, since it never rounds to zero."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+B = 256
+
+
+def _make(sizes, ptype, gtype, seed=0, offset=0, spread=2.0):
+    """Parameters and gradients as slices of longer buffers, `offset` elements from an aligned start."""
+    gen = torch.Generator().manual_seed(seed)
+    params, grads = [], []
+    for n in sizes:
+        x = torch.randn(n + 16, generator=gen) * 0.5
+        g = torch.randn(n + 16, generator=gen) * torch.exp(spread * torch.randn(n + 16, generator=gen)) * 1e-3
+        g[torch.rand(n + 16, generator=gen) < 0.1] = 0
+        p = torch.nn.Parameter(x.to(ptype).cuda()[offset:offset + n])
+        p.grad_dtype = gtype
+        params.append(p)
+        grads.append(g.to(gtype).cuda()[offset:offset + n])
+    return params, grads
+
+
+def _values(opt, p):
+    """(m, sqrt(v), scale of m, scale of sqrt(v)) of a parameter in float64; scales per element, 0 where 32 bits."""
+    st = opt.state[p]
+    if opt.state_bits == 32:
+        z = torch.zeros_like(st["exp_avg"], dtype=torch.float64)
+        return st["exp_avg"].double(), st["exp_avg_sq"].double().sqrt(), z, z
+    ms, ss = (st[k].double().repeat_interleave(B)[:p.numel()] for k in ("exp_avg_scale", "exp_avg_sq_root_scale"))
+    return st["exp_avg"].double() * ms, st["exp_avg_sq_root"].double() * ss, ms, ss
+
+
+def _snapshot(opt, params):
+    out = []
+    for p in params:
+        m, s, _, _ = _values(opt, p) if opt.state.get(p) else (torch.zeros_like(p, dtype=torch.float64),) * 4
+        master = opt.state[p].get("master") if opt.state.get(p) else None
+        out.append(((p if master is None else master).detach().double().clone(), m.clone(), s.clone(),
+                    float(opt.state[p]["step"]) if opt.state.get(p) else 0.0))
+    return out
+
+
+def _check_step(opt, before, params, grads, factor=1.0):
+    group_of = {id(p): g for g in opt.param_groups for p in g["params"]}
+    for (p0, m0, s0, t0), p, g in zip(before, params, grads):
+        grp = group_of[id(p)]
+        (b1, b2), lr, wd, eps = grp["betas"], grp["lr"], grp["weight_decay"], grp["eps"]
+        g = g.double() * factor
+        m1 = b1 * m0 + (1 - b1) * g
+        v1 = b2 * s0 ** 2 + (1 - b2) * g ** 2
+        t = t0 + 1
+        rate, den = lr / (1 - b1 ** t), v1.sqrt() / math.sqrt(1 - b2 ** t) + eps
+        want = p0 * (1 - lr * wd) - rate * m1 / den
+        size = (b1 * m0).abs() + ((1 - b1) * g).abs()
+        tol = 40 * E * rate * size / den + 4 * E * p0.abs() + 1e-40
+        st = opt.state[p]
+        assert float(st["step"]) == t
+        half = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[p.dtype]
+        if "master" in st:
+            assert bool(((st["master"].double() - want).abs() <= tol).all())
+            assert torch.equal(st["master"].to(p.dtype), p.detach())
+        smallest = 2.0 ** -25 if p.dtype == torch.float16 else 0.0     # half a step of fp16's denormals
+        assert bool(((p.detach().double() - want).abs() <= tol + half * (want.abs() + tol) + smallest).all())
+        m, s, ms, ss = _values(opt, p)
+        mt = 13 * E * size + 1e-40
+        stol = 11 * E * v1.sqrt() + 1e-40
+        if opt.state_bits == 8:
+            mt = mt + torch.maximum(2.0 ** -4 * m1.abs(), 2.0 ** -10 * ms) * (1 + 8 * E)
+            stol = stol + torch.maximum(2.0 ** -4 * v1.sqrt(), 2.0 ** -9 * ss) * (1 + 8 * E)
+            assert bool((s[v1 > 1e-60] > 0).all()), "a positive second moment was rounded to zero"
+            for name, x in (("exp_avg_scale", m1), ("exp_avg_sq_root_scale", v1.sqrt())):
+                top = torch.nn.functional.pad(x.abs(), (0, -x.numel() % B)).view(-1, B).amax(dim=1)
+                room = torch.nn.functional.pad(size if name == "exp_avg_scale" else x, (0, -x.numel() % B)).view(-1, B).amax(dim=1)
+                assert bool(((st[name].double() * 448 - top).abs() <= 16 * E * room + 1e-30).all()), name
+        assert bool(((m - m1).abs() <= mt).all()) and bool(((s - v1.sqrt()).abs() <= stol).all())
+
+
+SIZES = (1, 7, 255, 256, 257, 1000, 2047, 2048, 2049, 9001)
+KINDS = [(torch.float32, torch.float32, 32, False), (torch.float32, torch.float32, 8, False),
+         (torch.bfloat16, torch.bfloat16, 32, False), (torch.bfloat16, torch.float32, 32, True),
+         (torch.bfloat16, torch.bfloat16, 8, True), (torch.bfloat16, torch.float32, 8, False),
+         (torch.float16, torch.float16, 32, True), (torch.float16, torch.float32, 32, False),
+         (torch.float16, torch.float16, 8, False), (torch.float16, torch.float32, 8, True)]
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("ptype,gtype,bits,master", KINDS)
+def test_step_vs_formula(ptype, gtype, bits, master, offset):
+    from fsgs.optim import AdamW
+    params, _ = _make(SIZES, ptype, gtype, offset=offset)
+    opt = AdamW([dict(params=params[:4], weight_decay=0.1), dict(params=params[4:], lr=3e-4, betas=(0.8, 0.99))],
+                lr=1e-2, weight_decay=0.0, state_bits=bits, master_weights=master)
+    for k in range(3):
+        _, grads = _make(SIZES, ptype, gtype, seed=k + 1, offset=offset)
+        for p, g in zip(params, grads):
+            p.grad = g
+        before = _snapshot(opt, params)
+        opt.step()
+        _check_step(opt, before, params, grads)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_many_tensors_clipped_by_their_norm(bits):
+    """More tensors than one launch takes, of two types, with and without clipping taking hold."""
+    from fsgs.optim import AdamW
+    sizes = [(k * 37) % 700 + 1 for k in range(600)]
+    a, _ = _make(sizes[:300], torch.float32, torch.float32)
+    b, _ = _make(sizes[300:], torch.bfloat16, torch.bfloat16)
+    params = a + b
+    opt = AdamW(params, lr=1e-3, state_bits=bits, max_grad_norm=0.5, master_weights=True)
+    for k, amount in enumerate((1.0, 1e-3)):
+        ga, gb = _make(sizes[:300], torch.float32, torch.float32, seed=5 + k)[1], _make(sizes[300:], torch.bfloat16, torch.bfloat16, seed=7 + k)[1]
+        grads = [g * amount for g in ga + gb]
+        for p, g in zip(params, grads):
+            p.grad = g
+        before = _snapshot(opt, params)
+        opt.step()
+        norm = math.sqrt(sum(float((g.double() ** 2).sum()) for g in grads))
+        assert abs(float(opt.grad_norm) - norm) <= 4 * E * norm
+        factor = min(1.0, 0.5 / (norm + 1e-6))
+        assert (factor < 1.0) == (k == 0)
+        _check_step(opt, before, params, grads, factor)
+
+
+def test_follows_torchs_adamw():
+    """Twenty steps beside torch's AdamW in float64: float32 rounding only."""
+    from fsgs.optim import AdamW
+    params, _ = _make((300, 5000), torch.float32, torch.float32)
+    twins = [torch.nn.Parameter(p.detach().double()) for p in params]
+    opt, ref = AdamW(params, lr=1e-3, weight_decay=0.05), torch.optim.AdamW(twins, lr=1e-3, weight_decay=0.05)
+    for k in range(20):
+        for p, q, g in zip(params, twins, _make((300, 5000), torch.float32, torch.float32, seed=k)[1]):
+            p.grad, q.grad = g, g.double()
+        opt.step()
+        ref.step()
+    for p, q in zip(params, twins):
+        # a step is below lr / (1 - b1) sqrt(1 - b2^t) / ... < 10 lr, each off by 40 e of that, and 4 e |p|
+        assert float((p.double() - q).abs().max()) <= 20 * (40 * E * 10 * 1e-3 + 4 * E * float(q.abs().max()))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_dropped_steps_change_nothing(bits):
+    from fsgs.optim import AdamW
+    params, grads = _make((700, 3), torch.float32, torch.float32)
+    for p, g in zip(params, grads):
+        p.grad = g
+    opt = AdamW(params, state_bits=bits)
+    one = torch.ones(1, device="cuda")
+    opt.step(gate=one, grad_scale=one)
+
+    def frozen():
+        return [t.clone().view(torch.uint8) for p in params for t in [p.detach().reshape(-1)] +
+                [v.reshape(-1) for v in opt.state[p].values()]]
+
+    before = frozen()
+    nan, inf = float("nan"), float("inf")
+    for gate, scale in ((0.0, None), (-1.0, None), (nan, None), (-inf, None), (None, 0.0), (None, nan), (None, inf),
+                        (None, -1.0), (1.0, nan), (0.0, 1.0)):
+        opt.step(gate=None if gate is None else one * gate, grad_scale=None if scale is None else one * scale)
+        assert all(torch.equal(x, y) for x, y in zip(before, frozen())), (gate, scale)
+    clipped = AdamW(params, state_bits=bits, max_grad_norm=1.0)
+    clipped.step()
+    clipped.load_state_dict(opt.state_dict())
+    state, opt = opt, clipped
+    before = frozen()
+    for bad in (nan, inf, -inf):
+        params[1].grad = torch.tensor([0.0, bad, 1.0], device="cuda")
+        opt.step()
+        assert not math.isfinite(float(opt.grad_norm))
+        assert all(torch.equal(x, y) for x, y in zip(before, frozen())), bad
+    params[1].grad = grads[1]
+    opt.step()
+    assert float(opt.state[params[0]]["step"]) == 2.0 and math.isfinite(float(opt.grad_norm))
+
+
+def test_a_bad_gradient_spoils_its_element_or_its_block():
+    from fsgs.optim import AdamW
+    for bits in (32, 8):
+        params, grads = _make((1000,), torch.float32, torch.float32)
+        grads[0][300] = float("nan")
+        params[0].grad = grads[0]
+        opt = AdamW(params, state_bits=bits)
+        opt.step()
+        assert torch.isnan(params[0]).nonzero().flatten().tolist() == [300]
+        bad = torch.isnan(_values(opt, params[0])[0]).nonzero().flatten().tolist()
+        assert bad == ([300] if bits == 32 else list(range(256, 512)))
+
+
+def test_eight_bit_moments_at_the_ends_of_the_range():
+    """Blocks of zeros, of denormals, with one huge or one tiny element among others; the largest element of a block
+    keeps its value to float32 rounding (its 8-bit value is 448 exactly)."""
+    from fsgs.optim import AdamW
+    g = torch.zeros(6 * B)
+    g[B:2 * B] = 1e-40
+    g[2 * B] = 1e18
+    g[2 * B + 1:3 * B] = 1e-3
+    g[3 * B:4 * B] = 1.0
+    g[3 * B + 5] = 1e-12
+    g[4 * B:5 * B] = -2.0 ** -60
+    p = torch.nn.Parameter(torch.zeros(6 * B, device="cuda"))
+    p.grad = g.cuda()
+    opt = AdamW([p], lr=1.0, weight_decay=0.0, state_bits=8, eps=1e-8)
+    opt.step()
+    m, s, ms, ss = (t.cpu() for t in _values(opt, p))
+    assert bool(torch.isfinite(p).all()) and bool(torch.isfinite(m).all()) and bool(torch.isfinite(s).all())
+    for lo, hi in ((0, 2 * B), (5 * B, 6 * B)):
+        assert not bool(m[lo:hi].any()) and not bool(s[lo:hi].any())
+    for i in (2 * B, 3 * B, 4 * B):
+        assert abs(float(m[i]) - 0.1 * float(g[i])) <= 8 * E * 0.1 * abs(float(g[i]))
+        assert abs(float(s[i]) - math.sqrt(1e-3) * abs(float(g[i]))) <= 16 * E * math.sqrt(1e-3) * abs(float(g[i]))
+    assert float(s[3 * B + 5]) == 2.0 ** -9 * float(ss[3 * B + 5]) > 0 and float(m[3 * B + 5]) == 0.0
+    # no eps: where both moments of an element are zero the update is 0 / 0 of the formula, elsewhere finite
+    assert bool((p.detach().cpu()[3 * B:4 * B] < 0).all())
+
+
+def test_a_captured_step_counts_its_replays():
+    from fsgs.optim import AdamW
+    for bits, clip in ((32, None), (8, 0.3)):
+        sizes = (5000, 17)
+        a, grads = _make(sizes, torch.float32, torch.float32)
+        b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+        fixed = [torch.zeros_like(g) for g in grads]
+        oa, ob = (AdamW(x, lr=1e-2, state_bits=bits, max_grad_norm=clip) for x in (a, b))
+        for p, g in zip(a, fixed):
+            p.grad = g
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="captured|capture"):
+            with torch.cuda.graph(graph):
+                oa.step()
+        oa.init_state()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            oa.step()
+        for k in range(4):
+            now = _make(sizes, torch.float32, torch.float32, seed=20 + k)[1]
+            for f, g, q in zip(fixed, now, b):
+                f.copy_(g)
+                q.grad = g
+            graph.replay()
+            ob.step()
+            for p, q in zip(a, b):
+                assert torch.equal(p, q) and float(oa.state[p]["step"]) == k + 1
+                for name, t in ob.state[q].items():
+                    assert torch.equal(oa.state[p][name].float(), t.float()), name
+
+
+def test_on_another_stream_and_with_changing_tensors():
+    """A side stream; gradients that come and go, are strided, or have new memory each step; a learning rate, a
+    parameter's storage and a state tensor that are replaced between steps."""
+    from fsgs.optim import AdamW
+    params, _ = _make((64, 513, 12), torch.float32, torch.float32)
+    opt = AdamW(params, lr=1e-2)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for k in range(6):
+            grads = _make((64, 513, 12), torch.float32, torch.float32, seed=40 + k)[1]
+            use = [0, 2] if k == 1 else [0, 1, 2]
+            grads[1] = torch.stack([grads[1], grads[1]], dim=1)[:, 1]       # stride 2
+            for i, (p, g) in enumerate(zip(params, grads)):
+                p.grad = None
+                if i in use:
+                    p.grad = g
+            if k == 2:
+                opt.param_groups[0]["lr"] = 5e-3
+            if k == 3:
+                params[0].data = params[0].data.clone()
+            if k == 4:
+                opt.state[params[2]]["exp_avg"] = opt.state[params[2]]["exp_avg"].clone()
+            if k == 5:
+                opt.param_groups[0]["betas"] = (0.7, 0.95)
+            sel = [params[i] for i in use]
+            before = _snapshot(opt, sel)
+            opt.step()
+            _check_step(opt, before, sel, [grads[i] for i in use])
+        assert float(opt.state[params[1]]["step"]) == 5 and float(opt.state[params[0]]["step"]) == 6
+    torch.cuda.current_stream().wait_stream(stream)
+
+
+def test_refusals_on_the_device():
+    from fsgs.optim import AdamW, grad_norm
+    p = torch.nn.Parameter(torch.zeros(4, 6, device="cuda").t())
+    p.grad = torch.zeros_like(p)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        AdamW([p]).step()
+    q = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+    q.grad = torch.ones(8, device="cuda")
+    opt = AdamW([q], max_grad_norm=1.0)
+    with pytest.raises(RuntimeError, match="grad_scale"):
+        opt.step(grad_scale=torch.ones(1, device="cuda"))
+    for bad in (torch.ones(1), torch.ones(2, device="cuda"), torch.ones(1, device="cuda", dtype=torch.float64)):
+        with pytest.raises(RuntimeError, match="gate"):
+            opt.step(gate=bad)
+    opt.step()
+    opt.state[q]["exp_avg"] = torch.zeros(7, device="cuda")
+    with pytest.raises(RuntimeError, match="exp_avg"):
+        opt.step()
+    del opt.state[q]["exp_avg"]
+    with pytest.raises(RuntimeError, match="exp_avg"):
+        opt.step()
+    r = torch.nn.Parameter(torch.zeros(8))
+    r.grad = torch.ones(8)
+    with pytest.raises(RuntimeError, match="one device"):
+        AdamW([torch.nn.Parameter(q.detach()), q, r]).step()
+    with pytest.raises(RuntimeError):
+        grad_norm([torch.ones(3, device="cuda"), torch.ones(3, device="cuda", dtype=torch.float64)])
+    with pytest.raises(RuntimeError):
+        grad_norm([torch.ones(3, device="cuda")], max_norm=0.0)
+
+
+def test_empty_tensors():
+    from fsgs.optim import AdamW, grad_norm
+    params, grads = _make((0, 5, 0, 300, 0), torch.float32, torch.float32)
+    for p, g in zip(params, grads):
+        p.grad = g
+    opt = AdamW(params, state_bits=8, max_grad_norm=100.0)
+    before = _snapshot(opt, params)
+    opt.step()
+    _check_step(opt, before, params, grads)
+    norm, factor = grad_norm([torch.zeros(0, device="cuda")], max_norm=1.0)
+    assert float(norm) == 0.0 and float(factor) == 1.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_norm_vs_double(dtype):
+    """Eight squares are added in float32 (their sum 8 e off at most), the rest in double: 4 e relative on the norm, 1 e
+    for its own rounding; the factor 3 roundings more."""
+    from fsgs.optim import grad_norm
+    gen = torch.Generator().manual_seed(1)
+    sizes = [1, 3, 8191, 8192, 8193, 100_001] + [k % 50 for k in range(500)]
+    ts = [(torch.randn(n + 3, generator=gen) * 10.0 ** (k % 5 - 3)).to(dtype).cuda()[k % 3:k % 3 + n] for k, n in enumerate(sizes)]
+    ts.append(torch.randn(40, 30, generator=gen).to(dtype).cuda().t())
+    want = math.sqrt(sum(float((t.double() ** 2).sum()) for t in ts))
+    norm, factor = grad_norm(ts, max_norm=0.25)
+    assert abs(float(norm) - want) <= 5 * E * want
+    assert abs(float(factor) - 0.25 / (want + 1e-6)) <= 9 * E * float(factor)
+    again, _ = grad_norm(ts, max_norm=0.25)
+    assert torch.equal(norm, again)
+    assert float(grad_norm(ts)[1]) == 1.0
+
+
+def test_norm_at_the_ends_of_the_range():
+    from fsgs.optim import grad_norm
+    big = torch.full((100_000,), 1e17, device="cuda")
+    norm, factor = grad_norm([big], max_norm=1.0)
+    assert abs(float(norm) / (1e17 * math.sqrt(1e5)) - 1) < 1e-6 and 0 < float(factor) < 1e-19
+    for bad in (float("inf"), float("nan")):
+        t = torch.ones(50_000, device="cuda")
+        t[31_234] = bad
+        norm, factor = grad_norm([t, torch.ones(3, device="cuda")], max_norm=1.0)
+        assert not math.isfinite(float(norm)) and float(factor) == 0.0
+    mixed = [torch.ones(9, device="cuda"), torch.ones(7, device="cuda", dtype=torch.bfloat16),
+             torch.ones(9, device="cuda", dtype=torch.float16)]
+    assert float(grad_norm(mixed)[0]) == 5.0
