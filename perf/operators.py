@@ -207,6 +207,8 @@ def _optimizer(s):
     case = s["case"]
     params = [torch.nn.Parameter(s["p"][a:a + n]) for a, n in s["spans"]]
     grads = [s["g"][a:a + n] for a, n in s["spans"]]
+    for p in params:
+        p.grad_dtype = s["g"].dtype
     groups = [dict(params=[p for p, d in zip(params, s["decays"]) if d == first], lr=lr, weight_decay=wd)
               for first, (lr, wd) in zip((True, False), s["groups"])]
     opt = AdamW([g for g in groups if g["params"]], betas=BETAS, eps=EPS, state_bits=case["bits"],
