@@ -589,6 +589,34 @@ int fsgs_lbs_weights_backward(int P, int K, int M, const float *d2, const int64_
     fsgs_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Balance of the Gaussians over the superpoints.  Additive: a term that keeps superpoints in use, beside the LBS weights
+ * of fast_2d_gs/network.py:498-521.  N Gaussians bound to K of M superpoints each, idx [N,K] (values outside 0 .. M-1:
+ * not bound), mask [N] bytes (optional; zero: the row does not count).  c_m = pairs that name superpoint m, T = sum c,
+ * n = rows that count;  L = M sum_m (c_m / T) P_m  with P_m = 1/n times
+ *   the sum of weights [N,K] over the pairs that name m    (pairs form; dL/dw_ik = M c_idx / (T n)), or
+ *   the sum of softmax(table row)_m over the rows          (table form; dL/dz_im = M/(T n) p_im (c_m - sum_e p_ie c_e)).
+ * The counts carry no gradient.  T = 0 or n = 0: L = 0 and zero gradients.  A table row of nothing but -infinity adds
+ * nothing to P.  What does not count has gradient 0 (added nothing), and its weights are not read into the sum.
+ *
+ * fsgs_balance_count: counts [M+2] = c, T, n; codes (optional, fsgs_balance_codes_bytes): the superpoint of every pair in
+ * 2 or 4 bytes, for fsgs_balance_pairs.  It prepares the workspace (16-byte aligned) for one call of the other two.
+ * scale and *upstream (device, optional) multiply the loss and the gradient.  loss (device, one float) and the gradient
+ * are both optional; without loss the workspace may be NULL.  accumulate: the gradient is added to g_weights.
+ * fsgs_balance_table: rows of M elements of `type`, row_stride / g_row_stride elements apart; g_table has the table's
+ * type.  Sums are added in a fixed order: the same inputs give the same bits.
+ * ---------------------------------------------------------------------------------------------- */
+size_t fsgs_balance_workspace_bytes(void);
+size_t fsgs_balance_codes_bytes(int64_t N, int K, int M);
+int fsgs_balance_count(int64_t N, int K, int M, const int64_t *idx, const uint8_t *mask, int64_t *counts, void *codes,
+    void *workspace, size_t workspace_bytes, fsgs_stream_t stream);
+int fsgs_balance_pairs(int64_t N, int K, int M, const float *weights, const void *codes, const int64_t *counts,
+    float scale, const float *upstream, float *loss, float *g_weights, int accumulate, void *workspace,
+    size_t workspace_bytes, fsgs_stream_t stream);
+int fsgs_balance_table(int64_t N, int M, int type, const void *table, int64_t row_stride, const uint8_t *mask,
+    const int64_t *counts, float scale, const float *upstream, float *loss, void *g_table, int64_t g_row_stride,
+    void *workspace, size_t workspace_bytes, fsgs_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
  * One view of a training iteration in two calls (forward, backward), all intermediates in one workspace.
  * Covers the body of the reference's per-view loop, fast_2d_gs/network.py:683-745 -- sigmoid of the opacity
  * logits (:611), superpoint LBS warp (:523-573, 630-645), GS_2D_fast_render -- and the backward autograd derives

@@ -1,0 +1,84 @@
+"""What the balance losses refuse (no GPU), and the layout of the argument structures of the training-step operators."""
+import re
+import os
+
+import pytest
+import torch
+
+from conftest import ROOT
+
+
+def test_refusals_without_a_device():
+    from fsgs.loss import balance_loss, balance_value_and_grad, table_balance_loss, table_balance_value_and_grad
+    w, idx = torch.ones(4, 2), torch.zeros(4, 2, dtype=torch.int64)
+    for call in (lambda: balance_loss(w, idx, 3), lambda: balance_value_and_grad(w, idx, 3),
+                 lambda: table_balance_loss(w, idx), lambda: table_balance_value_and_grad(w, idx)):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_entry_points_check_their_arguments():
+    """The C side refuses before anything is launched (no device is needed to see it)."""
+    from fsgs._lib import lib
+    L = lib()
+    head = L.fsgs_balance_workspace_bytes()
+    assert head % 16 == 0 and L.fsgs_balance_codes_bytes(10, 3, 512) == 60 and L.fsgs_balance_codes_bytes(10, 3, 65536) == 120
+    assert L.fsgs_balance_codes_bytes(0, 3, 512) == 0
+    ok = dict(N=4, K=2, M=3, idx=4096, mask=0, counts=4096, codes=4096, ws=4096, n=head)
+    def count(**kw):
+        a = dict(ok, **kw)
+        return L.fsgs_balance_count(a["N"], a["K"], a["M"], a["idx"], a["mask"], a["counts"], a["codes"], a["ws"], a["n"], None)
+    for bad in (dict(N=-1), dict(K=0), dict(M=0), dict(idx=0), dict(counts=0)):
+        assert count(**bad) == -1, bad
+    assert count(ws=0) == -3 and count(ws=4100) == -3 and count(n=head - 1) == -3 and count(N=1 << 40) == -5
+    pairs = lambda N=4, K=2, M=3, w=4096, codes=4096, counts=4096, loss=4096, g=0, ws=4096, n=head: L.fsgs_balance_pairs(  # noqa: E731
+        N, K, M, w, codes, counts, 1.0, None, loss, g, 0, ws, n, None)
+    assert pairs(w=0) == -1 and pairs(codes=0) == -1 and pairs(counts=0) == -1 and pairs(N=-1) == -1 and pairs(ws=0) == -3
+    assert pairs(loss=0, ws=0) == 0                                      # nothing asked for
+    table = lambda N=4, M=3, type=0, t=4096, rs=3, counts=4096, loss=4096, g=0, gs=3, ws=4096, n=head: L.fsgs_balance_table(  # noqa: E731
+        N, M, type, t, rs, None, counts, 1.0, None, loss, g, gs, ws, n, None)
+    for bad in (dict(N=-1), dict(M=0), dict(type=3), dict(t=0), dict(rs=2), dict(g=4096, gs=2), dict(counts=0)):
+        assert table(**bad) == -1, bad
+    assert table(ws=0) == -3 and table(n=5) == -3 and table(loss=0, ws=0) == 0 and table(N=1 << 40) == -5
+
+
+def test_step_entry_points_check_their_arguments():
+    from fsgs import _lib
+    L = _lib.lib()
+    def step(n=1, p=0, g=0, bits=32, b1=0.9, b2=0.999, eps=1e-8, ticket=4096, **kw):
+        t = (_lib.AdamWTensor * 1)()
+        for k in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step"):
+            setattr(t[0], k, 4096)
+        t[0].numel = 8
+        for k, v in kw.items():
+            setattr(t[0], k, v)
+        import ctypes
+        return L.fsgs_adamw_multi(n, ctypes.addressof(t), p, g, bits, b1, b2, eps, None, None, ticket, None)
+    for bad in (dict(n=-1), dict(p=3), dict(g=-1), dict(bits=16), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0), dict(ticket=None),
+                dict(param=None), dict(grad=None), dict(exp_avg=None), dict(exp_avg_sq=None), dict(step=None), dict(numel=-1),
+                dict(bits=8, exp_avg_scale=None), dict(bits=8, exp_avg_sq_scale=None)):
+        assert step(**bad) == -1, bad
+    for bad in (dict(p=0, g=1), dict(p=1, g=2), dict(p=2, g=1), dict(p=0, master=4096)):
+        assert step(**bad) == -2, bad
+    assert step(numel=1 << 50) == -5 and step(n=0) == 0
+    n = L.fsgs_grad_norm_workspace_bytes()
+    one = (_lib.NormTensor * 1)()
+    import ctypes
+    def norm(count=1, most=1.0, ws=4096, size=n, out=4096, **kw):
+        one[0].data, one[0].numel, one[0].type = 4096, 8, 0
+        for k, v in kw.items():
+            setattr(one[0], k, v)
+        return L.fsgs_grad_norm(count, ctypes.addressof(one), most, ws, size, out, None)
+    for bad in (dict(count=-1), dict(most=0.0), dict(most=float("nan")), dict(out=None), dict(data=None), dict(numel=-1), dict(type=3)):
+        assert norm(**bad) == -1, bad
+    assert norm(ws=None) == -3 and norm(ws=4100) == -3 and norm(size=n - 1) == -3
+
+
+def test_argument_structures_follow_the_header():
+    from fsgs import _lib
+    header = open(os.path.join(ROOT, "include", "fsgs.h")).read()
+    for cname, cls in (("fsgs_adamw_tensor", _lib.AdamWTensor), ("fsgs_norm_tensor", _lib.NormTensor)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (cname, cname), header, re.S).group(1)
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+        names = [d.split()[-1].lstrip("*") for d in body.split(";") if d.strip()]
+        assert names == [f[0] for f in cls._fields_], cname

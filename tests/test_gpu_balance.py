@@ -1,0 +1,216 @@
+"""The balance losses over the superpoints against the formulas in float64.
+
+Tolerances, e = 2^-24.  Pairs form: a share is rounded once, its product with the scale once: 2 e relative on a gradient
+(3 e where it is added to another, of both); the loss sums exact products of rounded terms in double: 3 e of the sum of
+their magnitudes, and e for itself.  Table form, a row with R the range of its values and d the length of a thread's
+column sum and the tree behind it: an exponential is 4 e + R e off (its argument is rounded to R e), sums d e more, so
+`inner` = sum p share is (R + d + 8) e sum p |share| off and a gradient k p (share - inner) is
+(R + d + 12) e k p (|share| + 2 sum p |share|) off, plus half a unit of a 16-bit type."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+HALF = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def _indices(N, K, M, gen, outside=0.0):
+    idx = (torch.rand(N, K, generator=gen) ** 2 * M).long().clamp_(max=M - 1)
+    if outside:
+        bad = torch.rand(N, K, generator=gen) < outside
+        idx[bad] = torch.tensor([-1, M, -2 ** 40, 2 ** 33, M + 7])[torch.randint(0, 5, (int(bad.sum()),), generator=gen)]
+    return idx
+
+
+def _counts(idx, M, mask):
+    on = (idx >= 0) & (idx < M)
+    if mask is not None:
+        on = on & mask[:, None]
+    c = torch.bincount(idx[on], minlength=M) if bool(on.any()) else torch.zeros(M, dtype=torch.int64)
+    return c, on, int(c.sum()), idx.shape[0] if mask is None else int(mask.sum())
+
+
+PAIRS = [(1, 1, 1, None, 0.0), (1, 3, 512, None, 0.0), (1000, 3, 512, None, 0.0), (1001, 8, 7, 0.3, 0.1),
+         (33, 5, 9000, 0.5, 0.2), (50_003, 3, 512, 0.02, 0.0), (20_000, 2, 70_000, 0.1, 0.1), (3000, 16, 65_535, None, 0.1),
+         (257, 4, 100, 1.0, 0.0), (64, 2, 10, None, 1.0), (5, 40, 3, 0.2, 0.2), (300_000, 8, 4096, 0.3, 0.01)]
+
+
+@pytest.mark.parametrize("N,K,M,masked,outside", PAIRS)
+def test_pairs_vs_formula(N, K, M, masked, outside):
+    from fsgs.loss import balance_loss, balance_value_and_grad
+    gen = torch.Generator().manual_seed(N + K)
+    idx = _indices(N, K, M, gen, outside)
+    w = torch.softmax(2 * torch.randn(N, K, generator=gen), dim=1)
+    mask = None if masked is None else torch.rand(N, generator=gen) >= masked
+    c, on, T, n = _counts(idx, M, mask)
+    share = torch.zeros(N, K, dtype=torch.float64)
+    if T and n:
+        share[on] = M * c.double()[idx[on]] / (T * n)
+    terms = share * w.double()
+    w[~on] = float("nan")                     # what does not count is not read into anything
+    dev = [t.cuda() if t is not None else None for t in (w, idx, mask)]
+    loss, grad, counts = balance_value_and_grad(dev[0], dev[1], M, mask=dev[2], weight=0.25)
+    assert torch.equal(counts.cpu(), c) and counts.dtype == torch.int64
+    assert abs(float(loss) - 0.25 * float(terms.sum())) <= 5 * E * 0.25 * float(terms.sum())
+    assert bool(((grad.cpu().double() - 0.25 * share).abs() <= 2 * E * 0.25 * share).all())
+    base = torch.randn(N, K, generator=gen)
+    into = base.cuda()
+    _, same, _ = balance_value_and_grad(dev[0], dev[1], M, mask=dev[2], weight=0.25, grad=into)
+    assert same is into
+    assert bool(((into.cpu().double() - (base.double() + 0.25 * share)).abs() <= 3 * E * (0.25 * share + base.abs())).all())
+    leaf = dev[0].clone().requires_grad_()
+    value, counts = balance_loss(leaf, dev[1], M, mask=dev[2])
+    (3.0 * value).backward()
+    assert torch.equal(counts.cpu(), c) and abs(float(value) - float(terms.sum())) <= 5 * E * float(terms.sum())
+    assert bool(((leaf.grad.cpu().double() - 3.0 * share).abs() <= 3 * E * 3.0 * share).all())
+
+
+def _table_reference(z, idx, mask):
+    M = z.shape[1]
+    c, _, T, n = _counts(idx, M, mask)
+    z = z.double()
+    p = torch.softmax(z, dim=1)
+    p[(z == -math.inf).all(dim=1)] = 0.0
+    if mask is not None:
+        p[~mask] = 0.0
+    if T == 0 or n == 0:
+        return c, 0.0, torch.zeros_like(p), torch.zeros_like(p)
+    f = M * c.double() / T / n
+    grad = p * (f - (p @ f)[:, None])
+    centred = (M * c.double() - T) / (T * n)
+    spread = (p * centred.abs()).sum(dim=1, keepdim=True)
+    fin = torch.where(torch.isfinite(z), z, z.new_tensor(0.0))
+    R = (z.amax(dim=1, keepdim=True).clamp(min=-1e30) - torch.where(torch.isfinite(z), z, z.new_tensor(1e30)).amin(dim=1, keepdim=True)).clamp(0, 200)
+    del fin
+    return c, float((p @ f).sum()), grad, (R + M / 32 + 16 + 12) * E * p * (centred.abs() + 2 * spread)
+
+
+TABLES = [(1, 1, 1, None), (1, 1, 2, None), (5, 2, 3, 0.5), (100, 3, 128, None), (100, 3, 129, 0.3), (77, 2, 333, 0.1),
+          (1000, 3, 512, None), (64, 4, 513, 0.2), (40, 8, 2048, None), (33, 2, 2049, 0.2), (20, 3, 8192, None),
+          (10, 3, 8193, 0.2), (6, 2, 20_011, None), (3000, 3, 512, 1.0)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,K,M,masked", TABLES)
+def test_table_vs_formula(N, K, M, masked, dtype):
+    from fsgs.loss import table_balance_loss, table_balance_value_and_grad
+    gen = torch.Generator().manual_seed(N * M)
+    idx = _indices(N, K, M, gen, 0.05 if N > 50 else 0.0)
+    z = (2 * torch.randn(N, M, generator=gen)).to(dtype)
+    mask = None if masked is None else torch.rand(N, generator=gen) >= masked
+    c, want, g64, tol = _table_reference(z, idx, mask)
+    dz, di, dm = z.cuda(), idx.cuda(), None if mask is None else mask.cuda()
+    loss, grad, counts = table_balance_value_and_grad(dz, di, mask=dm, weight=0.5)
+    assert torch.equal(counts.cpu(), c) and grad.dtype == dtype and grad.shape == z.shape
+    off = float(tol.sum()) + 4 * E * abs(want)
+    assert abs(float(loss) - 0.5 * want) <= 0.5 * off, (float(loss), want)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-40
+    close = lambda got, k: bool(((got.cpu().double() - k * g64).abs() <= k * tol + HALF[dtype] * (k * g64.abs() + k * tol) + tiny).all())  # noqa: E731
+    assert close(grad, 0.5)
+    leaf = dz.clone().requires_grad_()
+    value, counts = table_balance_loss(leaf, di, mask=dm)
+    (2.0 * value).backward()
+    assert torch.equal(counts.cpu(), c) and abs(float(value) - want) <= off and close(leaf.grad, 2.0)
+
+
+def test_table_rows_with_infinities_and_strides():
+    """Columns at -infinity, rows of nothing else, masked rows full of NaN; a table that is a slice of a wider one, one
+    with its rows apart, a transposed one."""
+    from fsgs.loss import table_balance_loss, table_balance_value_and_grad
+    gen = torch.Generator().manual_seed(3)
+    N, M = 60, 70
+    idx = _indices(N, 3, M, gen)
+    z = torch.randn(N, M, generator=gen)
+    z[:, 5] = -math.inf
+    z[7] = -math.inf
+    z[8, 1:] = -math.inf
+    z[9] = torch.finfo(torch.float32).min        # a row of nothing but the type's lowest value: all alike
+    mask = torch.ones(N, dtype=torch.bool)
+    mask[11] = False
+    c, want, g64, tol = _table_reference(z, idx, mask)
+    z[11] = math.nan
+    assert float(g64[7].abs().max()) == 0.0
+    wide = torch.full((N, M + 9), math.nan)
+    wide[:, 4:4 + M] = z
+    tall = torch.full((2 * N, M), math.nan)
+    tall[::2] = z
+    for t in (z.cuda(), wide.cuda()[:, 4:4 + M], tall.cuda()[::2], z.t().contiguous().cuda().t()):
+        loss, grad, counts = table_balance_value_and_grad(t, idx.cuda(), mask=mask.cuda())
+        assert torch.equal(counts.cpu(), c)
+        assert abs(float(loss) - want) <= float(tol.sum()) + 4 * E * want
+        assert bool(((grad.cpu().double() - g64).abs() <= tol + 1e-40).all())
+    z[20, 3] = math.nan                           # a NaN that counts reaches its row and the loss, and no other row
+    loss, grad, _ = table_balance_value_and_grad(z.cuda(), idx.cuda(), mask=mask.cuda())
+    assert math.isnan(float(loss)) and torch.isnan(grad).any(dim=1).nonzero().flatten().tolist() == [20]
+    # nobody bound: no loss, no gradient
+    loss, grad, counts = table_balance_value_and_grad(torch.randn(4, 9).cuda(), torch.full((4, 2), -1).cuda())
+    assert float(loss) == 0.0 and not bool(grad.any()) and not bool(counts.any())
+    leaf = torch.zeros(0, 9, device="cuda", requires_grad=True)
+    value, counts = table_balance_loss(leaf, torch.zeros(0, 2, dtype=torch.int64, device="cuda"))
+    value.backward()
+    assert float(value) == 0.0 and leaf.grad.shape == (0, 9)
+
+
+def test_gradients_against_differences():
+    """Central differences of the loss itself.  L = M/(T n) sum p c with c <= T: along one table entry its third
+    derivative is at most 6 M / n (that of a softmax probability is below 1, times c / T <= 1, six terms), so a step h is
+    off by h^2 M / n, and by the rounding of two losses of at most M, 2 x 8 e M / (2 h)."""
+    from fsgs.loss import balance_value_and_grad, table_balance_value_and_grad
+    gen = torch.Generator().manual_seed(1)
+    N, K, M, h = 5, 2, 6, 2.0 ** -6
+    idx = _indices(N, K, M, gen).cuda()
+    z, w = torch.randn(N, M, generator=gen).cuda(), torch.rand(N, K, generator=gen).cuda()
+    _, gz, _ = table_balance_value_and_grad(z, idx)
+    _, gw, _ = balance_value_and_grad(w, idx, M)
+    tol = h * h * M / N + 8 * E * M / h
+    for x, g, f in ((z, gz, lambda t: table_balance_value_and_grad(t, idx)[0]), (w, gw, lambda t: balance_value_and_grad(t, idx, M)[0])):
+        for k in range(x.numel()):
+            up, down = x.clone().view(-1), x.clone().view(-1)
+            up[k] += h
+            down[k] -= h
+            d = (float(f(up.view_as(x))) - float(f(down.view_as(x)))) / (2 * h)
+            assert abs(d - float(g.view(-1)[k])) <= tol, (k, d, float(g.view(-1)[k]))
+
+
+def test_repeats_bit_for_bit_and_in_a_graph():
+    from fsgs.loss import balance_value_and_grad, table_balance_value_and_grad
+    gen = torch.Generator().manual_seed(2)
+    N, K, M = 40_000, 3, 300
+    idx, w = _indices(N, K, M, gen).cuda(), torch.rand(N, K, generator=gen).cuda()
+    z = torch.randn(N, M, generator=gen).cuda()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for call in (lambda: balance_value_and_grad(w, idx, M), lambda: table_balance_value_and_grad(z, idx)):
+            first, second = call(), call()
+            assert all(torch.equal(a, b) for a, b in zip(first, second))
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                held = call()
+            old = idx.clone()
+            for k in range(3):
+                idx.copy_((old + 31 * k) % M)
+                graph.replay()
+                assert all(torch.equal(a, b) for a, b in zip(held, call()))
+            idx.copy_(old)
+    torch.cuda.current_stream().wait_stream(stream)
+
+
+def test_refusals():
+    from fsgs.loss import balance_loss, balance_value_and_grad, table_balance_loss
+    w, idx = torch.ones(4, 2, device="cuda"), torch.zeros(4, 2, dtype=torch.int64, device="cuda")
+    ok = torch.ones(4, dtype=torch.bool, device="cuda")
+    for call in (lambda: balance_loss(w.double(), idx, 3), lambda: balance_loss(w, idx.int(), 3), lambda: balance_loss(w, idx, 0),
+                 lambda: balance_loss(w, idx[:3], 3), lambda: balance_loss(w[:, :1], idx, 3), lambda: balance_loss(w, idx.cpu(), 3),
+                 lambda: balance_loss(w, idx, 3, mask=ok[:3]), lambda: balance_loss(w, idx, 3, mask=ok.float()),
+                 lambda: balance_loss(w, idx, 3, mask=ok.cpu()), lambda: balance_loss(w[0], idx, 3),
+                 lambda: balance_loss(torch.ones(4, 0, device="cuda"), idx[:, :0], 3),
+                 lambda: balance_value_and_grad(w, idx, 3, grad=torch.zeros(2, 4, device="cuda").t()),
+                 lambda: balance_value_and_grad(w, idx, 3, grad=torch.zeros(4, 2)),
+                 lambda: table_balance_loss(w.double(), idx), lambda: table_balance_loss(w[0], idx),
+                 lambda: table_balance_loss(torch.ones(4, 0, device="cuda"), idx), lambda: table_balance_loss(w, idx[:, 0])):
+        with pytest.raises(RuntimeError):
+            call()
