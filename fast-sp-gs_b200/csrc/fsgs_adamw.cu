@@ -23,15 +23,26 @@
 
 namespace fsgs {
 
+#ifndef MINB8
+#define MINB8 3
+#endif
+#ifndef MINB32
+#define MINB32 3
+#endif
+#ifndef NB
+#define NB 1
+#endif
 constexpr int kOptThreads = 256;
-constexpr int kOptBlock = FSGS_ADAMW_BLOCK;               // elements that share a scale: one warp, 8 per lane
-constexpr int kOptChunk = (kOptThreads / 32) * kOptBlock;  // elements of one pass of a thread block
-constexpr int kOptCapacity = 256;                          // tensors in one launch's argument table
-constexpr float kTop = 448.0f;                             // largest e4m3 value
-constexpr float kLow = 0.001953125f;                       // smallest positive e4m3 value, 2^-9
-constexpr float kTiny = 7.70371978e-34f;                   // 2^-110: below it 448 / max overflows and max / 448 is denormal
+constexpr int kOptWarps = kOptThreads / 32;
+constexpr int kOptBlock = FSGS_ADAMW_BLOCK;   // elements that share a scale: one warp, 8 consecutive ones per lane
+constexpr int kOptChunk = kOptWarps * NB * kOptBlock;  // elements of a thread block
+constexpr int kOptCapacity = 256;             // tensors in one launch's argument table
+constexpr float kTop = 448.0f;                // largest e4m3 value
+constexpr float kLow = 0.001953125f;          // smallest positive e4m3 value, 2^-9
+constexpr float kTiny = 7.70371978e-34f;      // 2^-110: below it 448 / max overflows and max / 448 is denormal
+constexpr float kSafe = 7.88860905e-31f;      // 2^-100: from here up the root below needs no special cases
 
-// ---- four consecutive elements of any of the types, as float32 ---------------------------------------------
+// ---- eight consecutive elements of any of the types ----------------------------------------------------------
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -42,74 +53,127 @@ __device__ __forceinline__ void from_f32(__nv_bfloat16 &d, float x) { d = __floa
 __device__ __forceinline__ void from_f32(__half &d, float x) { d = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(__nv_fp8_e4m3 &d, float x) { d.__x = __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
 
-__device__ __forceinline__ void load4(const float *p, float *x) {
-  const float4 v = *reinterpret_cast<const float4 *>(p);
-  x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+__device__ __forceinline__ unsigned bits_of(__nv_bfloat162 x) { return *reinterpret_cast<const unsigned *>(&x); }
+__device__ __forceinline__ unsigned bits_of(__half2 x) { return *reinterpret_cast<const unsigned *>(&x); }
+
+// As they lie in memory: 32, 16 or 8 bytes, one or two accesses per lane.
+template <typename T>
+struct Packed;
+template <>
+struct Packed<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float *p) {
+    a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+  }
+  __device__ __forceinline__ void get(float *x) const {
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  }
+  static __device__ __forceinline__ void store(float *p, const float *x) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+};
+template <>
+struct Packed<__nv_bfloat16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __nv_bfloat16 *p) { a = *reinterpret_cast<const uint4 *>(p); }
+  __device__ __forceinline__ void get(float *x) const {
+    const unsigned w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[2 * u] = __uint_as_float(w[u] << 16), x[2 * u + 1] = __uint_as_float(w[u] & 0xffff0000u);
+  }
+  static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float *x) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(bits_of(__floats2bfloat162_rn(x[0], x[1])), bits_of(__floats2bfloat162_rn(x[2], x[3])),
+                                               bits_of(__floats2bfloat162_rn(x[4], x[5])), bits_of(__floats2bfloat162_rn(x[6], x[7])));
+  }
+};
+template <>
+struct Packed<__half> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __half *p) { a = *reinterpret_cast<const uint4 *>(p); }
+  __device__ __forceinline__ void get(float *x) const {
+    const unsigned w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[u]));
+      x[2 * u] = f.x, x[2 * u + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ void store(__half *p, const float *x) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(bits_of(__floats2half2_rn(x[0], x[1])), bits_of(__floats2half2_rn(x[2], x[3])),
+                                               bits_of(__floats2half2_rn(x[4], x[5])), bits_of(__floats2half2_rn(x[6], x[7])));
+  }
+};
+template <>
+struct Packed<__nv_fp8_e4m3> {
+  uint2 a;
+  __device__ __forceinline__ void load(const __nv_fp8_e4m3 *p) { a = *reinterpret_cast<const uint2 *>(p); }
+  __device__ __forceinline__ void get(float *x) const {
+    const unsigned w[2] = {a.x, a.y};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((unsigned short) (w[u >> 1] >> (16 * (u & 1))), __NV_E4M3);
+      const float2 f = __half22float2(__half2(h));
+      x[2 * u] = f.x, x[2 * u + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ void store(__nv_fp8_e4m3 *p, const float *x) {
+    unsigned c[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) c[u] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * u], x[2 * u + 1]), __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<uint2 *>(p) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+  }
+};
+
+// the same eight elements one by one, for a tensor's last block and for addresses that are not aligned
+template <typename T>
+__device__ __forceinline__ void load_some(const T *p, long long left, float *x) {
+#pragma unroll
+  for (int u = 0; u < 8; ++u) x[u] = u < left ? to_f32(p[u]) : 0.0f;
 }
-__device__ __forceinline__ void load4(const __nv_bfloat16 *p, float *x) {
-  const uint2 v = *reinterpret_cast<const uint2 *>(p);
-  x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
-  x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
-}
-__device__ __forceinline__ void load4(const __half *p, float *x) {
-  const uint2 v = *reinterpret_cast<const uint2 *>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
-  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-}
-__device__ __forceinline__ float2 pair_f32(unsigned short v) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
-  return __half22float2(__half2(h));
-}
-__device__ __forceinline__ void load4(const __nv_fp8_e4m3 *p, float *x) {
-  const unsigned v = *reinterpret_cast<const unsigned *>(p);
-  const float2 a = pair_f32((unsigned short) v), b = pair_f32((unsigned short) (v >> 16));
-  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-}
-__device__ __forceinline__ void store4(float *p, const float *x) {
-  *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
-}
-__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float *x) {
-  const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
-}
-__device__ __forceinline__ void store4(__half *p, const float *x) {
-  const __half2 a = __floats2half2_rn(x[0], x[1]), b = __floats2half2_rn(x[2], x[3]);
-  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
-}
-__device__ __forceinline__ void store4(__nv_fp8_e4m3 *p, const float *x) {
-  const unsigned a = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
-  const unsigned b = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
-  *reinterpret_cast<unsigned *>(p) = a | (b << 16);
+template <typename T>
+__device__ __forceinline__ void store_some(T *p, long long left, const float *x) {
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    if (u < left) from_f32(p[u], x[u]);
 }
 
-// Lane's eight elements of a 256-element block: 4 lane + {0..3} and 128 + 4 lane + {0..3}, so that every access of a
-// warp covers consecutive memory.  `left`: elements from the block's start to the tensor's end.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, bool vec, long long left, int lane, float *x) {
-  if (vec && left >= kOptBlock) {
-    load4(p + 4 * lane, x);
-    load4(p + 128 + 4 * lane, x + 4);
-  } else {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int e = (u >> 2) * 128 + 4 * lane + (u & 3);
-      x[u] = e < left ? to_f32(p[e]) : 0.0f;
-    }
-  }
+// ---- two float32 operations in one instruction, each rounded as the single one is --------------------------
+
+struct Two {
+  unsigned long long v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
 }
-template <typename T>
-__device__ __forceinline__ void store8(T *p, bool vec, long long left, int lane, const float *x) {
-  if (vec && left >= kOptBlock) {
-    store4(p + 4 * lane, x);
-    store4(p + 128 + 4 * lane, x + 4);
-  } else {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int e = (u >> 2) * 128 + 4 * lane + (u & 3);
-      if (e < left) from_f32(p[e], x[u]);
-    }
-  }
+__device__ __forceinline__ Two both(float a) { return two(a, a); }
+__device__ __forceinline__ void split(Two t, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(t.v)); }
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_rsqrt(float x) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -122,146 +186,216 @@ struct AdamWEntry {
   void *m, *v;
   float *m_scale, *v_scale;
   float *master;
-  float *step;
   long long numel;
-  float lr, keep;  // keep = 1 - lr * weight_decay
+  float keep;  // 1 - lr * weight_decay
 };
 
 struct AdamWTable {
   AdamWEntry t[kOptCapacity];
   int chunk_start[kOptCapacity + 1];  // prefix sums of ceil(numel / kOptChunk)
-  uint8_t vec[kOptCapacity];          // every array aligned for four-element accesses
+  uint8_t vec[kOptCapacity];          // every array aligned for the packed accesses
   int n;
 };
 
 struct AdamWScalars {
   float b1, b2, c1, c2, eps;   // c = 1 - b, formed in double
-  double log_b1, log_b2;
-  const float *grad_scale, *gate;
-  int *ticket;
 };
 
-// index of the tensor that holds `chunk`: the last k with chunk_start[k] <= chunk
-template <typename Table>
-__device__ __forceinline__ int tensor_of(const Table &a, int chunk) {
-  int lo = 0, hi = a.n - 1;
+// index of the tensor that holds a block: the last k with start[k] <= block
+__device__ __forceinline__ int tensor_of(const int *start, int n, int block) {
+  int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (a.chunk_start[mid] <= chunk) lo = mid;
+    if (start[mid] <= block) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
 
-// max over the warp of non-negative floats, as their bit patterns order (a NaN comes out on top)
-__device__ __forceinline__ float warp_max_abs(const float *x) {
-  unsigned top = 0;
-#pragma unroll
-  for (int u = 0; u < 8; ++u) top = max(top, __float_as_uint(x[u]) & 0x7fffffffu);
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, top));
+// largest magnitude and smallest value of eight; a NaN among them is the largest
+__device__ __forceinline__ float top8(const float *x) {
+  float t;
+  asm("{\n\t.reg .f32 a, b, c;\n\t"
+      "max.NaN.abs.f32 a, %1, %2, %3;\n\tmax.NaN.abs.f32 b, %4, %5, %6;\n\t"
+      "max.NaN.abs.f32 c, %7, %8, a;\n\tmax.NaN.abs.f32 %0, b, c, c;\n\t}"
+      : "=f"(t) : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+  return t;
+}
+__device__ __forceinline__ float low8(const float *x) {
+  float t;
+  asm("{\n\t.reg .f32 a, b, c;\n\t"
+      "min.f32 a, %1, %2, %3;\n\tmin.f32 b, %4, %5, %6;\n\t"
+      "min.f32 c, %7, %8, a;\n\tmin.f32 %0, b, c, c;\n\t}"
+      : "=f"(t) : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+  return t;
 }
 
+// Roots of eight non-negative numbers.  In [2^-100, infinity): the hardware's approximate reciprocal root, one step of
+// Newton's method on the residual v - s^2 (exact in a fused multiply-add), which leaves the one final rounding.
+// `plain`: all eight lie there.
+__device__ __forceinline__ void roots(const float *v, float *s, bool plain) {
+  if (plain) {
+#pragma unroll
+    for (int u = 0; u < 8; u += 2) {
+      const Two r = two(fast_rsqrt(v[u]), fast_rsqrt(v[u + 1]));
+      const Two q = mul2(two(v[u], v[u + 1]), r), h = mul2(r, both(-0.5f));
+      split(fma2(fma2(q, q, two(-v[u], -v[u + 1])), h, q), s[u], s[u + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s[u] = __fsqrt_rn(v[u]);
+  }
+}
+
+// One block of 256 elements, eight per lane: m (decoded where 8 bits), v (sqrt(v) decoded where 8 bits), p in and out;
+// 8 bits: m and v come out as multiples of the block's new scales.
+template <bool EIGHT>
+__device__ __forceinline__ void update(const float *g, float *m, float *v, float *p, float scale, float ms, float vs,
+    const AdamWScalars &s, float step, float root, float keep, float *m_scale, float *v_scale, int lane) {
+#pragma unroll
+  for (int u = 0; u < 8; u += 2) {
+    const Two gs = mul2(two(g[u], g[u + 1]), both(scale));
+    Two a = two(m[u], m[u + 1]), b = two(v[u], v[u + 1]);
+    if (EIGHT) a = mul2(a, both(ms)), b = mul2(b, both(vs)), b = mul2(b, b);
+    split(add2(mul2(a, both(s.b1)), mul2(gs, both(s.c1))), m[u], m[u + 1]);
+    split(add2(mul2(b, both(s.b2)), mul2(mul2(gs, gs), both(s.c2))), v[u], v[u + 1]);
+  }
+  // a NaN among others passes: its own root is a NaN either way.  An infinite v passes with 8-bit moments only, where it
+  // spoils its block whatever its root is.
+  const bool plain = low8(v) >= kSafe && (EIGHT || top8(v) < INFINITY);
+  float q[8];
+  roots(v, q, plain);
+#pragma unroll
+  for (int u = 0; u < 8; u += 2) {
+    float d0, d1;
+    split(fma2(two(q[u], q[u + 1]), both(root), both(s.eps)), d0, d1);
+    const Two w = mul2(two(m[u], m[u + 1]), two(fast_rcp(d0), fast_rcp(d1)));
+    split(fma2(w, both(-step), mul2(two(p[u], p[u + 1]), both(keep))), p[u], p[u + 1]);
+  }
+  if (EIGHT) {
+    // maxima over the warp as the bit patterns of non-negative floats order; odd lanes go on with the one of sqrt(v)
+    const unsigned mt = __reduce_max_sync(0xffffffffu, __float_as_uint(top8(m)));
+    const unsigned vt = __reduce_max_sync(0xffffffffu, __float_as_uint(top8(q)));
+    const float top = __uint_as_float(lane & 1 ? vt : mt);
+    const bool zero = top < kTiny;  // a block of nothing but zeros (or denormals) has scale 0 and values 0
+    const float inv = zero ? 0.0f : __fmul_rn(__frcp_rn(top), kTop);
+    if (lane < 2) *(lane ? v_scale : m_scale) = zero ? 0.0f : __fmul_rn(top, 1.0f / kTop);
+    const float mr = __shfl_sync(0xffffffffu, inv, 0), vr = __shfl_sync(0xffffffffu, inv, 1);
+#pragma unroll
+    for (int u = 0; u < 8; u += 2) {
+      split(mul2(two(m[u], m[u + 1]), both(mr)), m[u], m[u + 1]);
+      split(mul2(two(q[u], q[u + 1]), both(vr)), v[u], v[u + 1]);
+    }
+    if (plain && vr > 0.0f) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = fmaxf(v[u], kLow);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = v[u] > 0.0f && v[u] < kLow ? kLow : v[u];
+    }
+  }
+}
+
+// what the update needs of a tensor's step count
+struct AdamWFactors {
+  float step, root;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+};
+
+struct AdamWBegin {
+  float *step[kOptCapacity];
+  float lr[kOptCapacity];
+  int n;
+};
+
+// Decides whether the step is taken, counts it and forms the bias corrections, one thread per tensor; scale_out < 0 tells
+// the kernel behind it that the step is dropped.
+__global__ void __launch_bounds__(kOptCapacity) adamw_begin_kernel(const __grid_constant__ AdamWBegin a, double log_b1, double log_b2,
+    const float *grad_scale, const float *gate, float *scale_out, AdamWFactors *out) {
+  const float scale = grad_scale ? *grad_scale : 1.0f;
+  const bool open = !(gate && !(*gate > 0.0f)) && scale > 0.0f && scale < INFINITY;
+  if (threadIdx.x == 0) *scale_out = open ? scale : -1.0f;
+  const int k = threadIdx.x;
+  if (!open || k >= a.n) return;
+  const double t = (double) *a.step[k] + 1.0;
+  *a.step[k] = (float) t;
+  out[k].step = (float) (a.lr[k] / (1.0 - exp(log_b1 * t)));
+  out[k].root = (float) (1.0 / sqrt(1.0 - exp(log_b2 * t)));
+}
+
+// One warp per block of 256 elements, NB blocks one after another with their loads ahead.  The grid covers the tensors
+// and leaves the order to the hardware, which hands out thread blocks as others finish: the memory in use at any moment
+// is one short stretch of every array.
 template <typename P, typename G, bool EIGHT, bool MASTER>
-__global__ void __launch_bounds__(kOptThreads) adamw_kernel(const __grid_constant__ AdamWTable a, const AdamWScalars s) {
+__global__ void __launch_bounds__(kOptThreads, EIGHT ? MINB8 : MINB32) adamw_kernel(const __grid_constant__ AdamWTable a, const AdamWScalars s,
+    const float *__restrict__ scale_in, const AdamWFactors *__restrict__ factors) {
   using S = typename std::conditional<EIGHT, __nv_fp8_e4m3, float>::type;
   using W = typename std::conditional<MASTER, float, P>::type;  // where the parameter's value is read from
-  __shared__ float s_step, s_root;
-  __shared__ int s_last;
-  float scale = 1.0f;
-  if (s.gate && !(*s.gate > 0.0f)) return;  // the same for every thread of the grid
-  if (s.grad_scale) {
-    scale = *s.grad_scale;
-    if (!(scale > 0.0f && scale < INFINITY)) return;
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int total = a.chunk_start[a.n];
-  int have = -1;
-  for (int chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
-    const int k = tensor_of(a, chunk);
-    const AdamWEntry &t = a.t[k];
-    const long long e0 = (long long) (chunk - a.chunk_start[k]) * kOptChunk + warp * kOptBlock;
-    const long long left = t.numel - e0;
-    const bool vec = a.vec[k] != 0;
-    float g[8], m[8], v[8], p[8];
-    if (left > 0) {
-      load8((const G *) t.grad + e0, vec, left, lane, g);
-      load8((const S *) t.m + e0, vec, left, lane, m);
-      load8((const S *) t.v + e0, vec, left, lane, v);
-      if (MASTER) load8((const float *) t.master + e0, vec, left, lane, p);
-      else load8((const W *) t.param + e0, vec, left, lane, p);
-      if (EIGHT) {
-        const float ms = t.m_scale[e0 / kOptBlock], vs = t.v_scale[e0 / kOptBlock];
+  const int lane = threadIdx.x & 31;
+  const int k = tensor_of(a.chunk_start, a.n, blockIdx.x);
+  const AdamWEntry &t = a.t[k];
+  const long long block = (long long) (blockIdx.x - a.chunk_start[k]) * (kOptWarps * NB) + (threadIdx.x >> 5);
+  const float scale = *scale_in;
+  const AdamWFactors f = factors[k];
+  const bool vec = a.vec[k] != 0;
+  Packed<G> ng[NB];
+  Packed<S> nm[NB], nv[NB];
+  Packed<W> nw[NB];
+  float nms[NB], nvs[NB];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) m[u] = __fmul_rn(m[u], ms), v[u] = __fmul_rn(v[u], vs), v[u] = __fmul_rn(v[u], v[u]);
-      }
+  for (int i = 0; i < NB; ++i) {
+    const long long b = block + i * kOptWarps, at = b * kOptBlock + 8 * lane;
+    if (vec && (b + 1) * kOptBlock <= t.numel) {
+      ng[i].load((const G *) t.grad + at), nm[i].load((const S *) t.m + at), nv[i].load((const S *) t.v + at);
+      nw[i].load((MASTER ? (const W *) t.master : (const W *) t.param) + at);
+      if (EIGHT) nms[i] = t.m_scale[b], nvs[i] = t.v_scale[b];
     }
-    if (k != have) {  // bias corrections of this tensor: two exponentials in double, by one thread of two warps each
-      __syncthreads();
-      if (threadIdx.x == 0) s_step = (float) (t.lr / (1.0 - exp(s.log_b1 * ((double) *t.step + 1.0))));
-      if (threadIdx.x == 32) s_root = (float) (1.0 / sqrt(1.0 - exp(s.log_b2 * ((double) *t.step + 1.0))));
-      __syncthreads();
-      have = k;
-    }
-    if (left <= 0) continue;
-    const float step = s_step, root = s_root, keep = t.keep;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float gs = __fmul_rn(g[u], scale);
-      m[u] = __fadd_rn(__fmul_rn(m[u], s.b1), __fmul_rn(gs, s.c1));
-      v[u] = __fadd_rn(__fmul_rn(v[u], s.b2), __fmul_rn(__fmul_rn(gs, gs), s.c2));
-      const float sq = __fsqrt_rn(v[u]);
-      p[u] = p[u] * keep - step * __fdividef(m[u], sq * root + s.eps);
-      if (EIGHT) v[u] = sq;
-    }
-    if (MASTER) store8(t.master + e0, vec, left, lane, p);
-    store8((P *) t.param + e0, vec, left, lane, p);
-    if (EIGHT) {
-      const float mt = warp_max_abs(m), vt = warp_max_abs(v);
-      // a block of nothing but zeros (or denormals) has scale 0 and values 0
-      const bool mz = mt < kTiny, vz = vt < kTiny;
-      const float mr = mz ? 0.0f : __fmul_rn(__frcp_rn(mt), kTop), vr = vz ? 0.0f : __fmul_rn(__frcp_rn(vt), kTop);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        m[u] = __fmul_rn(m[u], mr);
-        const float y = __fmul_rn(v[u], vr);
-        v[u] = y > 0.0f && y < kLow ? kLow : y;
-      }
-      if (lane == 0) {
-        t.m_scale[e0 / kOptBlock] = mz ? 0.0f : __fdiv_rn(mt, kTop);
-        t.v_scale[e0 / kOptBlock] = vz ? 0.0f : __fdiv_rn(vt, kTop);
-      }
-    }
-    store8((S *) t.m + e0, vec, left, lane, m);
-    store8((S *) t.v + e0, vec, left, lane, v);
   }
-  // the block that finishes last counts the step: by then every block has read the counts
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    s_last = atomicAdd(s.ticket, 1) == (int) gridDim.x - 1;
+  if (scale < 0.0f) return;  // dropped
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const long long b = block + i * kOptWarps, at = b * kOptBlock + 8 * lane, left = t.numel - at;
+    if (b * kOptBlock >= t.numel) return;
+    const bool whole = vec && (b + 1) * kOptBlock <= t.numel;
+    float g[8], m[8], v[8], p[8], ms = 1.0f, vs = 1.0f;
+    P *p_at = (P *) t.param + at;
+    S *m_at = (S *) t.m + at, *v_at = (S *) t.v + at;
+    W *w_at = MASTER ? (W *) t.master + at : (W *) p_at;
+    if (whole) {
+      ng[i].get(g), nm[i].get(m), nv[i].get(v), nw[i].get(p);
+      if (EIGHT) ms = nms[i], vs = nvs[i];
+    } else {  // a tensor's last block, or addresses that are not aligned
+      load_some((const G *) t.grad + at, left, g), load_some(m_at, left, m), load_some(v_at, left, v), load_some(w_at, left, p);
+      if (EIGHT) ms = t.m_scale[b], vs = t.v_scale[b];
+    }
+    __syncwarp();  // every lane has the old scales
+    update<EIGHT>(g, m, v, p, scale, ms, vs, s, f.step, f.root, t.keep, t.m_scale + b, t.v_scale + b, lane);
+    if (whole) {
+      if (MASTER) Packed<W>::store(w_at, p);
+      Packed<P>::store(p_at, p);
+      Packed<S>::store(m_at, m);
+      Packed<S>::store(v_at, v);
+    } else {
+      if (MASTER) store_some(w_at, left, p);
+      store_some(p_at, left, p);
+      store_some(m_at, left, m);
+      store_some(v_at, left, v);
+    }
   }
-  __syncthreads();
-  if (!s_last) return;
-  for (int k = threadIdx.x; k < a.n; k += kOptThreads) *a.t[k].step += 1.0f;
-  if (threadIdx.x == 0) *s.ticket = 0;
 }
 
 template <typename P, typename G, bool EIGHT, bool MASTER>
-static int adamw_launch(const AdamWTable &a, const AdamWScalars &s, cudaStream_t st) {
-  int dev = 0, sms = 0, per_sm = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, adamw_kernel<P, G, EIGHT, MASTER>, kOptThreads, 0) != cudaSuccess)
-    return FSGS_ERR_LAUNCH;
-  const int total = a.chunk_start[a.n], most = sms * (per_sm > 0 ? per_sm : 1);
-  adamw_kernel<P, G, EIGHT, MASTER><<<total < most ? (total > 0 ? total : 1) : most, kOptThreads, 0, st>>>(a, s);
+static int adamw_launch(const AdamWTable &a, const AdamWScalars &s, const float *scale, const AdamWFactors *f, cudaStream_t st) {
+  if (a.chunk_start[a.n] == 0) return FSGS_OK;
+  adamw_kernel<P, G, EIGHT, MASTER><<<a.chunk_start[a.n], kOptThreads, 0, st>>>(a, s, scale, f);
   FSGS_LAUNCH_CHECK();
   return FSGS_OK;
 }
 
 template <typename P, typename G>
-static int adamw_pick(bool eight, bool master, const AdamWTable &a, const AdamWScalars &s, cudaStream_t st) {
-  if (eight) return master ? adamw_launch<P, G, true, true>(a, s, st) : adamw_launch<P, G, true, false>(a, s, st);
-  return master ? adamw_launch<P, G, false, true>(a, s, st) : adamw_launch<P, G, false, false>(a, s, st);
+static int adamw_pick(bool eight, bool master, const AdamWTable &a, const AdamWScalars &s, const float *scale,
+    const AdamWFactors *f, cudaStream_t st) {
+  if (eight) return master ? adamw_launch<P, G, true, true>(a, s, scale, f, st) : adamw_launch<P, G, true, false>(a, s, scale, f, st);
+  return master ? adamw_launch<P, G, false, true>(a, s, scale, f, st) : adamw_launch<P, G, false, false>(a, s, scale, f, st);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -280,7 +414,8 @@ struct NormTable {
   int n;
 };
 
-constexpr int kNormChunk = 4 * kOptChunk;
+constexpr int kNormPart = kOptWarps * kOptBlock;   // elements of one pass of a thread block
+constexpr int kNormChunk = 4 * kNormPart;
 constexpr int kNormSlots = FSGS_GRAD_NORM_SLOTS;
 
 struct NormArgs {
@@ -299,11 +434,17 @@ template <typename T>
 __device__ __forceinline__ double chunk_squares(const T *p, bool vec, long long left, int warp, int lane) {
   double sum = 0.0;
 #pragma unroll
-  for (int j = 0; j < kNormChunk / kOptChunk; ++j) {
-    const long long e0 = (long long) j * kOptChunk + warp * kOptBlock;
-    if (left - e0 > 0) {
+  for (int j = 0; j < kNormChunk / kNormPart; ++j) {
+    const long long e0 = (long long) j * kNormPart + warp * kOptBlock + 8 * lane;
+    if (left > e0) {
       float x[8];
-      load8(p + e0, vec, left - e0, lane, x);
+      if (vec && left - e0 >= 8) {
+        Packed<T> w;
+        w.load(p + e0);
+        w.get(x);
+      } else {
+        load_some(p + e0, left - e0, x);
+      }
       float q = 0.0f;
 #pragma unroll
       for (int u = 0; u < 8; ++u) q = fmaf(x[u], x[u], q);
@@ -320,7 +461,7 @@ __global__ void __launch_bounds__(kOptThreads) grad_norm_kernel(const __grid_con
   const int total = a.chunk_start[a.n];
   double sum = 0.0;
   for (int chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
-    const int k = tensor_of(a, chunk);
+    const int k = tensor_of(a.chunk_start, a.n, chunk);
     const long long e0 = (long long) (chunk - a.chunk_start[k]) * kNormChunk;
     const long long left = a.t[k].numel - e0;
     const bool vec = a.vec[k] != 0;
@@ -359,17 +500,18 @@ __global__ void __launch_bounds__(kOptThreads) grad_norm_kernel(const __grid_con
   }
 }
 
-static int type_bytes(int type) { return type == FSGS_F32 ? 4 : 2; }
 static bool is_type(int type) { return type == FSGS_F32 || type == FSGS_BF16 || type == FSGS_F16; }
 
 }  // namespace fsgs
 
 using namespace fsgs;
 
+extern "C" size_t fsgs_adamw_workspace_bytes(void) { return 16 + sizeof(AdamWFactors) * kOptCapacity; }
+
 extern "C" int fsgs_adamw_multi(int n_tensors, const fsgs_adamw_tensor *tensors, int param_type, int grad_type,
-    int state_bits, double beta1, double beta2, float eps, const float *grad_scale, const float *gate, int32_t *ticket,
-    fsgs_stream_t stream) {
-  FSGS_REQUIRE(n_tensors >= 0 && (tensors || n_tensors == 0) && ticket && is_type(param_type) && is_type(grad_type));
+    int state_bits, double beta1, double beta2, float eps, const float *grad_scale, const float *gate, void *workspace,
+    size_t workspace_bytes, fsgs_stream_t stream) {
+  FSGS_REQUIRE(n_tensors >= 0 && (tensors || n_tensors == 0) && is_type(param_type) && is_type(grad_type));
   FSGS_REQUIRE(state_bits == 8 || state_bits == 32);
   FSGS_REQUIRE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0);
   if (param_type == FSGS_F32 ? grad_type != FSGS_F32 : grad_type != FSGS_F32 && grad_type != param_type) return FSGS_ERR_UNSUPPORTED;
@@ -381,39 +523,42 @@ extern "C" int fsgs_adamw_multi(int n_tensors, const fsgs_adamw_tensor *tensors,
     FSGS_REQUIRE(t.numel >= 0 && t.step && (t.master != nullptr) == master);
     FSGS_REQUIRE(t.numel == 0 || (t.param && t.grad && t.exp_avg && t.exp_avg_sq));
     FSGS_REQUIRE(t.numel == 0 || !eight || (t.exp_avg_scale && t.exp_avg_sq_scale));
+    if ((t.numel + kOptChunk - 1) / kOptChunk > INT32_MAX) return FSGS_ERR_LIMIT;
   }
-  AdamWScalars s;
-  s.b1 = (float) beta1, s.b2 = (float) beta2, s.c1 = (float) (1.0 - beta1), s.c2 = (float) (1.0 - beta2), s.eps = eps;
-  s.log_b1 = log(beta1), s.log_b2 = log(beta2);  // beta 0: -infinity, whose exponential is 0
-  s.grad_scale = grad_scale, s.gate = gate, s.ticket = ticket;
-  const uintptr_t pa = 4 * type_bytes(param_type) - 1, ga = 4 * type_bytes(grad_type) - 1, sa = eight ? 3 : 15;
+  if (!workspace || ((uintptr_t) workspace & 15) || workspace_bytes < fsgs_adamw_workspace_bytes()) return FSGS_ERR_WORKSPACE;
+  float *scale = (float *) workspace;
+  AdamWFactors *f = (AdamWFactors *) ((char *) workspace + 16);
+  const AdamWScalars s = {(float) beta1, (float) beta2, (float) (1.0 - beta1), (float) (1.0 - beta2), eps};
+  const double log_b1 = log(beta1), log_b2 = log(beta2);  // beta 0: -infinity, whose exponential is 0
+  cudaStream_t st = (cudaStream_t) stream;
   for (int first = 0; first < n_tensors;) {
     AdamWTable a;
+    AdamWBegin begin;
     a.n = 0, a.chunk_start[0] = 0;
-    int64_t chunks = 0;
     for (; first < n_tensors && a.n < kOptCapacity; ++first) {
       const fsgs_adamw_tensor &t = tensors[first];
-      const int64_t c = (t.numel + kOptChunk - 1) / kOptChunk;
-      if (c > INT32_MAX - (1 << 20)) return FSGS_ERR_LIMIT;
-      if (chunks + c > INT32_MAX - (1 << 20)) break;  // the rest in a launch of its own
+      const int64_t chunks = (t.numel + kOptChunk - 1) / kOptChunk;
+      if (a.chunk_start[a.n] + chunks > INT32_MAX) break;  // the rest in a launch of its own
       AdamWEntry &d = a.t[a.n];
       d.param = t.param, d.grad = t.grad, d.m = t.exp_avg, d.v = t.exp_avg_sq, d.m_scale = t.exp_avg_scale;
-      d.v_scale = t.exp_avg_sq_scale, d.master = t.master, d.step = t.step, d.numel = t.numel, d.lr = t.lr;
+      d.v_scale = t.exp_avg_sq_scale, d.master = t.master, d.numel = t.numel;
       d.keep = (float) (1.0 - (double) t.lr * (double) t.weight_decay);
-      a.vec[a.n] = !(((uintptr_t) t.param & pa) | ((uintptr_t) t.grad & ga) | ((uintptr_t) t.exp_avg & sa) |
-                     ((uintptr_t) t.exp_avg_sq & sa) | ((uintptr_t) t.master & 15));
-      chunks += c;
-      a.chunk_start[++a.n] = (int) chunks;
+      begin.step[a.n] = t.step, begin.lr[a.n] = t.lr;
+      a.vec[a.n] = !((((uintptr_t) t.param | (uintptr_t) t.grad | (uintptr_t) t.master) & 15) |
+                     (((uintptr_t) t.exp_avg | (uintptr_t) t.exp_avg_sq) & (eight ? 7 : 15)));
+      a.chunk_start[a.n + 1] = a.chunk_start[a.n] + (int) chunks;
+      begin.n = ++a.n;
     }
-    cudaStream_t st = (cudaStream_t) stream;
+    adamw_begin_kernel<<<1, kOptCapacity, 0, st>>>(begin, log_b1, log_b2, grad_scale, gate, scale, f);
+    FSGS_LAUNCH_CHECK();
     int rc;
-    if (param_type == FSGS_F32) rc = eight ? adamw_launch<float, float, true, false>(a, s, st) : adamw_launch<float, float, false, false>(a, s, st);
+    if (param_type == FSGS_F32) rc = eight ? adamw_launch<float, float, true, false>(a, s, scale, f, st) : adamw_launch<float, float, false, false>(a, s, scale, f, st);
     else if (param_type == FSGS_BF16)
-      rc = grad_type == FSGS_F32 ? adamw_pick<__nv_bfloat16, float>(eight, master, a, s, st)
-                                 : adamw_pick<__nv_bfloat16, __nv_bfloat16>(eight, master, a, s, st);
+      rc = grad_type == FSGS_F32 ? adamw_pick<__nv_bfloat16, float>(eight, master, a, s, scale, f, st)
+                                 : adamw_pick<__nv_bfloat16, __nv_bfloat16>(eight, master, a, s, scale, f, st);
     else
-      rc = grad_type == FSGS_F32 ? adamw_pick<__half, float>(eight, master, a, s, st)
-                                 : adamw_pick<__half, __half>(eight, master, a, s, st);
+      rc = grad_type == FSGS_F32 ? adamw_pick<__half, float>(eight, master, a, s, scale, f, st)
+                                 : adamw_pick<__half, __half>(eight, master, a, s, scale, f, st);
     if (rc != FSGS_OK) return rc;
   }
   return FSGS_OK;
@@ -440,7 +585,7 @@ extern "C" int fsgs_grad_norm(int n_tensors, const fsgs_norm_tensor *tensors, fl
       if (c > INT32_MAX - (1 << 20)) return FSGS_ERR_LIMIT;
       if (chunks + c > INT32_MAX - (1 << 20)) break;
       a.t[a.n].data = t.data, a.t[a.n].numel = t.numel, a.type[a.n] = (uint8_t) t.type;
-      a.vec[a.n] = ((uintptr_t) t.data & (4 * type_bytes(t.type) - 1)) == 0;
+      a.vec[a.n] = ((uintptr_t) t.data & 15) == 0;
       chunks += c;
       a.chunk_start[++a.n] = (int) chunks;
     }

@@ -130,7 +130,8 @@ SYMBOLS = {
     "fsgs_adam_masked": (c_int, [_vp, _vp, _vp, _vp, _vp, c_float, c_float, c_float, c_float, c_int64, c_int64, _vp]),
     "fsgs_adam_masked_multi": (c_int, [c_int, POINTER(AdamTensor), _vp, c_int64, c_float, c_float, _vp]),
     "fsgs_adam_masked_multi_fmask": (c_int, [c_int, POINTER(AdamTensor), _vp, c_int64, c_float, c_float, _vp]),
-    "fsgs_adamw_multi": (c_int, [c_int, _vp, c_int, c_int, c_int, c_double, c_double, c_float, _vp, _vp, _vp, _vp]),
+    "fsgs_adamw_workspace_bytes": (c_size_t, []),
+    "fsgs_adamw_multi": (c_int, [c_int, _vp, c_int, c_int, c_int, c_double, c_double, c_float, _vp, _vp, _vp, c_size_t, _vp]),
     "fsgs_grad_norm_workspace_bytes": (c_size_t, []),
     "fsgs_grad_norm": (c_int, [c_int, _vp, c_float, _vp, c_size_t, _vp, _vp]),
     "fsgs_balance_workspace_bytes": (c_size_t, []),

@@ -309,7 +309,7 @@ class AdamW(torch.optim.Optimizer):
         _need(max_grad_norm is None or max_grad_norm > 0, "AdamW: max_grad_norm must be positive")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         self.state_bits, self.master_weights, self.max_grad_norm = state_bits, bool(master_weights), max_grad_norm
-        self._plan = self._ticket = self._norm = None
+        self._plan = self._work = self._norm = None
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -396,7 +396,7 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._plan = None
-        self.__dict__.setdefault("_ticket", None)
+        self.__dict__.setdefault("_work", None)
         self.__dict__.setdefault("_norm", None)
 
     # ---- the step -----------------------------------------------------------------------------------------------
@@ -432,15 +432,15 @@ class AdamW(torch.optim.Optimizer):
             if self.max_grad_norm is not None:
                 _launch_norm(data, plan.numel, plan.grad_types, self.max_grad_norm, self._norm[1], self._norm[0])
                 grad_scale = self._norm[0][1:]
-            tail = (_ptr(grad_scale), _ptr(gate), _ptr(self._ticket[0]), _stream())
+            tail = (_ptr(grad_scale), _ptr(gate), _ptr(self._work[0]), self._work[0].numel(), _stream())
             for launch in plan.launches:
                 launch.table["grad"] = data if launch.whole else [data[i] for i in launch.rows]
                 check(lib().fsgs_adamw_multi(*launch.head, self.state_bits, *launch.scalars, *tail), "fsgs_adamw_multi")
 
     def _workspaces(self, device):
-        """Created once, zeroed once: the kernels leave their counters at zero.  Never replaced on the same device: a
-        captured step goes on using them."""
-        for name, wanted, make in (("_ticket", True, lambda: (torch.zeros(1, dtype=torch.int32, device=device),)),
+        """Created once and never replaced on the same device: a captured step goes on using them."""
+        for name, wanted, make in (("_work", True, lambda: (torch.empty(int(lib().fsgs_adamw_workspace_bytes()),
+                                                                       dtype=torch.uint8, device=device),)),
                                    ("_norm", self.max_grad_norm is not None,
                                     lambda: (torch.zeros(2, device=device), _norm_workspace(device)))):
             have = getattr(self, name)

@@ -120,8 +120,8 @@ int fsgs_adam_masked_multi_fmask(int n_tensors, const fsgs_adam_tensor *tensors 
  * parameters; for all tensors of a call or for none): the float32 parameter that is updated, param receives it rounded.
  * grad_scale (device, optional): c; gate (device, optional).  A call with *gate <= 0, or with *grad_scale <= 0 or not
  * finite, changes nothing, the step counts included.
- * step: one float per tensor, advanced by the call.  ticket: one int32 in device memory, zero before its first call;
- * calls leave it zero.  Calls that may run at the same time need tickets of their own.
+ * step: one float per tensor, advanced by the call.  workspace: 16-byte aligned, needs no preparation; calls that may
+ * run at the same time need workspaces of their own.
  * Tensors are contiguous; any alignment of the element type works, 16 bytes is the fast one.
  * ---------------------------------------------------------------------------------------------- */
 #define FSGS_F32 0
@@ -144,8 +144,9 @@ typedef struct fsgs_adamw_tensor {
 } fsgs_adamw_tensor;
 
 int fsgs_adamw_multi(int n_tensors, const fsgs_adamw_tensor *tensors /* host */, int param_type, int grad_type,
-    int state_bits, double beta1, double beta2, float eps, const float *grad_scale, const float *gate, int32_t *ticket,
-    fsgs_stream_t stream);
+    int state_bits, double beta1, double beta2, float eps, const float *grad_scale, const float *gate, void *workspace,
+    size_t workspace_bytes, fsgs_stream_t stream);
+size_t fsgs_adamw_workspace_bytes(void);
 
 /* out[0] = sqrt(sum of the squares of all elements of all tensors), out[1] = min(1, max_norm / (out[0] + 1e-6)), or 0
  * where the norm is not finite: the grad_scale of fsgs_adamw_multi.  Summed in a fixed order: the same gradients give

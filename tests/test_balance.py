@@ -45,7 +45,7 @@ def test_entry_points_check_their_arguments():
 def test_step_entry_points_check_their_arguments():
     from fsgs import _lib
     L = _lib.lib()
-    def step(n=1, p=0, g=0, bits=32, b1=0.9, b2=0.999, eps=1e-8, ticket=4096, **kw):
+    def step(n=1, p=0, g=0, bits=32, b1=0.9, b2=0.999, eps=1e-8, ws=4096, size=None, **kw):
         t = (_lib.AdamWTensor * 1)()
         for k in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step"):
             setattr(t[0], k, 4096)
@@ -53,14 +53,15 @@ def test_step_entry_points_check_their_arguments():
         for k, v in kw.items():
             setattr(t[0], k, v)
         import ctypes
-        return L.fsgs_adamw_multi(n, ctypes.addressof(t), p, g, bits, b1, b2, eps, None, None, ticket, None)
-    for bad in (dict(n=-1), dict(p=3), dict(g=-1), dict(bits=16), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0), dict(ticket=None),
+        return L.fsgs_adamw_multi(n, ctypes.addressof(t), p, g, bits, b1, b2, eps, None, None, ws,
+                                  L.fsgs_adamw_workspace_bytes() if size is None else size, None)
+    for bad in (dict(n=-1), dict(p=3), dict(g=-1), dict(bits=16), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0),
                 dict(param=None), dict(grad=None), dict(exp_avg=None), dict(exp_avg_sq=None), dict(step=None), dict(numel=-1),
                 dict(bits=8, exp_avg_scale=None), dict(bits=8, exp_avg_sq_scale=None)):
         assert step(**bad) == -1, bad
     for bad in (dict(p=0, g=1), dict(p=1, g=2), dict(p=2, g=1), dict(p=0, master=4096)):
         assert step(**bad) == -2, bad
-    assert step(numel=1 << 50) == -5 and step(n=0) == 0
+    assert step(numel=1 << 50) == -5 and step(n=0) == 0 and step(ws=None) == step(ws=4100) == step(size=15) == -3
     n = L.fsgs_grad_norm_workspace_bytes()
     one = (_lib.NormTensor * 1)()
     import ctypes
