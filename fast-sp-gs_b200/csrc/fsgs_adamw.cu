@@ -23,19 +23,9 @@
 
 namespace fsgs {
 
-#ifndef MINB8
-#define MINB8 3
-#endif
-#ifndef MINB32
-#define MINB32 3
-#endif
-#ifndef NB
-#define NB 1
-#endif
 constexpr int kOptThreads = 256;
 constexpr int kOptWarps = kOptThreads / 32;
 constexpr int kOptBlock = FSGS_ADAMW_BLOCK;   // elements that share a scale: one warp, 8 consecutive ones per lane
-constexpr int kOptChunk = kOptWarps * NB * kOptBlock;  // elements of a thread block
 constexpr int kOptCapacity = 256;             // tensors in one launch's argument table
 constexpr float kTop = 448.0f;                // largest e4m3 value
 constexpr float kLow = 0.001953125f;          // smallest positive e4m3 value, 2^-9
@@ -192,7 +182,7 @@ struct AdamWEntry {
 
 struct AdamWTable {
   AdamWEntry t[kOptCapacity];
-  int chunk_start[kOptCapacity + 1];  // prefix sums of ceil(numel / kOptChunk)
+  int chunk_start[kOptCapacity + 1];  // prefix sums of thread blocks
   uint8_t vec[kOptCapacity];          // every array aligned for the packed accesses
   int n;
 };
@@ -212,7 +202,7 @@ __device__ __forceinline__ int tensor_of(const int *start, int n, int block) {
   return lo;
 }
 
-// largest magnitude and smallest value of eight; a NaN among them is the largest
+// largest magnitude and largest value of eight; a NaN among them is the largest magnitude
 __device__ __forceinline__ float top8(const float *x) {
   float t;
   asm("{\n\t.reg .f32 a, b, c;\n\t"
@@ -221,29 +211,29 @@ __device__ __forceinline__ float top8(const float *x) {
       : "=f"(t) : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
   return t;
 }
-__device__ __forceinline__ float low8(const float *x) {
+__device__ __forceinline__ float high8(const float *x) {
   float t;
   asm("{\n\t.reg .f32 a, b, c;\n\t"
-      "min.f32 a, %1, %2, %3;\n\tmin.f32 b, %4, %5, %6;\n\t"
-      "min.f32 c, %7, %8, a;\n\tmin.f32 %0, b, c, c;\n\t}"
+      "max.f32 a, %1, %2, %3;\n\tmax.f32 b, %4, %5, %6;\n\t"
+      "max.f32 c, %7, %8, a;\n\tmax.f32 %0, b, c, c;\n\t}"
       : "=f"(t) : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
   return t;
 }
 
-// Roots of eight non-negative numbers.  In [2^-100, infinity): the hardware's approximate reciprocal root, one step of
-// Newton's method on the residual v - s^2 (exact in a fused multiply-add), which leaves the one final rounding.
-// `plain`: all eight lie there.
-__device__ __forceinline__ void roots(const float *v, float *s, bool plain) {
+// The negatives s = -sqrt(-v) of the roots of eight numbers -v.  From 2^-100 up: the hardware's approximate reciprocal
+// root, one step of Newton's method on the residual s^2 - (-v) (exact in a fused multiply-add), which leaves the one final
+// rounding.  `plain`: all eight lie there and are finite.  (Negatives, because the residual wants -v.)
+__device__ __forceinline__ void neg_roots(const float *v, float *s, bool plain) {
   if (plain) {
 #pragma unroll
     for (int u = 0; u < 8; u += 2) {
-      const Two r = two(fast_rsqrt(v[u]), fast_rsqrt(v[u + 1]));
-      const Two q = mul2(two(v[u], v[u + 1]), r), h = mul2(r, both(-0.5f));
-      split(fma2(fma2(q, q, two(-v[u], -v[u + 1])), h, q), s[u], s[u + 1]);
+      const Two r = two(fast_rsqrt(fabsf(v[u])), fast_rsqrt(fabsf(v[u + 1]))), n = two(v[u], v[u + 1]);
+      const Two q = mul2(n, r);
+      split(fma2(fma2(q, q, n), mul2(r, both(0.5f)), q), s[u], s[u + 1]);
     }
   } else {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) s[u] = __fsqrt_rn(v[u]);
+    for (int u = 0; u < 8; ++u) s[u] = -__fsqrt_rn(-v[u]);
   }
 }
 
@@ -258,19 +248,23 @@ __device__ __forceinline__ void update(const float *g, float *m, float *v, float
     Two a = two(m[u], m[u + 1]), b = two(v[u], v[u + 1]);
     if (EIGHT) a = mul2(a, both(ms)), b = mul2(b, both(vs)), b = mul2(b, b);
     split(add2(mul2(a, both(s.b1)), mul2(gs, both(s.c1))), m[u], m[u + 1]);
-    split(add2(mul2(b, both(s.b2)), mul2(mul2(gs, gs), both(s.c2))), v[u], v[u + 1]);
+    split(add2(mul2(b, both(-s.b2)), mul2(mul2(gs, gs), both(-s.c2))), v[u], v[u + 1]);  // -v'
   }
   // a NaN among others passes: its own root is a NaN either way.  An infinite v passes with 8-bit moments only, where it
   // spoils its block whatever its root is.
-  const bool plain = low8(v) >= kSafe && (EIGHT || top8(v) < INFINITY);
-  float q[8];
-  roots(v, q, plain);
+  const bool plain = high8(v) <= -kSafe && (EIGHT || top8(v) < INFINITY);
+  float q[8];  // -sqrt(v')
+  neg_roots(v, q, plain);
 #pragma unroll
   for (int u = 0; u < 8; u += 2) {
     float d0, d1;
-    split(fma2(two(q[u], q[u + 1]), both(root), both(s.eps)), d0, d1);
+    split(fma2(two(q[u], q[u + 1]), both(-root), both(s.eps)), d0, d1);
     const Two w = mul2(two(m[u], m[u + 1]), two(fast_rcp(d0), fast_rcp(d1)));
     split(fma2(w, both(-step), mul2(two(p[u], p[u + 1]), both(keep))), p[u], p[u + 1]);
+  }
+  if (!EIGHT) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = -v[u];
   }
   if (EIGHT) {
     // maxima over the warp as the bit patterns of non-negative floats order; odd lanes go on with the one of sqrt(v)
@@ -284,7 +278,7 @@ __device__ __forceinline__ void update(const float *g, float *m, float *v, float
 #pragma unroll
     for (int u = 0; u < 8; u += 2) {
       split(mul2(two(m[u], m[u + 1]), both(mr)), m[u], m[u + 1]);
-      split(mul2(two(q[u], q[u + 1]), both(vr)), v[u], v[u + 1]);
+      split(mul2(two(q[u], q[u + 1]), both(-vr)), v[u], v[u + 1]);
     }
     if (plain && vr > 0.0f) {
 #pragma unroll
@@ -322,14 +316,30 @@ __global__ void __launch_bounds__(kOptCapacity) adamw_begin_kernel(const __grid_
   out[k].root = (float) (1.0 / sqrt(1.0 - exp(log_b2 * t)));
 }
 
-// One warp per block of 256 elements, NB blocks one after another with their loads ahead.  The grid covers the tensors
-// and leaves the order to the hardware, which hands out thread blocks as others finish: the memory in use at any moment
-// is one short stretch of every array.
+// One warp per block of 256 elements, or per two blocks whose loads go out together.  The grid covers the tensors and
+// leaves the order to the hardware, which hands out thread blocks as others finish, each reading all that it needs before
+// it writes: the memory in use at any moment is one short stretch of every array, and DRAM pages are opened once.  Measured
+// (us; 116 M elements in float32 with float32 moments | bf16 with 8-bit moments, the norm before it included):
+//   this order                                                                  469 | 258
+//   a grid that fills the device, blocks interleaved (2 / 3 thread blocks an SM)  507 / 598 | 320
+//   every warp a run of its own                                                 588 | 269
+//   bulk copies through a ring in shared memory, 3 thread blocks an SM            - | 293, and 272 with no arithmetic at all
+//   this order, a warp's second block loaded while the first is computed        592 | 290
+// Two blocks per warp where an element brings 4 bytes of parameter and gradient (258 against 281: half the address and
+// argument work per element), one where it brings more (49 against 57 us for 17.4 M float32 elements: the second
+// block's registers push the loads behind the first block's stores).
 template <typename P, typename G, bool EIGHT, bool MASTER>
-__global__ void __launch_bounds__(kOptThreads, EIGHT ? MINB8 : MINB32) adamw_kernel(const __grid_constant__ AdamWTable a, const AdamWScalars s,
+struct PerWarp {
+  static constexpr int blocks = EIGHT && sizeof(G) + (MASTER ? 4 : sizeof(P)) <= 4 ? 2 : 1;
+  static constexpr int elements = kOptWarps * kOptBlock * blocks;  // of a thread block
+};
+
+template <typename P, typename G, bool EIGHT, bool MASTER>
+__global__ void __launch_bounds__(kOptThreads, EIGHT ? 4 : 3) adamw_kernel(const __grid_constant__ AdamWTable a, const AdamWScalars s,
     const float *__restrict__ scale_in, const AdamWFactors *__restrict__ factors) {
   using S = typename std::conditional<EIGHT, __nv_fp8_e4m3, float>::type;
   using W = typename std::conditional<MASTER, float, P>::type;  // where the parameter's value is read from
+  constexpr int NB = PerWarp<P, G, EIGHT, MASTER>::blocks;
   const int lane = threadIdx.x & 31;
   const int k = tensor_of(a.chunk_start, a.n, blockIdx.x);
   const AdamWEntry &t = a.t[k];
@@ -337,65 +347,104 @@ __global__ void __launch_bounds__(kOptThreads, EIGHT ? MINB8 : MINB32) adamw_ker
   const float scale = *scale_in;
   const AdamWFactors f = factors[k];
   const bool vec = a.vec[k] != 0;
+  const long long at = block * kOptBlock + 8 * lane;
+  const long long left = t.numel - block * kOptBlock;  // elements from the block's start on
+  const G *g_at = (const G *) t.grad + at;
+  S *m_at = (S *) t.m + at, *v_at = (S *) t.v + at;
+  P *p_at = (P *) t.param + at;
+  W *w_at = MASTER ? (W *) t.master + at : (W *) p_at;
+  float *ms_at = EIGHT ? t.m_scale + block : nullptr, *vs_at = EIGHT ? t.v_scale + block : nullptr;
+  constexpr int hop = kOptWarps * kOptBlock;
   Packed<G> ng[NB];
   Packed<S> nm[NB], nv[NB];
   Packed<W> nw[NB];
   float nms[NB], nvs[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
-    const long long b = block + i * kOptWarps, at = b * kOptBlock + 8 * lane;
-    if (vec && (b + 1) * kOptBlock <= t.numel) {
-      ng[i].load((const G *) t.grad + at), nm[i].load((const S *) t.m + at), nv[i].load((const S *) t.v + at);
-      nw[i].load((MASTER ? (const W *) t.master : (const W *) t.param) + at);
-      if (EIGHT) nms[i] = t.m_scale[b], nvs[i] = t.v_scale[b];
+    if (vec && left >= i * hop + kOptBlock) {
+      ng[i].load(g_at + i * hop), nm[i].load(m_at + i * hop), nv[i].load(v_at + i * hop), nw[i].load(w_at + i * hop);
+      if (EIGHT) nms[i] = ms_at[i * kOptWarps], nvs[i] = vs_at[i * kOptWarps];
     }
   }
   if (scale < 0.0f) return;  // dropped
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
-    const long long b = block + i * kOptWarps, at = b * kOptBlock + 8 * lane, left = t.numel - at;
-    if (b * kOptBlock >= t.numel) return;
-    const bool whole = vec && (b + 1) * kOptBlock <= t.numel;
+    const long long here = left - i * hop, some = here - 8 * lane;
+    if (here <= 0) return;
+    const bool whole = vec && here >= kOptBlock;
     float g[8], m[8], v[8], p[8], ms = 1.0f, vs = 1.0f;
-    P *p_at = (P *) t.param + at;
-    S *m_at = (S *) t.m + at, *v_at = (S *) t.v + at;
-    W *w_at = MASTER ? (W *) t.master + at : (W *) p_at;
     if (whole) {
       ng[i].get(g), nm[i].get(m), nv[i].get(v), nw[i].get(p);
       if (EIGHT) ms = nms[i], vs = nvs[i];
     } else {  // a tensor's last block, or addresses that are not aligned
-      load_some((const G *) t.grad + at, left, g), load_some(m_at, left, m), load_some(v_at, left, v), load_some(w_at, left, p);
-      if (EIGHT) ms = t.m_scale[b], vs = t.v_scale[b];
+      load_some(g_at + i * hop, some, g), load_some(m_at + i * hop, some, m), load_some(v_at + i * hop, some, v);
+      load_some(w_at + i * hop, some, p);
+      if (EIGHT) ms = ms_at[i * kOptWarps], vs = vs_at[i * kOptWarps];
     }
     __syncwarp();  // every lane has the old scales
-    update<EIGHT>(g, m, v, p, scale, ms, vs, s, f.step, f.root, t.keep, t.m_scale + b, t.v_scale + b, lane);
+    update<EIGHT>(g, m, v, p, scale, ms, vs, s, f.step, f.root, t.keep, EIGHT ? ms_at + i * kOptWarps : nullptr,
+                  EIGHT ? vs_at + i * kOptWarps : nullptr, lane);
     if (whole) {
-      if (MASTER) Packed<W>::store(w_at, p);
-      Packed<P>::store(p_at, p);
-      Packed<S>::store(m_at, m);
-      Packed<S>::store(v_at, v);
+      if (MASTER) Packed<W>::store(w_at + i * hop, p);
+      Packed<P>::store(p_at + i * hop, p);
+      Packed<S>::store(m_at + i * hop, m);
+      Packed<S>::store(v_at + i * hop, v);
     } else {
-      if (MASTER) store_some(w_at, left, p);
-      store_some(p_at, left, p);
-      store_some(m_at, left, m);
-      store_some(v_at, left, v);
+      if (MASTER) store_some(w_at + i * hop, some, p);
+      store_some(p_at + i * hop, some, p);
+      store_some(m_at + i * hop, some, m);
+      store_some(v_at + i * hop, some, v);
     }
   }
 }
 
+struct AdamWCall {
+  int n;
+  const fsgs_adamw_tensor *tensors;
+  AdamWScalars scalars;
+  double log_b1, log_b2;
+  const float *grad_scale, *gate;
+  float *scale;       // workspace: the factor, then the bias corrections
+  AdamWFactors *factors;
+  cudaStream_t stream;
+};
+
 template <typename P, typename G, bool EIGHT, bool MASTER>
-static int adamw_launch(const AdamWTable &a, const AdamWScalars &s, const float *scale, const AdamWFactors *f, cudaStream_t st) {
-  if (a.chunk_start[a.n] == 0) return FSGS_OK;
-  adamw_kernel<P, G, EIGHT, MASTER><<<a.chunk_start[a.n], kOptThreads, 0, st>>>(a, s, scale, f);
-  FSGS_LAUNCH_CHECK();
+static int adamw_run(const AdamWCall &c) {
+  constexpr int per = PerWarp<P, G, EIGHT, MASTER>::elements;
+  for (int k = 0; k < c.n; ++k)
+    if ((c.tensors[k].numel + per - 1) / per > INT32_MAX) return FSGS_ERR_LIMIT;
+  for (int first = 0; first < c.n;) {
+    AdamWTable a;
+    AdamWBegin begin;
+    a.n = 0, a.chunk_start[0] = 0;
+    for (; first < c.n && a.n < kOptCapacity; ++first) {
+      const fsgs_adamw_tensor &t = c.tensors[first];
+      const int64_t chunks = (t.numel + per - 1) / per;
+      if (a.chunk_start[a.n] + chunks > INT32_MAX) break;  // the rest in a launch of its own
+      AdamWEntry &d = a.t[a.n];
+      d.param = t.param, d.grad = t.grad, d.m = t.exp_avg, d.v = t.exp_avg_sq, d.m_scale = t.exp_avg_scale;
+      d.v_scale = t.exp_avg_sq_scale, d.master = t.master, d.numel = t.numel;
+      d.keep = (float) (1.0 - (double) t.lr * (double) t.weight_decay);
+      begin.step[a.n] = t.step, begin.lr[a.n] = t.lr;
+      a.vec[a.n] = !((((uintptr_t) t.param | (uintptr_t) t.grad | (uintptr_t) t.master) & 15) |
+                     (((uintptr_t) t.exp_avg | (uintptr_t) t.exp_avg_sq) & (EIGHT ? 7 : 15)));
+      a.chunk_start[a.n + 1] = a.chunk_start[a.n] + (int) chunks;
+      begin.n = ++a.n;
+    }
+    adamw_begin_kernel<<<1, kOptCapacity, 0, c.stream>>>(begin, c.log_b1, c.log_b2, c.grad_scale, c.gate, c.scale, c.factors);
+    FSGS_LAUNCH_CHECK();
+    if (a.chunk_start[a.n] == 0) continue;
+    adamw_kernel<P, G, EIGHT, MASTER><<<a.chunk_start[a.n], kOptThreads, 0, c.stream>>>(a, c.scalars, c.scale, c.factors);
+    FSGS_LAUNCH_CHECK();
+  }
   return FSGS_OK;
 }
 
 template <typename P, typename G>
-static int adamw_pick(bool eight, bool master, const AdamWTable &a, const AdamWScalars &s, const float *scale,
-    const AdamWFactors *f, cudaStream_t st) {
-  if (eight) return master ? adamw_launch<P, G, true, true>(a, s, scale, f, st) : adamw_launch<P, G, true, false>(a, s, scale, f, st);
-  return master ? adamw_launch<P, G, false, true>(a, s, scale, f, st) : adamw_launch<P, G, false, false>(a, s, scale, f, st);
+static int adamw_pick(bool eight, bool master, const AdamWCall &c) {
+  if (eight) return master ? adamw_run<P, G, true, true>(c) : adamw_run<P, G, true, false>(c);
+  return master ? adamw_run<P, G, false, true>(c) : adamw_run<P, G, false, false>(c);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -523,45 +572,18 @@ extern "C" int fsgs_adamw_multi(int n_tensors, const fsgs_adamw_tensor *tensors,
     FSGS_REQUIRE(t.numel >= 0 && t.step && (t.master != nullptr) == master);
     FSGS_REQUIRE(t.numel == 0 || (t.param && t.grad && t.exp_avg && t.exp_avg_sq));
     FSGS_REQUIRE(t.numel == 0 || !eight || (t.exp_avg_scale && t.exp_avg_sq_scale));
-    if ((t.numel + kOptChunk - 1) / kOptChunk > INT32_MAX) return FSGS_ERR_LIMIT;
   }
   if (!workspace || ((uintptr_t) workspace & 15) || workspace_bytes < fsgs_adamw_workspace_bytes()) return FSGS_ERR_WORKSPACE;
-  float *scale = (float *) workspace;
-  AdamWFactors *f = (AdamWFactors *) ((char *) workspace + 16);
-  const AdamWScalars s = {(float) beta1, (float) beta2, (float) (1.0 - beta1), (float) (1.0 - beta2), eps};
-  const double log_b1 = log(beta1), log_b2 = log(beta2);  // beta 0: -infinity, whose exponential is 0
-  cudaStream_t st = (cudaStream_t) stream;
-  for (int first = 0; first < n_tensors;) {
-    AdamWTable a;
-    AdamWBegin begin;
-    a.n = 0, a.chunk_start[0] = 0;
-    for (; first < n_tensors && a.n < kOptCapacity; ++first) {
-      const fsgs_adamw_tensor &t = tensors[first];
-      const int64_t chunks = (t.numel + kOptChunk - 1) / kOptChunk;
-      if (a.chunk_start[a.n] + chunks > INT32_MAX) break;  // the rest in a launch of its own
-      AdamWEntry &d = a.t[a.n];
-      d.param = t.param, d.grad = t.grad, d.m = t.exp_avg, d.v = t.exp_avg_sq, d.m_scale = t.exp_avg_scale;
-      d.v_scale = t.exp_avg_sq_scale, d.master = t.master, d.numel = t.numel;
-      d.keep = (float) (1.0 - (double) t.lr * (double) t.weight_decay);
-      begin.step[a.n] = t.step, begin.lr[a.n] = t.lr;
-      a.vec[a.n] = !((((uintptr_t) t.param | (uintptr_t) t.grad | (uintptr_t) t.master) & 15) |
-                     (((uintptr_t) t.exp_avg | (uintptr_t) t.exp_avg_sq) & (eight ? 7 : 15)));
-      a.chunk_start[a.n + 1] = a.chunk_start[a.n] + (int) chunks;
-      begin.n = ++a.n;
-    }
-    adamw_begin_kernel<<<1, kOptCapacity, 0, st>>>(begin, log_b1, log_b2, grad_scale, gate, scale, f);
-    FSGS_LAUNCH_CHECK();
-    int rc;
-    if (param_type == FSGS_F32) rc = eight ? adamw_launch<float, float, true, false>(a, s, scale, f, st) : adamw_launch<float, float, false, false>(a, s, scale, f, st);
-    else if (param_type == FSGS_BF16)
-      rc = grad_type == FSGS_F32 ? adamw_pick<__nv_bfloat16, float>(eight, master, a, s, scale, f, st)
-                                 : adamw_pick<__nv_bfloat16, __nv_bfloat16>(eight, master, a, s, scale, f, st);
-    else
-      rc = grad_type == FSGS_F32 ? adamw_pick<__half, float>(eight, master, a, s, scale, f, st)
-                                 : adamw_pick<__half, __half>(eight, master, a, s, scale, f, st);
-    if (rc != FSGS_OK) return rc;
-  }
-  return FSGS_OK;
+  AdamWCall c;
+  c.n = n_tensors, c.tensors = tensors;
+  c.scalars = {(float) beta1, (float) beta2, (float) (1.0 - beta1), (float) (1.0 - beta2), eps};
+  c.log_b1 = log(beta1), c.log_b2 = log(beta2);  // beta 0: -infinity, whose exponential is 0
+  c.grad_scale = grad_scale, c.gate = gate, c.stream = (cudaStream_t) stream;
+  c.scale = (float *) workspace, c.factors = (AdamWFactors *) ((char *) workspace + 16);
+  if (param_type == FSGS_F32) return eight ? adamw_run<float, float, true, false>(c) : adamw_run<float, float, false, false>(c);
+  if (param_type == FSGS_BF16)
+    return grad_type == FSGS_F32 ? adamw_pick<__nv_bfloat16, float>(eight, master, c) : adamw_pick<__nv_bfloat16, __nv_bfloat16>(eight, master, c);
+  return grad_type == FSGS_F32 ? adamw_pick<__half, float>(eight, master, c) : adamw_pick<__half, __half>(eight, master, c);
 }
 
 extern "C" size_t fsgs_grad_norm_workspace_bytes(void) { return 16 + sizeof(double) * kNormSlots; }

@@ -3,10 +3,11 @@
 There is no fallback: if the library cannot be loaded every operator raises.
 """
 import ctypes
+import importlib.util
 import os
 from ctypes import POINTER, Structure, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_void_p
 
-from .build import LIB
+from .build import HOST, LIB
 
 _vp = c_void_p
 
@@ -203,6 +204,27 @@ def lib():
             fn.restype, fn.argtypes = res, args
         _lib = handle
     return _lib
+
+
+_host = None
+
+
+def host():
+    """The host extension (``csrc/fsgs_host.cpp``); raises when it has not been built."""
+    global _host
+    if _host is None:
+        if not os.path.exists(HOST):
+            raise RuntimeError(f"{HOST} is missing: build it with `python -m fsgs.build`.")
+        spec = importlib.util.spec_from_file_location("_fsgs_host", HOST)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _host = module
+    return _host
+
+
+def address(name):
+    """Address of an entry point of the library."""
+    return ctypes.cast(getattr(lib(), name), c_void_p).value
 
 
 def check(status, what):

@@ -6,6 +6,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(PKG), "csrc")
 LIB = os.path.join(os.path.dirname(PKG), "lib", "libfsgs.so")
+HOST = os.path.join(os.path.dirname(PKG), "lib", "_fsgs_host.so")   # CPython extension over torch's headers
 SOURCES = ["fsgs_preprocess.cu", "fsgs_bin.cu", "fsgs_blend.cu", "fsgs_knn.cu", "fsgs_epilogue.cu", "fsgs_loss.cu", "fsgs_compact.cu", "fsgs_step.cu", "fsgs_motion.cu",
            "fsgs_adamw.cu", "fsgs_balance.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -13,16 +14,29 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
 
 
 def _stale():
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(HOST):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(HOST))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps.append(os.path.join(os.path.dirname(os.path.dirname(PKG)), "include", "fsgs.h"))
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _host_command():
+    """g++ command line of the host extension: torch's headers and libraries, this interpreter's headers."""
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"]]
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", os.path.join(CSRC, "fsgs_host.cpp"), "-o", HOST,
+            "-Wl,--no-as-needed", "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"] + ["-I" + d for d in inc]
+
+
 def build(force=False, verbose=False):
-    """Compile every CUDA source for sm_100a and link the shared library.  Returns the library path."""
+    """Compile every CUDA source for sm_100a and link the shared library, and compile the host extension beside it.  Returns
+    the library path."""
     if not force and not _stale():
         return LIB
     os.makedirs(os.path.dirname(LIB), exist_ok=True)
@@ -32,12 +46,14 @@ def build(force=False, verbose=False):
         cmd = ["nvcc", "-c", os.path.join(CSRC, src), "-o", obj] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else [])
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
         objs.append(obj)
+    cmd = _host_command()
+    procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     for cmd, p in procs:
         out, _ = p.communicate()
         if verbose or p.returncode:
             sys.stderr.write(out)
         if p.returncode:
-            raise RuntimeError("nvcc failed: " + " ".join(cmd))
+            raise RuntimeError("compilation failed: " + " ".join(cmd))
     subprocess.check_call(["nvcc", "-shared", "-o", LIB] + objs + ["-gencode", "arch=compute_100a,code=sm_100a",
                                                                   "-lcudart"])
     return LIB

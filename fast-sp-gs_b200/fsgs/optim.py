@@ -3,10 +3,10 @@ with every parameter group updated by ONE kernel launch instead of one launch pe
 parameters through the same kernel; ``AdamW`` over many dense tensors with moments in 32 or in 8 bits, clipping by the
 norm of all gradients (``grad_norm``) and a step count on the device."""
 import ctypes
-import operator
 
 import numpy as np
 import torch
+from torch.optim.optimizer import _global_optimizer_post_hooks, _global_optimizer_pre_hooks
 
 from . import _lib
 from ._lib import lib, check
@@ -139,21 +139,13 @@ def masked_adam_step(batch, visibility, N, b1=0.9, b2=0.999):
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # FSGS_F32, FSGS_BF16, FSGS_F16
 _BLOCK = 256                                                        # FSGS_ADAMW_BLOCK
-_data_ptr, _numel, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_STALE, _STRIDED = 1, 2                                             # answers of the host extension besides a status
 _table_type = np.dtype([(n, np.float32 if t is ctypes.c_float else np.int64) for n, t in _lib.AdamWTensor._fields_])
-_norm_type = np.dtype([("data", np.int64), ("numel", np.int64), ("type", np.int64)])
-assert _table_type.itemsize == ctypes.sizeof(_lib.AdamWTensor) and _norm_type.itemsize == ctypes.sizeof(_lib.NormTensor)
+assert _table_type.itemsize == ctypes.sizeof(_lib.AdamWTensor)
 
 
 def _norm_workspace(device):
     return torch.zeros(int(lib().fsgs_grad_norm_workspace_bytes()), dtype=torch.uint8, device=device)
-
-
-def _launch_norm(data, numel, types, max_norm, workspace, out):
-    table = np.empty(len(data), _norm_type)
-    table["data"], table["numel"], table["type"] = data, numel, types
-    check(lib().fsgs_grad_norm(len(data), table.ctypes.data, max_norm, _ptr(workspace), workspace.numel(), _ptr(out),
-                               _stream()), "fsgs_grad_norm")
 
 
 def grad_norm(tensors, max_norm=None):
@@ -162,37 +154,31 @@ def grad_norm(tensors, max_norm=None):
     where the norm is not finite.  Two float32 device scalars, one launch (per 256 tensors) and no synchronisation; the
     factor can be given to ``AdamW.step(grad_scale=...)``.  Summed in a fixed order: the same gradients give the same
     bits."""
-    tensors = [t.detach() for t in tensors]
-    _need(len(tensors) > 0, "grad_norm: no tensors")
+    tensors = list(tensors)
+    _need(len(tensors) > 0 and isinstance(tensors[0], torch.Tensor) and tensors[0].is_cuda,
+          "grad_norm: dense float32, bfloat16 or float16 CUDA tensors on one device")
     _need(max_norm is None or max_norm > 0, "grad_norm: max_norm must be positive")
     device = tensors[0].device
-    for t in tensors:
-        _need(t.is_cuda and t.device == device and t.dtype in _TYPES and t.layout == torch.strided,
-              "grad_norm: dense float32, bfloat16 or float16 CUDA tensors on one device")
-    tensors = [t.contiguous() for t in tensors]
     with _on_device(device):
-        out = torch.empty(2, device=device)
-        _launch_norm(list(map(_data_ptr, tensors)), list(map(_numel, tensors)), [_TYPES[t.dtype] for t in tensors],
-                     float("inf") if max_norm is None else float(max_norm), _norm_workspace(device), out)
+        out, work = torch.empty(2, device=device), _norm_workspace(device)
+        args = (_lib.address("fsgs_grad_norm"), float("inf") if max_norm is None else float(max_norm), work.data_ptr(),
+                work.numel(), out.data_ptr(), _stream().value or 0)
+        rc = _lib.host().norm(tensors, *args)
+        if rc == _STRIDED:
+            tensors = [t.detach().contiguous() for t in tensors]
+            rc = _lib.host().norm(tensors, *args)
+        check(rc, "fsgs_grad_norm")
     return out[0], out[1]
 
 
-class _Launch:
-    """The tensors of one ``fsgs_adamw_multi`` call: those that share their types, betas and eps."""
-
-    def __init__(self, rows, whole, param_type, grad_type, betas, eps):
-        self.rows, self.whole = rows, whole     # places in the plan's lists; whether they are all of them
-        self.table = np.zeros(len(rows), _table_type)
-        self.head = (len(rows), self.table.ctypes.data, param_type, grad_type)
-        self.scalars = (float(betas[0]), float(betas[1]), float(eps))
-
-
 class _Plan:
-    """The argument tables of a step for one list of parameters.  ``matches`` reads every address and length anew: a
-    plan is used only while the parameters, their state tensors and their places are what it was made from."""
+    """The argument tables of a step for one list of parameters, and what the host extension compares them with: it reads
+    every address, length and type of the parameters, gradients and states anew each step, and a plan is used only while
+    they are what it was made from."""
 
-    def __init__(self, opt, params):
-        self.params, self.device = params, params[0].device
+    def __init__(self, opt):
+        self.params = params = [p for g in opt.param_groups for p in g["params"] if p.grad is not None]
+        self.device = params[0].device
         group_of = {id(p): k for k, g in enumerate(opt.param_groups) for p in g["params"]}
         self.groups = [group_of[id(p)] for p in params]
         for p in params:
@@ -200,80 +186,55 @@ class _Plan:
             _need(p.is_contiguous() and p.dtype in _TYPES, "AdamW: contiguous float32, bfloat16 or float16 parameters")
             _need(p.grad.layout == torch.strided and (p.grad.dtype == p.dtype or p.grad.dtype == torch.float32),
                   "AdamW: a dense gradient of its parameter's type or float32")
-        self.numel = list(map(_numel, params))
-        self.grad_dtypes = [p.grad.dtype for p in params]
-        self.grad_types = [_TYPES[t] for t in self.grad_dtypes]
-        self.states = [opt._state_of(p) for p in params]
-        self.names = [opt._names(p) for p in params]
-        self.read = [operator.itemgetter(*n) for n in self.names]
-        for p, st, names in zip(params, self.states, self.names):
-            for name in names:
+            _need(p.grad.numel() == p.numel(), "AdamW: a gradient has another size than its parameter")
+        states, names = [opt._state_of(p) for p in params], [opt._names(p) for p in params]
+        for p, st, wanted in zip(params, states, names):
+            for name in wanted:
                 _need(name in st, f"AdamW: a parameter's state has no {name}")
                 t = st[name]
-                want = (p.numel() + _BLOCK - 1) // _BLOCK if name.endswith("_scale") else 1 if name == "step" else p.numel()
+                size = (p.numel() + _BLOCK - 1) // _BLOCK if name.endswith("_scale") else 1 if name == "step" else p.numel()
                 kind = torch.float8_e4m3fn if opt.state_bits == 8 and name in ("exp_avg", "exp_avg_sq_root") else torch.float32
-                _need(t.device == self.device and t.dtype == kind and t.numel() == want and t.is_contiguous(),
-                      f"AdamW: the state {name} must be a contiguous {kind} tensor of {want} elements on {self.device}")
-        self.settings_key = self._settings(opt)
-        self.addresses = self._addresses(params)
+                _need(t.device == self.device and t.dtype == kind and t.numel() == size and t.is_contiguous(),
+                      f"AdamW: the state {name} must be a contiguous {kind} tensor of {size} elements on {self.device}")
+        self.settings = self.current_settings(opt)
         kinds = {}
         for i, (p, k) in enumerate(zip(params, self.groups)):
             g = opt.param_groups[k]
-            key = (_TYPES[p.dtype], self.grad_types[i], "master" in self.names[i], tuple(g["betas"]), g["eps"])
+            key = (_TYPES[p.dtype], _TYPES[p.grad.dtype], "master" in names[i], tuple(g["betas"]), g["eps"])
             kinds.setdefault(key, []).append(i)
-        self.launches = []
+        self.launches, entries = [], [None] * len(params)
         for (param_type, grad_type, _, betas, eps), rows in kinds.items():
-            launch = _Launch(rows, len(rows) == len(params), param_type, grad_type, betas, eps)
-            t = launch.table
-            pick = lambda name: [self.states[i][name].data_ptr() if name in self.names[i] else 0 for i in rows]  # noqa: E731
-            t["param"], t["numel"] = [params[i].data_ptr() for i in rows], [self.numel[i] for i in rows]
-            t["step"], t["exp_avg"], t["master"] = pick("step"), pick("exp_avg"), pick("master")
-            t["exp_avg_sq"] = pick("exp_avg_sq" if opt.state_bits == 32 else "exp_avg_sq_root")
-            t["exp_avg_scale"], t["exp_avg_sq_scale"] = pick("exp_avg_scale"), pick("exp_avg_sq_root_scale")
-            self.launches.append(launch)
-        self._rates(opt)
+            t = np.zeros(len(rows), _table_type)
+            address = lambda name: [states[i][name].data_ptr() if name in names[i] else 0 for i in rows]  # noqa: E731
+            t["param"], t["numel"] = [params[i].data_ptr() for i in rows], [params[i].numel() for i in rows]
+            t["step"], t["exp_avg"], t["master"] = address("step"), address("exp_avg"), address("master")
+            t["exp_avg_sq"] = address("exp_avg_sq" if opt.state_bits == 32 else "exp_avg_sq_root")
+            t["exp_avg_scale"], t["exp_avg_sq_scale"] = address("exp_avg_scale"), address("exp_avg_sq_root_scale")
+            self.launches.append((rows, t, (len(rows), t.ctypes.data, param_type, grad_type, opt.state_bits, float(betas[0]),
+                                            float(betas[1]), float(eps))))
+            for k, i in enumerate(rows):
+                entries[i] = (params[i], self.groups[i], states[i], names[i], t.ctypes.data + k * _table_type.itemsize)
+        self.rates(opt)
+        self.handle = _lib.host().plan(entries, [l[2] for l in self.launches])
 
     @staticmethod
-    def _settings(opt):
-        return [(len(g["params"]), tuple(g["betas"]), g["eps"], float(g["lr"]), g["weight_decay"]) for g in opt.param_groups]
+    def current_settings(opt):
+        return [(float(g["lr"]), float(g["weight_decay"]), *g["betas"], g["eps"]) for g in opt.param_groups]
 
-    def _rates(self, opt):
-        lr, wd = ([float(g[k]) for g in opt.param_groups] for k in ("lr", "weight_decay"))
-        for launch in self.launches:
-            launch.table["lr"] = [lr[self.groups[i]] for i in launch.rows]
-            launch.table["weight_decay"] = [wd[self.groups[i]] for i in launch.rows]
-
-    def _addresses(self, params):
-        out = list(map(_data_ptr, params))
-        for read, st in zip(self.read, self.states):
-            out.extend(map(_data_ptr, read(st)))
-        return out
-
-    def matches(self, opt, params):
-        if len(params) != len(self.params) or not all(map(operator.is_, params, self.params)):
-            return False
-        if not all(map(operator.is_, map(opt.state.get, params), self.states)):
-            return False
-        try:
-            if self._addresses(params) != self.addresses or list(map(_numel, params)) != self.numel:
+    def follow(self, opt):
+        """Take over changed learning rates and weight decays; False where betas or eps changed."""
+        now = self.current_settings(opt)
+        if now != self.settings:
+            if [s[2:] for s in now] != [s[2:] for s in self.settings]:
                 return False
-        except KeyError:
-            return False
-        settings = self._settings(opt)
-        if settings != self.settings_key:
-            if [s[:3] for s in settings] != [s[:3] for s in self.settings_key]:
-                return False
-            self.settings_key = settings
-            self._rates(opt)
+            self.settings = now
+            self.rates(opt)
         return True
 
-    def gradients(self, grads):
-        """Addresses of the gradients, contiguous (``self.kept`` holds copies until the next step)."""
-        self.kept = None
-        if not all(map(_is_contiguous, grads)):
-            grads = self.kept = [g.contiguous() for g in grads]
-        _need(list(map(_numel, grads)) == self.numel, "AdamW: a gradient has another size than its parameter")
-        return list(map(_data_ptr, grads))
+    def rates(self, opt):
+        lr, wd = ([float(g[k]) for g in opt.param_groups] for k in ("lr", "weight_decay"))
+        for rows, table, _ in self.launches:
+            table["lr"], table["weight_decay"] = ([v[self.groups[i]] for i in rows] for v in (lr, wd))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -400,42 +361,64 @@ class AdamW(torch.optim.Optimizer):
         self.__dict__.setdefault("_norm", None)
 
     # ---- the step -----------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, gate=None, grad_scale=None):
         """``gate``: a one-element float32 device tensor; the step is applied where it is > 0.  ``grad_scale``: a
         one-element float32 device tensor that multiplies every gradient; the step is dropped where it is not positive
         and finite (not together with ``max_grad_norm``, which makes its own)."""
+        if self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _global_optimizer_pre_hooks or \
+                _global_optimizer_post_hooks or torch.autograd._profiler_enabled():
+            return _hooked_step(self, gate, grad_scale)
         self.step_gated(gate, grad_scale)
 
+    step.hooked = True   # the base class would wrap it: 10 us per step for hooks that are looked for above
+
     def step_gated(self, gate=None, grad_scale=None):
-        """The body of ``step`` without the hook layers that ``torch.optim.Optimizer`` wraps around it."""
-        params, grads = [], []
-        for group in self.param_groups:
-            for p in group["params"]:
-                g = p.grad
-                if g is not None:
-                    params.append(p)
-                    grads.append(g)
-        if not params:
-            return
+        """The body of ``step``, without hooks."""
+        for t in (gate, grad_scale):
+            _need(t is None or (t.is_cuda and t.numel() == 1 and t.dtype == torch.float32),
+                  "AdamW: gate and grad_scale are one-element float32 tensors on the parameters' device")
         _need(grad_scale is None or self.max_grad_norm is None, "AdamW: grad_scale together with max_grad_norm")
         plan = self._plan
-        if plan is None or [g.dtype for g in grads] != plan.grad_dtypes or not plan.matches(self, params):
-            plan = self._plan = _Plan(self, params)
+        if plan is None or not plan.follow(self):
+            plan = self._new_plan()
+            if plan is None:
+                return
+        rc = self._run(plan, gate, grad_scale)
+        if rc == _STALE:   # other parameters have gradients, or something lies elsewhere
+            plan = self._new_plan()
+            if plan is None:
+                return
+            rc = self._run(plan, gate, grad_scale)
+        if rc == _STRIDED:
+            kept = [p.grad for p in plan.params]
+            for p, g in zip(plan.params, kept):
+                p.grad = g.contiguous()
+            try:
+                rc = self._run(plan, gate, grad_scale)
+            finally:
+                for p, g in zip(plan.params, kept):
+                    p.grad = g
+        check(rc, "fsgs_adamw_multi")
+
+    def _new_plan(self):
+        self._plan = None
+        if any(p.grad is not None for g in self.param_groups for p in g["params"]):
+            self._plan = _Plan(self)
+        return self._plan
+
+    def _run(self, plan, gate, grad_scale):
         device = plan.device
         for t in (gate, grad_scale):
-            _need(t is None or (t.device == device and t.numel() == 1 and t.dtype == torch.float32),
-                  "AdamW: gate and grad_scale are one-element float32 tensors on the parameters' device")
+            _need(t is None or t.device == device, "AdamW: gate and grad_scale are on the parameters' device")
         with _on_device(device):
             self._workspaces(device)
-            data = plan.gradients(grads)
-            if self.max_grad_norm is not None:
-                _launch_norm(data, plan.numel, plan.grad_types, self.max_grad_norm, self._norm[1], self._norm[0])
-                grad_scale = self._norm[0][1:]
-            tail = (_ptr(grad_scale), _ptr(gate), _ptr(self._work[0]), self._work[0].numel(), _stream())
-            for launch in plan.launches:
-                launch.table["grad"] = data if launch.whole else [data[i] for i in launch.rows]
-                check(lib().fsgs_adamw_multi(*launch.head, self.state_bits, *launch.scalars, *tail), "fsgs_adamw_multi")
+            work, clip = self._work[0], self.max_grad_norm is not None
+            norm = (float(self.max_grad_norm), self._norm[1].data_ptr(), self._norm[1].numel(), self._norm[0].data_ptr()) \
+                if clip else (0.0, 0, 0, 0)
+            return _lib.host().step(plan.handle, self.param_groups, self.state, _lib.address("fsgs_adamw_multi"),
+                                    _lib.address("fsgs_grad_norm"), *norm, 0 if grad_scale is None else grad_scale.data_ptr(),
+                                    0 if gate is None else gate.data_ptr(), work.data_ptr(), work.numel(),
+                                    _stream().value or 0)
 
     def _workspaces(self, device):
         """Created once and never replaced on the same device: a captured step goes on using them."""
@@ -448,3 +431,6 @@ class AdamW(torch.optim.Optimizer):
                 _need(not torch.cuda.is_current_stream_capturing(),
                       "AdamW: take a step, or call init_state(), before a step is captured")
                 setattr(self, name, make())
+
+
+_hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW.step_gated)

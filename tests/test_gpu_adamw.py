@@ -367,3 +367,56 @@ def test_norm_at_the_ends_of_the_range():
     mixed = [torch.ones(9, device="cuda"), torch.ones(7, device="cuda", dtype=torch.bfloat16),
              torch.ones(9, device="cuda", dtype=torch.float16)]
     assert float(grad_norm(mixed)[0]) == 5.0
+
+
+def test_the_plan_follows_the_optimiser():
+    """Between steps: states replaced or cleared, a group added, a parameter put in another's place, hooks, a scheduler,
+    a state dictionary loaded: each following step is the formula's."""
+    from fsgs.optim import AdamW
+    params, _ = _make((400, 30, 2100), torch.float32, torch.float32)
+    opt = AdamW(params[:2], lr=1e-2)
+    seen = []
+    opt.register_step_pre_hook(lambda o, args, kwargs: seen.append("pre"))
+    opt.register_step_post_hook(lambda o, args, kwargs: seen.append("post"))
+    sched = torch.optim.lr_scheduler.StepLR(opt, step_size=1, gamma=0.5)
+
+    def one(sel, seed):
+        for p, g in zip(params, _make((400, 30, 2100), torch.float32, torch.float32, seed=seed)[1]):
+            p.grad = g
+        before = _snapshot(opt, sel)
+        opt.step()
+        _check_step(opt, before, sel, [p.grad for p in sel])
+
+    one(params[:2], 1)
+    assert seen == ["pre", "post"]
+    sched.step()
+    assert opt.param_groups[0]["lr"] == 5e-3
+    one(params[:2], 2)
+    opt.state[params[0]] = {k: v.clone() for k, v in opt.state[params[0]].items()}
+    one(params[:2], 3)
+    del opt.state[params[1]]
+    one(params[:2], 4)
+    assert float(opt.state[params[1]]["step"]) == 1 and float(opt.state[params[0]]["step"]) == 4
+    opt.add_param_group(dict(params=[params[2]], lr=1e-3, weight_decay=0.3))
+    one(params, 5)
+    opt.load_state_dict(opt.state_dict())
+    one(params, 6)
+    other = torch.nn.Parameter(torch.randn(30, device="cuda"))
+    opt.state[other] = opt.state.pop(params[1])
+    opt.param_groups[0]["params"][1] = params[1] = other
+    one(params, 7)
+    assert float(opt.state[other]["step"]) == 4
+    params[2].data = params[2].data[:1000]          # same address, another length
+    opt.state[params[2]] = {k: v if k == "step" else v[:1000].clone() for k, v in opt.state[params[2]].items()}
+    g = torch.randn(1000, device="cuda")
+    params[2].grad = None
+    params[0].grad = None
+    params[2].grad = g
+    before = _snapshot(opt, [params[1], params[2]])
+    opt.step()
+    _check_step(opt, before, [params[1], params[2]], [params[1].grad, g])
+    with torch.autograd.profiler.profile():
+        one_grad = [p.grad for p in params[1:]]
+        before = _snapshot(opt, params[1:])
+        opt.step()
+    _check_step(opt, before, params[1:], one_grad)
