@@ -87,33 +87,33 @@ def _balance_check(what, rows, idx, M, mask):
                                mask.device == rows.device), f"{what}: mask must be bool [N] on the same device")
 
 
-def _balance_count(idx, M, mask, with_codes):
-    """(counts with T and n behind them, codes or None, workspace), see fsgs_balance_count."""
+_PAIRS, _TABLE = 0, 1   # FSGS_BALANCE_PAIRS, FSGS_BALANCE_TABLE
+
+
+def _balance_count(idx, M, mask, form):
+    """(counts with T and n behind them, workspace for the other two calls), see fsgs_balance_count."""
     N, K = idx.shape
     idx, mask = idx.contiguous(), None if mask is None else mask.contiguous()
+    size = int(lib().fsgs_balance_workspace_bytes(N, K, M, form))
+    ops._need(size > 0, "balance: more than 2^36 pairs or table entries")
     counts = torch.empty(M + 2, dtype=torch.int64, device=idx.device)
-    head = int(lib().fsgs_balance_workspace_bytes())
-    more = int(lib().fsgs_balance_codes_bytes(N, K, M)) if with_codes else 0
-    buf = torch.empty(head + more, dtype=torch.uint8, device=idx.device)   # the head is a multiple of 16 bytes
-    codes = buf[head:] if with_codes else None
+    ws = torch.empty(size, dtype=torch.uint8, device=idx.device)
     p = ops._ptr
-    check(lib().fsgs_balance_count(N, K, M, p(idx), p(mask), p(counts), p(codes), p(buf), head, ops._stream()),
+    check(lib().fsgs_balance_count(N, K, M, p(idx), p(mask), form, p(counts), p(ws), size, ops._stream()),
           "fsgs_balance_count")
-    return counts, codes, buf
+    return counts, ws
 
 
-def _pairs(N, K, M, weights, codes, counts, scale, upstream, loss, grad, accumulate, workspace):
+def _pairs(N, K, M, weights, ws, scale, upstream, loss, grad, accumulate):
     p = ops._ptr
-    check(lib().fsgs_balance_pairs(N, K, M, p(weights), p(codes), p(counts), scale, p(upstream), p(loss), p(grad),
-                                   int(accumulate), p(workspace), 0 if workspace is None else workspace.numel(),
-                                   ops._stream()), "fsgs_balance_pairs")
+    check(lib().fsgs_balance_pairs(N, K, M, p(weights), p(ws), ws.numel(), scale, p(upstream), p(loss), p(grad),
+                                   int(accumulate), ops._stream()), "fsgs_balance_pairs")
 
 
-def _table(table, mask, counts, scale, upstream, loss, grad, workspace):
+def _table(table, mask, ws, scale, upstream, loss, grad):
     p, (N, M) = ops._ptr, table.shape
-    check(lib().fsgs_balance_table(N, M, _TYPES[table.dtype], p(table), table.stride(0) if N > 1 else M, p(mask), p(counts),
-                                   scale, p(upstream), p(loss), p(grad), M, p(workspace),
-                                   0 if workspace is None else workspace.numel(), ops._stream()), "fsgs_balance_table")
+    check(lib().fsgs_balance_table(N, M, _TYPES[table.dtype], p(table), table.stride(0) if N > 1 else M, p(mask), p(ws),
+                                   ws.numel(), scale, p(upstream), p(loss), p(grad), M, ops._stream()), "fsgs_balance_table")
 
 
 def _check_weights(weights, idx, M, mask):
@@ -137,10 +137,10 @@ class _BalanceLoss(torch.autograd.Function):
     def forward(ctx, weights, idx, M, mask):
         weights = weights.contiguous()
         with ops._on_device(weights.device):
-            counts, codes, ws = _balance_count(idx, M, mask, True)
+            counts, ws = _balance_count(idx, M, mask, _PAIRS)
             loss = torch.empty((), device=weights.device)
-            _pairs(*idx.shape, M, weights, codes, counts, 1.0, None, loss, None, False, ws)
-        ctx.save_for_backward(counts, codes)
+            _pairs(*idx.shape, M, weights, ws, 1.0, None, loss, None, False)
+        ctx.save_for_backward(ws)
         ctx.size = (*idx.shape, M)
         out = counts[:M]
         ctx.mark_non_differentiable(out)
@@ -149,12 +149,11 @@ class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _):
-        counts, codes = ctx.saved_tensors
+        ws, = ctx.saved_tensors
         N, K, M = ctx.size
-        g_loss = g_loss.float().contiguous()
-        grad = torch.empty(N, K, device=counts.device)
-        with ops._on_device(counts.device):
-            _pairs(N, K, M, None, codes, counts, 1.0, g_loss, None, grad, False, None)
+        grad = torch.empty(N, K, device=ws.device)
+        with ops._on_device(ws.device):
+            _pairs(N, K, M, None, ws, 1.0, g_loss, None, grad, False)
         return grad, None, None, None
 
 
@@ -180,10 +179,10 @@ def balance_value_and_grad(weights, idx, M, mask=None, weight=1.0, grad=None):
                                grad.device == weights.device), "balance_value_and_grad: grad must be contiguous float32 [N,K]")
     weights = weights.detach().contiguous()
     with ops._on_device(weights.device):
-        counts, codes, ws = _balance_count(idx, int(M), mask, True)
+        counts, ws = _balance_count(idx, int(M), mask, _PAIRS)
         loss = torch.empty((), device=weights.device)
         out = torch.empty_like(weights) if grad is None else grad
-        _pairs(*idx.shape, int(M), weights, codes, counts, float(weight), None, loss, out, grad is not None, ws)
+        _pairs(*idx.shape, int(M), weights, ws, float(weight), None, loss, out, grad is not None)
     return loss, out, counts[:M]
 
 
@@ -192,10 +191,10 @@ class _TableBalanceLoss(torch.autograd.Function):
     def forward(ctx, table, idx, mask):
         table, mask = _rows_of(table), None if mask is None else mask.contiguous()
         with ops._on_device(table.device):
-            counts, _, ws = _balance_count(idx, table.shape[1], mask, False)
+            counts, ws = _balance_count(idx, table.shape[1], mask, _TABLE)
             loss = torch.empty((), device=table.device)
-            _table(table, mask, counts, 1.0, None, loss, None, ws)
-        ctx.save_for_backward(table, mask, counts)
+            _table(table, mask, ws, 1.0, None, loss, None)
+        ctx.save_for_backward(table, mask, ws)
         out = counts[:table.shape[1]]
         ctx.mark_non_differentiable(out)
         return loss, out
@@ -203,11 +202,10 @@ class _TableBalanceLoss(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _):
-        table, mask, counts = ctx.saved_tensors
-        g_loss = g_loss.float().contiguous()
+        table, mask, ws = ctx.saved_tensors
         grad = torch.empty(table.shape, dtype=table.dtype, device=table.device)
         with ops._on_device(table.device):
-            _table(table, mask, counts, 1.0, g_loss, None, grad, None)
+            _table(table, mask, ws, 1.0, g_loss, None, grad)
         return grad, None, None
 
 
@@ -230,8 +228,8 @@ def table_balance_value_and_grad(table, idx, mask=None, weight=1.0):
     _check_table(table, idx, mask)
     table, mask = _rows_of(table.detach()), None if mask is None else mask.contiguous()
     with ops._on_device(table.device):
-        counts, _, ws = _balance_count(idx, table.shape[1], mask, False)
+        counts, ws = _balance_count(idx, table.shape[1], mask, _TABLE)
         loss = torch.empty((), device=table.device)
         grad = torch.empty(table.shape, dtype=table.dtype, device=table.device)
-        _table(table, mask, counts, float(weight), None, loss, grad, ws)
+        _table(table, mask, ws, float(weight), None, loss, grad)
     return loss, grad, counts[:table.shape[1]]

@@ -599,23 +599,24 @@ int fsgs_lbs_weights_backward(int P, int K, int M, const float *d2, const int64_
  * The counts carry no gradient.  T = 0 or n = 0: L = 0 and zero gradients.  A table row of nothing but -infinity adds
  * nothing to P.  What does not count has gradient 0 (added nothing), and its weights are not read into the sum.
  *
- * fsgs_balance_count: counts [M+2] = c, T, n; codes (optional, fsgs_balance_codes_bytes): the superpoint of every pair in
- * 2 or 4 bytes, for fsgs_balance_pairs.  It prepares the workspace (16-byte aligned) for one call of the other two.
- * scale and *upstream (device, optional) multiply the loss and the gradient.  loss (device, one float) and the gradient
- * are both optional; without loss the workspace may be NULL.  accumulate: the gradient is added to g_weights.
- * fsgs_balance_table: rows of M elements of `type`, row_stride / g_row_stride elements apart; g_table has the table's
- * type.  Sums are added in a fixed order: the same inputs give the same bits.
+ * fsgs_balance_count: counts [M+2] = c, T, n, and into the workspace (16-byte aligned, needs no preparation) what the other
+ * two calls need: FSGS_BALANCE_PAIRS for fsgs_balance_pairs, FSGS_BALANCE_TABLE for fsgs_balance_table, which may then be
+ * called any number of times, one after another, with the same workspace.  scale and *upstream (device, optional)
+ * multiply the loss and the gradient.  loss (device, one float) and the gradient are both optional.  accumulate: the
+ * gradient is added to g_weights.  fsgs_balance_table: rows of M elements of `type`, row_stride / g_row_stride elements
+ * apart; g_table has the table's type; its workspace is that of any K.  Sums are added in a fixed order: the same inputs
+ * give the same bits.  N K <= 2^36, and N M <= 2^36 in the table form.
  * ---------------------------------------------------------------------------------------------- */
-size_t fsgs_balance_workspace_bytes(void);
-size_t fsgs_balance_codes_bytes(int64_t N, int K, int M);
-int fsgs_balance_count(int64_t N, int K, int M, const int64_t *idx, const uint8_t *mask, int64_t *counts, void *codes,
+#define FSGS_BALANCE_PAIRS 0
+#define FSGS_BALANCE_TABLE 1
+size_t fsgs_balance_workspace_bytes(int64_t N, int K, int M, int form);
+int fsgs_balance_count(int64_t N, int K, int M, const int64_t *idx, const uint8_t *mask, int form, int64_t *counts,
     void *workspace, size_t workspace_bytes, fsgs_stream_t stream);
-int fsgs_balance_pairs(int64_t N, int K, int M, const float *weights, const void *codes, const int64_t *counts,
-    float scale, const float *upstream, float *loss, float *g_weights, int accumulate, void *workspace,
-    size_t workspace_bytes, fsgs_stream_t stream);
+int fsgs_balance_pairs(int64_t N, int K, int M, const float *weights, void *workspace, size_t workspace_bytes, float scale,
+    const float *upstream, float *loss, float *g_weights, int accumulate, fsgs_stream_t stream);
 int fsgs_balance_table(int64_t N, int M, int type, const void *table, int64_t row_stride, const uint8_t *mask,
-    const int64_t *counts, float scale, const float *upstream, float *loss, void *g_table, int64_t g_row_stride,
-    void *workspace, size_t workspace_bytes, fsgs_stream_t stream);
+    void *workspace, size_t workspace_bytes, float scale, const float *upstream, float *loss, void *g_table,
+    int64_t g_row_stride, fsgs_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
  * One view of a training iteration in two calls (forward, backward), all intermediates in one workspace.

@@ -21,25 +21,33 @@ def test_entry_points_check_their_arguments():
     """The C side refuses before anything is launched (no device is needed to see it)."""
     from fsgs._lib import lib
     L = lib()
-    head = L.fsgs_balance_workspace_bytes()
-    assert head % 16 == 0 and L.fsgs_balance_codes_bytes(10, 3, 512) == 60 and L.fsgs_balance_codes_bytes(10, 3, 65536) == 120
-    assert L.fsgs_balance_codes_bytes(0, 3, 512) == 0
-    ok = dict(N=4, K=2, M=3, idx=4096, mask=0, counts=4096, codes=4096, ws=4096, n=head)
+    need = L.fsgs_balance_workspace_bytes
+    pairs_ws, table_ws = need(4, 2, 3, 0), need(4, 2, 3, 1)
+    assert pairs_ws % 16 == 0 and need(10, 3, 70_000, 0) - need(0, 3, 70_000, 0) == 128 and need(0, 1, 1, 1) > 0
+    for bad in ((-1, 2, 3, 0), (4, 0, 3, 0), (4, 2, 0, 0), (4, 2, 3, 2), (1 << 36, 2, 3, 0), (1 << 26, 2, 2048, 1)):
+        assert need(*bad) == 0, bad
+    ok = dict(N=4, K=2, M=3, idx=4096, mask=0, form=0, counts=4096, ws=4096, n=pairs_ws)
+
     def count(**kw):
         a = dict(ok, **kw)
-        return L.fsgs_balance_count(a["N"], a["K"], a["M"], a["idx"], a["mask"], a["counts"], a["codes"], a["ws"], a["n"], None)
-    for bad in (dict(N=-1), dict(K=0), dict(M=0), dict(idx=0), dict(counts=0)):
+        return L.fsgs_balance_count(a["N"], a["K"], a["M"], a["idx"], a["mask"], a["form"], a["counts"], a["ws"], a["n"], None)
+
+    for bad in (dict(N=-1), dict(K=0), dict(M=0), dict(idx=0), dict(counts=0), dict(form=2)):
         assert count(**bad) == -1, bad
-    assert count(ws=0) == -3 and count(ws=4100) == -3 and count(n=head - 1) == -3 and count(N=1 << 40) == -5
-    pairs = lambda N=4, K=2, M=3, w=4096, codes=4096, counts=4096, loss=4096, g=0, ws=4096, n=head: L.fsgs_balance_pairs(  # noqa: E731
-        N, K, M, w, codes, counts, 1.0, None, loss, g, 0, ws, n, None)
-    assert pairs(w=0) == -1 and pairs(codes=0) == -1 and pairs(counts=0) == -1 and pairs(N=-1) == -1 and pairs(ws=0) == -3
-    assert pairs(loss=0, ws=0) == 0                                      # nothing asked for
-    table = lambda N=4, M=3, type=0, t=4096, rs=3, counts=4096, loss=4096, g=0, gs=3, ws=4096, n=head: L.fsgs_balance_table(  # noqa: E731
-        N, M, type, t, rs, None, counts, 1.0, None, loss, g, gs, ws, n, None)
-    for bad in (dict(N=-1), dict(M=0), dict(type=3), dict(t=0), dict(rs=2), dict(g=4096, gs=2), dict(counts=0)):
+    assert count(ws=0) == -3 and count(ws=4100) == -3 and count(n=pairs_ws - 1) == -3 and count(N=1 << 40) == -5
+
+    def pairs(N=4, K=2, M=3, w=4096, ws=4096, n=pairs_ws, loss=4096, g=0):
+        return L.fsgs_balance_pairs(N, K, M, w, ws, n, 1.0, None, loss, g, 0, None)
+
+    assert pairs(w=0) == -1 and pairs(N=-1) == -1 and pairs(ws=0) == -3 and pairs(n=8) == -3 and pairs(N=1 << 40) == -5
+    assert pairs(loss=0) == 0                                      # nothing asked for
+
+    def table(N=4, M=3, type=0, t=4096, rs=3, ws=4096, n=table_ws, loss=4096, g=0, gs=3):
+        return L.fsgs_balance_table(N, M, type, t, rs, None, ws, n, 1.0, None, loss, g, gs, None)
+
+    for bad in (dict(N=-1), dict(M=0), dict(type=3), dict(t=0), dict(rs=2), dict(g=4096, gs=2)):
         assert table(**bad) == -1, bad
-    assert table(ws=0) == -3 and table(n=5) == -3 and table(loss=0, ws=0) == 0 and table(N=1 << 40) == -5
+    assert table(ws=0) == -3 and table(n=5) == -3 and table(loss=0) == 0 and table(N=1 << 40) == -5
 
 
 def test_step_entry_points_check_their_arguments():

@@ -33,7 +33,7 @@ def _counts(idx, M, mask):
     return c, on, int(c.sum()), idx.shape[0] if mask is None else int(mask.sum())
 
 
-PAIRS = [(1, 1, 1, None, 0.0), (1, 3, 512, None, 0.0), (1000, 3, 512, None, 0.0), (1001, 8, 7, 0.3, 0.1),
+PAIRS = [(1, 1, 1, None, 0.0), (7, 3, 8192, 0.2, 0.1), (100_001, 5, 8193, 0.2, 0.1), (1, 3, 512, None, 0.0), (1000, 3, 512, None, 0.0), (1001, 8, 7, 0.3, 0.1),
          (33, 5, 9000, 0.5, 0.2), (50_003, 3, 512, 0.02, 0.0), (20_000, 2, 70_000, 0.1, 0.1), (3000, 16, 65_535, None, 0.1),
          (257, 4, 100, 1.0, 0.0), (64, 2, 10, None, 1.0), (5, 40, 3, 0.2, 0.2), (300_000, 8, 4096, 0.3, 0.01)]
 
@@ -90,7 +90,9 @@ def _table_reference(z, idx, mask):
 
 TABLES = [(1, 1, 1, None), (1, 1, 2, None), (5, 2, 3, 0.5), (100, 3, 128, None), (100, 3, 129, 0.3), (77, 2, 333, 0.1),
           (1000, 3, 512, None), (64, 4, 513, 0.2), (40, 8, 2048, None), (33, 2, 2049, 0.2), (20, 3, 8192, None),
-          (10, 3, 8193, 0.2), (6, 2, 20_011, None), (3000, 3, 512, 1.0)]
+          (10, 3, 8193, 0.2), (6, 2, 20_011, None), (3000, 3, 512, 1.0), (1003, 3, 8, 0.1), (333, 2, 64, None),
+          (65, 2, 65, 0.2), (50, 3, 256, 0.1), (50, 3, 260, None), (30, 3, 1024, 0.1), (30, 3, 1025, None), (21, 2, 4096, None),
+          (21, 2, 4100, 0.2), (9, 2, 8188, None)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
