@@ -26,7 +26,7 @@ constexpr int kBalSlots = 1184;           // partial sums of the pairs form
 // The workspace: this, the share of every superpoint as float32, then the codes of the pairs (pairs form) or the sums of
 // the thread blocks (table form).
 struct BalanceHead {
-  int counted, closed;      // tickets: blocks that have finished counting / summing
+  int closed, pad;          // ticket: blocks that have finished summing
   double total, rows;       // T and n
   double slots[kBalSlots];
 };
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long lo
   }
   __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) s_last = atomicAdd(&head->counted, 1) == (int) gridDim.x - 1;
+  if (threadIdx.x == 0) s_last = atomicAdd(counts + M + 2, 1ull) == gridDim.x - 1;
   __syncthreads();
   if (!s_last) return;
   __threadfence();
@@ -443,9 +443,7 @@ extern "C" int fsgs_balance_count(int64_t N, int K, int M, const int64_t *idx, c
   if (!balance_workspace(N, K, M, form, workspace, workspace_bytes)) return FSGS_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t) stream;
   const BalanceSpace w = balance_space(workspace, M);
-  if (cudaMemsetAsync(counts, 0, sizeof(int64_t) * ((size_t) M + 2), st) != cudaSuccess ||
-      cudaMemsetAsync(w.head, 0, 2 * sizeof(int), st) != cudaSuccess)
-    return FSGS_ERR_LAUNCH;
+  if (cudaMemsetAsync(counts, 0, sizeof(int64_t) * ((size_t) M + 4), st) != cudaSuccess) return FSGS_ERR_LAUNCH;
   const int grid = balance_blocks((N * K + 3) / 4, kCountThreads, 2 * 148);
   const size_t smem = M <= kBalSharedPoints ? sizeof(int) * ((size_t) M + 1) : 0;
   unsigned long long *c = (unsigned long long *) counts;

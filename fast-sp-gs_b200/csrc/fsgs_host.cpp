@@ -1,10 +1,17 @@
-// The host side of the optimiser step for many tensors: reads every address and length of the parameters, gradients and
-// states anew each step, straight from the tensors, and hands them to the C entry points.  In Python the same walk costs
-// 1.2 us per tensor (190 us for a network of 120 tensors whose kernels take 17 us); here 0.06 us.
+// The host side of the training-step operators where Python would take longer than the kernels.
 //
-// A CPython extension of two functions and a capsule, compiled against torch's headers; it holds no CUDA code and calls
-// libfsgs.so through the function pointers that fsgs/optim.py gives it.
+// The optimiser step: reads every address and length of the parameters, gradients and states anew each step, straight from
+// the tensors, and hands them to the C entry points.  In Python the same walk costs 1.2 us per tensor (190 us for a network
+// of 120 tensors whose kernels take 17 us); here 0.06 us.  The balance losses: argument checks, outputs, and the autograd
+// nodes.
+//
+// A CPython extension compiled against torch's headers; it holds no CUDA code and calls libfsgs.so through the function
+// pointers that bind() gives it.
 #include <Python.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <unordered_map>
@@ -17,6 +24,17 @@ namespace {
 using AdamWFn = int (*)(int, const fsgs_adamw_tensor *, int, int, int, double, double, float, const float *, const float *,
     void *, size_t, fsgs_stream_t);
 using NormFn = int (*)(int, const fsgs_norm_tensor *, float, void *, size_t, float *, fsgs_stream_t);
+
+struct {
+  AdamWFn adamw;
+  NormFn norm;
+  size_t (*balance_bytes)(int64_t, int, int, int);
+  int (*balance_count)(int64_t, int, int, const int64_t *, const uint8_t *, int, int64_t *, void *, size_t, fsgs_stream_t);
+  int (*balance_pairs)(int64_t, int, int, const float *, void *, size_t, float, const float *, float *, float *, int, fsgs_stream_t);
+  int (*balance_table)(int64_t, int, int, const void *, int64_t, const uint8_t *, void *, size_t, float, const float *, float *,
+      void *, int64_t, fsgs_stream_t);
+  const char *(*status_string)(int);
+} lib;
 
 // what a walk found, besides a status of the C entry points (0 or negative)
 enum { kStale = 1, kStrided = 2 };
@@ -165,21 +183,19 @@ int walk(Plan &plan, PyObject *groups, PyObject *state) {
   return found != plan.entries.size() ? kStale : strided ? kStrided : 0;
 }
 
-// step(plan, groups, state, adamw, norm, max_norm, norm workspace, its bytes, norm out, grad_scale, gate, workspace, its
-// bytes, stream): addresses as integers, 0 for none; norm out 0: no norm
+// step(plan, groups, state, max_norm, norm workspace, its bytes, norm out, grad_scale, gate, workspace, its bytes, stream):
+// addresses as integers, 0 for none; norm out 0: no norm
 PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 14 || !PyList_Check(args[1]) || !PyDict_Check(args[2])) return refuse("fsgs_host.step: wrong arguments");
+  if (n != 12 || !PyList_Check(args[1]) || !PyDict_Check(args[2])) return refuse("fsgs_host.step: wrong arguments");
   Plan *plan = (Plan *) PyCapsule_GetPointer(args[0], "fsgs.plan");
   if (!plan) return nullptr;
   auto at = [&](int k) { return (uintptr_t) PyLong_AsUnsignedLongLong(args[k]); };
-  const auto adamw = (AdamWFn) at(3);
-  const auto norm = (NormFn) at(4);
-  const float max_norm = (float) PyFloat_AsDouble(args[5]);
-  void *norm_ws = (void *) at(6), *ws = (void *) at(11);
-  const size_t norm_bytes = at(7), bytes = at(12);
-  float *norm_out = (float *) at(8);
-  const float *grad_scale = (const float *) at(9), *gate = (const float *) at(10);
-  const auto stream = (fsgs_stream_t) at(13);
+  const float max_norm = (float) PyFloat_AsDouble(args[3]);
+  void *norm_ws = (void *) at(4), *ws = (void *) at(9);
+  const size_t norm_bytes = at(5), bytes = at(10);
+  float *norm_out = (float *) at(6);
+  const float *grad_scale = (const float *) at(7), *gate = (const float *) at(8);
+  const auto stream = (fsgs_stream_t) at(11);
   if (PyErr_Occurred()) return nullptr;
   int rc;
   try {
@@ -189,27 +205,26 @@ PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   }
   if (rc != 0) return PyLong_FromLong(rc);
   if (norm_out) {
-    rc = norm((int) plan->norm.size(), plan->norm.data(), max_norm, norm_ws, norm_bytes, norm_out, stream);
+    rc = lib.norm((int) plan->norm.size(), plan->norm.data(), max_norm, norm_ws, norm_bytes, norm_out, stream);
     if (rc != 0) return PyLong_FromLong(rc);
     grad_scale = norm_out + 1;
   }
   for (const Launch &l : plan->launches) {
-    rc = adamw(l.n, l.table, l.param_type, l.grad_type, l.bits, l.b1, l.b2, l.eps, grad_scale, gate, ws, bytes, stream);
+    rc = lib.adamw(l.n, l.table, l.param_type, l.grad_type, l.bits, l.b1, l.b2, l.eps, grad_scale, gate, ws, bytes, stream);
     if (rc != 0) break;
   }
   return PyLong_FromLong(rc);
 }
 
-// norm(tensors, norm, max_norm, workspace, its bytes, out, stream)
+// norm(tensors, max_norm, workspace, its bytes, out, stream)
 PyObject *norm_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 7 || !PyList_Check(args[0])) return refuse("fsgs_host.norm: wrong arguments");
+  if (n != 6 || !PyList_Check(args[0])) return refuse("fsgs_host.norm: wrong arguments");
   auto at = [&](int k) { return (uintptr_t) PyLong_AsUnsignedLongLong(args[k]); };
-  const auto norm = (NormFn) at(1);
-  const float max_norm = (float) PyFloat_AsDouble(args[2]);
-  void *ws = (void *) at(3);
-  const size_t bytes = at(4);
-  float *out = (float *) at(5);
-  const auto stream = (fsgs_stream_t) at(6);
+  const float max_norm = (float) PyFloat_AsDouble(args[1]);
+  void *ws = (void *) at(2);
+  const size_t bytes = at(3);
+  float *out = (float *) at(4);
+  const auto stream = (fsgs_stream_t) at(5);
   if (PyErr_Occurred()) return nullptr;
   static const char *want = "grad_norm: dense float32, bfloat16 or float16 CUDA tensors on one device";
   try {
@@ -226,15 +241,246 @@ PyObject *norm_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
       if (!t.is_contiguous()) return PyLong_FromLong(kStrided);
       table[(size_t) i] = {t.data_ptr(), t.numel(), type};
     }
-    return PyLong_FromLong(norm((int) count, table.data(), max_norm, ws, bytes, out, stream));
+    return PyLong_FromLong(lib.norm((int) count, table.data(), max_norm, ws, bytes, out, stream));
   } catch (const std::exception &e) {
     return refuse(e.what());
   }
 }
 
+// ---- balance losses -----------------------------------------------------------------------------------------
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void need(bool ok, const char *what, const char *message) {
+  if (!ok) throw std::runtime_error(std::string(what) + ": " + message);
+}
+
+void check(int rc, const char *what) {
+  if (rc != 0) throw std::runtime_error(std::string(what) + ": " + lib.status_string(rc) + " (status " + std::to_string(rc) + ")");
+}
+
+constexpr const char *kPairs = "balance_loss", *kTable = "table_balance_loss";
+
+void check_rows(const char *what, const Tensor &rows, const Tensor &idx, int64_t M, const std::optional<Tensor> &mask) {
+  need(lib.balance_count, what, "the library is not bound");
+  need(rows.is_cuda() && rows.layout() == at::kStrided && rows.dim() == 2, what, "a two-dimensional CUDA tensor is expected");
+  need(idx.dim() == 2 && idx.layout() == at::kStrided && idx.scalar_type() == at::kLong && idx.size(0) == rows.size(0) &&
+           idx.size(1) > 0 && idx.size(1) <= INT32_MAX && idx.device() == rows.device(),
+       what, "idx must be int64 [N,K] on the same device");
+  need(M > 0 && M < INT32_MAX, what, "the number of superpoints must be positive");
+  if (mask)
+    need((mask->scalar_type() == at::kBool || mask->scalar_type() == at::kByte) && mask->layout() == at::kStrided &&
+             mask->dim() == 1 && mask->size(0) == rows.size(0) && mask->device() == rows.device(),
+         what, "mask must be bool [N] on the same device");
+}
+
+void check_pairs(const Tensor &weights, const Tensor &idx, int64_t M, const std::optional<Tensor> &mask) {
+  check_rows(kPairs, weights, idx, M, mask);
+  need(weights.scalar_type() == at::kFloat && weights.sizes() == idx.sizes(), kPairs, "weights must be float32 [N,K]");
+}
+
+int check_table(const Tensor &table, const Tensor &idx, const std::optional<Tensor> &mask) {
+  check_rows(kTable, table, idx, table.dim() == 2 ? table.size(1) : 0, mask);
+  const int type = type_of(table.scalar_type());
+  need(type >= 0, kTable, "float32, bfloat16 or float16 table");
+  return type;
+}
+
+const uint8_t *bytes_of(const std::optional<Tensor> &mask) { return mask ? (const uint8_t *) mask->data_ptr() : nullptr; }
+std::optional<Tensor> dense(const std::optional<Tensor> &mask) { return mask ? std::optional<Tensor>(mask->contiguous()) : mask; }
+fsgs_stream_t stream_of(const Tensor &t) { return (fsgs_stream_t) c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+struct Counted {
+  Tensor counts, ws;  // counts [M + 4]
+};
+
+Counted count(const char *what, const Tensor &idx, int64_t M, const std::optional<Tensor> &mask, int form) {
+  const size_t bytes = lib.balance_bytes(idx.size(0), (int) idx.size(1), (int) M, form);
+  need(bytes > 0, what, "more than 2^36 pairs or table entries");
+  Counted c{at::empty({M + 4}, idx.options()), at::empty({(int64_t) bytes}, idx.options().dtype(at::kByte))};
+  const Tensor i = idx.contiguous();
+  check(lib.balance_count(i.size(0), (int) i.size(1), (int) M, i.data_ptr<int64_t>(), bytes_of(mask), form,
+                          c.counts.data_ptr<int64_t>(), c.ws.data_ptr(), bytes, stream_of(i)),
+        "fsgs_balance_count");
+  return c;
+}
+
+void pairs(int64_t N, int64_t K, int64_t M, const float *weights, const Tensor &ws, float scale, const float *upstream, float *loss,
+    float *grad, bool accumulate) {
+  check(lib.balance_pairs(N, (int) K, (int) M, weights, ws.data_ptr(), (size_t) ws.numel(), scale, upstream, loss, grad, accumulate,
+                          stream_of(ws)),
+        "fsgs_balance_pairs");
+}
+
+void table_pass(const Tensor &t, int type, const std::optional<Tensor> &mask, const Tensor &ws, float scale, const float *upstream,
+    float *loss, void *grad) {
+  const int64_t N = t.size(0), M = t.size(1);
+  check(lib.balance_table(N, (int) M, type, t.data_ptr(), N > 1 ? t.stride(0) : M, bytes_of(mask), ws.data_ptr(), (size_t) ws.numel(),
+                          scale, upstream, loss, grad, M, stream_of(ws)),
+        "fsgs_balance_table");
+}
+
+// the table itself where its rows are runs of memory that do not overlap, else a copy
+Tensor rows_of(const Tensor &t) {
+  return (t.stride(1) == 1 || t.size(1) == 1) && t.stride(0) >= t.size(1) ? t : t.contiguous();
+}
+
+// A backward pass is not differentiable itself: a graph through it raises when it is used.
+Tensor once(const Tensor &grad, const Tensor &upstream) {
+  if (!at::GradMode::is_enabled() || !upstream.requires_grad()) return grad;
+  auto error = std::make_shared<torch::autograd::DelayedError>("the balance losses have no second derivatives", 1);
+  return (*error)({grad.detach().set_requires_grad(true)})[0];
+}
+
+struct PairsLoss : torch::autograd::Function<PairsLoss> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &weights, const Tensor &idx, int64_t M, const std::optional<Tensor> &mask) {
+    const c10::cuda::CUDAGuard guard(weights.device());
+    const Tensor w = weights.contiguous();
+    const Counted c = count(kPairs, idx, M, dense(mask), FSGS_BALANCE_PAIRS);
+    Tensor loss = at::empty({}, w.options().requires_grad(false)), counts = c.counts.narrow(0, 0, M);
+    pairs(idx.size(0), idx.size(1), M, w.data_ptr<float>(), c.ws, 1.0f, nullptr, loss.data_ptr<float>(), nullptr, false);
+    ctx->save_for_backward({c.ws});
+    ctx->saved_data["N"] = idx.size(0), ctx->saved_data["K"] = idx.size(1), ctx->saved_data["M"] = M;
+    ctx->mark_non_differentiable({counts});
+    return {loss, counts};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    if (!g[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const Tensor ws = ctx->get_saved_variables()[0];
+    const c10::cuda::CUDAGuard guard(ws.device());
+    const int64_t N = ctx->saved_data["N"].toInt(), K = ctx->saved_data["K"].toInt();
+    Tensor grad = at::empty({N, K}, g[0].options().requires_grad(false));
+    pairs(N, K, ctx->saved_data["M"].toInt(), nullptr, ws, 1.0f, g[0].data_ptr<float>(), nullptr, grad.data_ptr<float>(), false);
+    return {once(grad, g[0]), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct TableLoss : torch::autograd::Function<TableLoss> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &table, const Tensor &idx, const std::optional<Tensor> &mask) {
+    const c10::cuda::CUDAGuard guard(table.device());
+    const Tensor t = rows_of(table);
+    const auto m = dense(mask);
+    const Counted c = count(kTable, idx, t.size(1), m, FSGS_BALANCE_TABLE);
+    Tensor loss = at::empty({}, t.options().dtype(at::kFloat).requires_grad(false)), counts = c.counts.narrow(0, 0, t.size(1));
+    table_pass(t, type_of(t.scalar_type()), m, c.ws, 1.0f, nullptr, loss.data_ptr<float>(), nullptr);
+    ctx->save_for_backward({t, m ? *m : Tensor(), c.ws});
+    ctx->mark_non_differentiable({counts});
+    return {loss, counts};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    if (!g[0].defined()) return {Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &t = saved[0];
+    const c10::cuda::CUDAGuard guard(t.device());
+    Tensor grad = at::empty(t.sizes(), t.options().requires_grad(false));
+    table_pass(t, type_of(t.scalar_type()), saved[1].defined() ? std::optional<Tensor>(saved[1]) : std::nullopt, saved[2], 1.0f,
+               g[0].data_ptr<float>(), nullptr, grad.data_ptr());
+    return {once(grad, g[0]), Tensor(), Tensor()};
+  }
+};
+
+bool tensor_of(PyObject *o, Tensor &t) {
+  if (!THPVariable_Check(o)) return false;
+  t = THPVariable_Unpack(o);
+  return true;
+}
+
+std::optional<Tensor> mask_of(const char *what, PyObject *o) {
+  if (o == Py_None) return std::nullopt;
+  need(THPVariable_Check(o), what, "mask must be bool [N] on the same device");
+  return THPVariable_Unpack(o);
+}
+
+PyObject *tuple_of(std::initializer_list<Tensor> list) {
+  PyObject *out = PyTuple_New((Py_ssize_t) list.size());
+  Py_ssize_t i = 0;
+  for (const Tensor &t : list) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
+  return out;
+}
+
+// balance_pairs(weights, idx, M, mask, weight, grad, autograd) -> (loss, counts) or (loss, grad, counts)
+PyObject *balance_pairs(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 7) return refuse("fsgs_host.balance_pairs: wrong arguments");
+  const int64_t M = PyLong_AsLongLong(args[2]);
+  const float weight = (float) PyFloat_AsDouble(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  try {
+    Tensor w, idx, grad;
+    need(tensor_of(args[0], w) && tensor_of(args[1], idx), kPairs, "weights and idx must be tensors");
+    const auto mask = mask_of(kPairs, args[3]);
+    check_pairs(w, idx, M, mask);
+    if (args[6] == Py_True) {
+      const auto out = PairsLoss::apply(w, idx, M, mask);
+      return tuple_of({out[0], out[1]});
+    }
+    const bool add = args[5] != Py_None;
+    if (add)
+      need(tensor_of(args[5], grad) && grad.sizes() == w.sizes() && grad.scalar_type() == at::kFloat && grad.is_contiguous() &&
+               grad.device() == w.device(),
+           "balance_value_and_grad", "grad must be contiguous float32 [N,K]");
+    const c10::cuda::CUDAGuard guard(w.device());
+    const at::NoGradGuard none;
+    w = w.contiguous();
+    const Counted c = count(kPairs, idx, M, dense(mask), FSGS_BALANCE_PAIRS);
+    Tensor loss = at::empty({}, w.options().requires_grad(false));
+    if (!add) grad = at::empty(w.sizes(), w.options().requires_grad(false));
+    pairs(idx.size(0), idx.size(1), M, w.data_ptr<float>(), c.ws, weight, nullptr, loss.data_ptr<float>(), grad.data_ptr<float>(), add);
+    return tuple_of({loss, grad, c.counts.narrow(0, 0, M)});
+  } catch (const std::exception &e) {
+    return refuse(e.what());
+  }
+}
+
+// balance_table(table, idx, mask, weight, autograd) -> (loss, counts) or (loss, grad, counts)
+PyObject *balance_table(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (n != 5) return refuse("fsgs_host.balance_table: wrong arguments");
+  const float weight = (float) PyFloat_AsDouble(args[3]);
+  if (PyErr_Occurred()) return nullptr;
+  try {
+    Tensor t, idx;
+    need(tensor_of(args[0], t) && tensor_of(args[1], idx), kTable, "table and idx must be tensors");
+    const auto mask = mask_of(kTable, args[2]);
+    const int type = check_table(t, idx, mask);
+    if (args[4] == Py_True) {
+      const auto out = TableLoss::apply(t, idx, mask);
+      return tuple_of({out[0], out[1]});
+    }
+    const c10::cuda::CUDAGuard guard(t.device());
+    const at::NoGradGuard none;
+    t = rows_of(t);
+    const auto m = dense(mask);
+    const Counted c = count(kTable, idx, t.size(1), m, FSGS_BALANCE_TABLE);
+    Tensor loss = at::empty({}, t.options().dtype(at::kFloat).requires_grad(false));
+    Tensor grad = at::empty(t.sizes(), t.options().requires_grad(false));
+    table_pass(t, type, m, c.ws, weight, nullptr, loss.data_ptr<float>(), grad.data_ptr());
+    return tuple_of({loss, grad, c.counts.narrow(0, 0, t.size(1))});
+  } catch (const std::exception &e) {
+    return refuse(e.what());
+  }
+}
+
+// bind(addresses): the entry points in the order of `lib`
+PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  constexpr Py_ssize_t count = sizeof(lib) / sizeof(void *);
+  if (n != count) return refuse("fsgs_host.bind: wrong number of addresses");
+  void *address[count];
+  for (Py_ssize_t i = 0; i < count; ++i) address[i] = PyLong_AsVoidPtr(args[i]);
+  if (PyErr_Occurred()) return nullptr;
+  memcpy(&lib, address, sizeof(lib));
+  Py_RETURN_NONE;
+}
+
+using Fast = PyObject *(*) (PyObject *, PyObject *const *, Py_ssize_t);
+PyCFunction fast(Fast f) { return (PyCFunction) (void (*)(void)) f; }
+
 PyMethodDef methods[] = {{"plan", make_plan, METH_VARARGS, nullptr},
-                         {"step", (PyCFunction) (void (*)(void)) step, METH_FASTCALL, nullptr},
-                         {"norm", (PyCFunction) (void (*)(void)) norm_of, METH_FASTCALL, nullptr},
+                         {"step", fast(step), METH_FASTCALL, nullptr},
+                         {"norm", fast(norm_of), METH_FASTCALL, nullptr},
+                         {"balance_pairs", fast(balance_pairs), METH_FASTCALL, nullptr},
+                         {"balance_table", fast(balance_table), METH_FASTCALL, nullptr},
+                         {"bind", fast(bind), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fsgs_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -216,13 +216,11 @@ def host():
         spec = importlib.util.spec_from_file_location("_fsgs_host", HOST)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib(), name), c_void_p).value for name in (
+            "fsgs_adamw_multi", "fsgs_grad_norm", "fsgs_balance_workspace_bytes", "fsgs_balance_count", "fsgs_balance_pairs",
+            "fsgs_balance_table", "fsgs_status_string")))
         _host = module
     return _host
-
-
-def address(name):
-    """Address of an entry point of the library."""
-    return ctypes.cast(getattr(lib(), name), c_void_p).value
 
 
 def check(status, what):

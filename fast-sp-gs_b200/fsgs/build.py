@@ -1,5 +1,6 @@
 """Builds ``libfsgs.so`` (sm_100a) next to the sources.  ``python -m fsgs.build`` or ``fsgs.build.build()``."""
 import os
+import shutil
 import subprocess
 import sys
 
@@ -22,15 +23,20 @@ def _stale():
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _cuda_home():
+    nvcc = shutil.which("nvcc")
+    return os.path.dirname(os.path.dirname(os.path.realpath(nvcc))) if nvcc else "/usr/local/cuda"
+
+
 def _host_command():
     """g++ command line of the host extension: torch's headers and libraries, this interpreter's headers."""
     import sysconfig
     import torch
     root = os.path.dirname(torch.__file__)
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
-           sysconfig.get_paths()["include"]]
+           sysconfig.get_paths()["include"], os.path.join(_cuda_home(), "include")]
     return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", os.path.join(CSRC, "fsgs_host.cpp"), "-o", HOST,
-            "-Wl,--no-as-needed", "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+            "-Wl,--no-as-needed", "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"] + ["-I" + d for d in inc]
 
 

@@ -7,7 +7,7 @@ compositing backward reads."""
 import torch
 
 from . import ops
-from ._lib import lib, check
+from ._lib import check, host, lib
 
 C1, C2 = 0.01 ** 2, 0.03 ** 2
 
@@ -75,88 +75,6 @@ def l1_ssim_value_and_grad(image, target, lambda_l1=0.8, lambda_ssim=0.2):
 
 # ---- balance over the superpoints ------------------------------------------------------------------------------------
 
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # FSGS_F32, FSGS_BF16, FSGS_F16
-
-
-def _balance_check(what, rows, idx, M, mask):
-    ops._need(rows.is_cuda and rows.dim() == 2, f"{what}: a two-dimensional CUDA tensor is expected")
-    ops._need(idx.dim() == 2 and idx.dtype == torch.int64 and idx.shape[0] == rows.shape[0] and idx.shape[1] > 0 and
-              idx.device == rows.device, f"{what}: idx must be int64 [N,K] on the same device")
-    ops._need(0 < int(M) < 2 ** 31, f"{what}: the number of superpoints must be positive")
-    ops._need(mask is None or (mask.dtype in (torch.bool, torch.uint8) and tuple(mask.shape) == (rows.shape[0],) and
-                               mask.device == rows.device), f"{what}: mask must be bool [N] on the same device")
-
-
-_PAIRS, _TABLE = 0, 1   # FSGS_BALANCE_PAIRS, FSGS_BALANCE_TABLE
-
-
-def _balance_count(idx, M, mask, form):
-    """(counts with T and n behind them, workspace for the other two calls), see fsgs_balance_count."""
-    N, K = idx.shape
-    idx, mask = idx.contiguous(), None if mask is None else mask.contiguous()
-    size = int(lib().fsgs_balance_workspace_bytes(N, K, M, form))
-    ops._need(size > 0, "balance: more than 2^36 pairs or table entries")
-    counts = torch.empty(M + 2, dtype=torch.int64, device=idx.device)
-    ws = torch.empty(size, dtype=torch.uint8, device=idx.device)
-    p = ops._ptr
-    check(lib().fsgs_balance_count(N, K, M, p(idx), p(mask), form, p(counts), p(ws), size, ops._stream()),
-          "fsgs_balance_count")
-    return counts, ws
-
-
-def _pairs(N, K, M, weights, ws, scale, upstream, loss, grad, accumulate):
-    p = ops._ptr
-    check(lib().fsgs_balance_pairs(N, K, M, p(weights), p(ws), ws.numel(), scale, p(upstream), p(loss), p(grad),
-                                   int(accumulate), ops._stream()), "fsgs_balance_pairs")
-
-
-def _table(table, mask, ws, scale, upstream, loss, grad):
-    p, (N, M) = ops._ptr, table.shape
-    check(lib().fsgs_balance_table(N, M, _TYPES[table.dtype], p(table), table.stride(0) if N > 1 else M, p(mask), p(ws),
-                                   ws.numel(), scale, p(upstream), p(loss), p(grad), M, ops._stream()), "fsgs_balance_table")
-
-
-def _check_weights(weights, idx, M, mask):
-    _balance_check("balance_loss", weights, idx, M, mask)
-    ops._need(weights.dtype == torch.float32 and weights.shape == idx.shape, "balance_loss: weights must be float32 [N,K]")
-
-
-def _check_table(table, idx, mask):
-    _balance_check("table_balance_loss", table, idx, table.shape[-1] if table.dim() == 2 else 0, mask)
-    ops._need(table.dtype in _TYPES, "table_balance_loss: float32, bfloat16 or float16 table")
-
-
-def _rows_of(table):
-    """The table itself where its rows are runs of memory that do not overlap, else a copy."""
-    one = table.stride(1) == 1 or table.shape[1] == 1
-    return table if one and (table.stride(0) >= table.shape[1]) else table.contiguous()
-
-
-class _BalanceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weights, idx, M, mask):
-        weights = weights.contiguous()
-        with ops._on_device(weights.device):
-            counts, ws = _balance_count(idx, M, mask, _PAIRS)
-            loss = torch.empty((), device=weights.device)
-            _pairs(*idx.shape, M, weights, ws, 1.0, None, loss, None, False)
-        ctx.save_for_backward(ws)
-        ctx.size = (*idx.shape, M)
-        out = counts[:M]
-        ctx.mark_non_differentiable(out)
-        return loss, out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_loss, _):
-        ws, = ctx.saved_tensors
-        N, K, M = ctx.size
-        grad = torch.empty(N, K, device=ws.device)
-        with ops._on_device(ws.device):
-            _pairs(N, K, M, None, ws, 1.0, g_loss, None, grad, False)
-        return grad, None, None, None
-
-
 def balance_loss(weights, idx, M, mask=None):
     """``(loss, counts)``: how evenly the Gaussians use the ``M`` superpoints.  ``weights`` [N,K] float32 are the blend
     weights of each Gaussian's superpoints ``idx`` [N,K] int64 (``lbs_weights``, ``motion.kernel_weights``); ``counts``
@@ -167,46 +85,13 @@ def balance_loss(weights, idx, M, mask=None):
     is 1 when every superpoint has its share.  Differentiable in ``weights`` (the counts carry no gradient).  ``mask``
     (bool [N]): the Gaussians that count, ``n`` of them; an index outside 0 .. M-1 is a pair that does not count.  No
     Gaussian or no pair that counts: loss 0.  No synchronisation; the same inputs give the same bits."""
-    _check_weights(weights, idx, M, mask)
-    return _BalanceLoss.apply(weights, idx, int(M), mask)
+    return host().balance_pairs(weights, idx, int(M), mask, 1.0, None, True)
 
 
 def balance_value_and_grad(weights, idx, M, mask=None, weight=1.0, grad=None):
     """``(weight * loss, weight * dloss/dweights, counts)`` of ``balance_loss`` without autograd.  ``grad`` (float32 [N,K],
     contiguous): the gradient is added to it instead of written to a new tensor."""
-    _check_weights(weights, idx, M, mask)
-    ops._need(grad is None or (grad.shape == weights.shape and grad.dtype == torch.float32 and grad.is_contiguous() and
-                               grad.device == weights.device), "balance_value_and_grad: grad must be contiguous float32 [N,K]")
-    weights = weights.detach().contiguous()
-    with ops._on_device(weights.device):
-        counts, ws = _balance_count(idx, int(M), mask, _PAIRS)
-        loss = torch.empty((), device=weights.device)
-        out = torch.empty_like(weights) if grad is None else grad
-        _pairs(*idx.shape, int(M), weights, ws, float(weight), None, loss, out, grad is not None)
-    return loss, out, counts[:M]
-
-
-class _TableBalanceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, idx, mask):
-        table, mask = _rows_of(table), None if mask is None else mask.contiguous()
-        with ops._on_device(table.device):
-            counts, ws = _balance_count(idx, table.shape[1], mask, _TABLE)
-            loss = torch.empty((), device=table.device)
-            _table(table, mask, ws, 1.0, None, loss, None)
-        ctx.save_for_backward(table, mask, ws)
-        out = counts[:table.shape[1]]
-        ctx.mark_non_differentiable(out)
-        return loss, out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_loss, _):
-        table, mask, ws = ctx.saved_tensors
-        grad = torch.empty(table.shape, dtype=table.dtype, device=table.device)
-        with ops._on_device(table.device):
-            _table(table, mask, ws, 1.0, g_loss, None, grad)
-        return grad, None, None
+    return host().balance_pairs(weights, idx, int(M), mask, float(weight), grad, False)
 
 
 def table_balance_loss(table, idx, mask=None):
@@ -215,21 +100,13 @@ def table_balance_loss(table, idx, mask=None):
 
         ``loss = M * sum_m (counts_m / sum(counts)) * mean over the Gaussians of softmax(table)_m``
 
-    ``balance_loss`` with the probabilities of all superpoints in the place of the K blend weights; the gradient of the
-    table (in its type) is formed in the same pass over it that forms the softmax.  A row of nothing but -infinity adds
-    nothing.  ``mask``, indices outside 0 .. M-1 and ``counts`` as in ``balance_loss``."""
-    _check_table(table, idx, mask)
-    return _TableBalanceLoss.apply(table, idx, mask)
+    ``balance_loss`` with the probabilities of all superpoints in the place of the K blend weights, differentiable in
+    ``table`` (gradient in its type).  A row of nothing but -infinity adds nothing.  ``mask``, indices outside 0 .. M-1
+    and ``counts`` as in ``balance_loss``."""
+    return host().balance_table(table, idx, mask, 1.0, True)
 
 
 def table_balance_value_and_grad(table, idx, mask=None, weight=1.0):
     """``(weight * loss, weight * dloss/dtable, counts)`` of ``table_balance_loss`` without autograd: one pass that reads
     the table once and writes the gradient once."""
-    _check_table(table, idx, mask)
-    table, mask = _rows_of(table.detach()), None if mask is None else mask.contiguous()
-    with ops._on_device(table.device):
-        counts, ws = _balance_count(idx, table.shape[1], mask, _TABLE)
-        loss = torch.empty((), device=table.device)
-        grad = torch.empty(table.shape, dtype=table.dtype, device=table.device)
-        _table(table, mask, ws, float(weight), None, loss, grad)
-    return loss, grad, counts[:table.shape[1]]
+    return host().balance_table(table, idx, mask, float(weight), False)

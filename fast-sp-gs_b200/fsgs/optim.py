@@ -161,7 +161,7 @@ def grad_norm(tensors, max_norm=None):
     device = tensors[0].device
     with _on_device(device):
         out, work = torch.empty(2, device=device), _norm_workspace(device)
-        args = (_lib.address("fsgs_grad_norm"), float("inf") if max_norm is None else float(max_norm), work.data_ptr(),
+        args = (float("inf") if max_norm is None else float(max_norm), work.data_ptr(),
                 work.numel(), out.data_ptr(), _stream().value or 0)
         rc = _lib.host().norm(tensors, *args)
         if rc == _STRIDED:
@@ -415,8 +415,8 @@ class AdamW(torch.optim.Optimizer):
             work, clip = self._work[0], self.max_grad_norm is not None
             norm = (float(self.max_grad_norm), self._norm[1].data_ptr(), self._norm[1].numel(), self._norm[0].data_ptr()) \
                 if clip else (0.0, 0, 0, 0)
-            return _lib.host().step(plan.handle, self.param_groups, self.state, _lib.address("fsgs_adamw_multi"),
-                                    _lib.address("fsgs_grad_norm"), *norm, 0 if grad_scale is None else grad_scale.data_ptr(),
+            return _lib.host().step(plan.handle, self.param_groups, self.state, *norm,
+                                    0 if grad_scale is None else grad_scale.data_ptr(),
                                     0 if gate is None else gate.data_ptr(), work.data_ptr(), work.numel(),
                                     _stream().value or 0)
 

@@ -599,7 +599,7 @@ int fsgs_lbs_weights_backward(int P, int K, int M, const float *d2, const int64_
  * The counts carry no gradient.  T = 0 or n = 0: L = 0 and zero gradients.  A table row of nothing but -infinity adds
  * nothing to P.  What does not count has gradient 0 (added nothing), and its weights are not read into the sum.
  *
- * fsgs_balance_count: counts [M+2] = c, T, n, and into the workspace (16-byte aligned, needs no preparation) what the other
+ * fsgs_balance_count: counts [M+4] = c, T, n and two words of its own, and into the workspace (16-byte aligned, needs no preparation) what the other
  * two calls need: FSGS_BALANCE_PAIRS for fsgs_balance_pairs, FSGS_BALANCE_TABLE for fsgs_balance_table, which may then be
  * called any number of times, one after another, with the same workspace.  scale and *upstream (device, optional)
  * multiply the loss and the gradient.  loss (device, one float) and the gradient are both optional.  accumulate: the

@@ -216,3 +216,42 @@ def test_refusals():
                  lambda: table_balance_loss(torch.ones(4, 0, device="cuda"), idx), lambda: table_balance_loss(w, idx[:, 0])):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_autograd_of_the_losses():
+    """Through other operations on both sides, with an upstream factor on the device; no gradient asked for; the table
+    changed between the passes; a second derivative."""
+    from fsgs.loss import balance_loss, balance_value_and_grad, table_balance_loss, table_balance_value_and_grad
+    gen = torch.Generator().manual_seed(6)
+    N, K, M = 500, 3, 40
+    idx = _indices(N, K, M, gen).cuda()
+    raw, z = torch.randn(N, K, generator=gen).cuda(), torch.randn(N, M, generator=gen).cuda()
+    a = raw.clone().requires_grad_()
+    w = torch.softmax(a, dim=1)
+    loss, counts = balance_loss(w, idx, M)
+    assert not counts.requires_grad and loss.requires_grad
+    (loss ** 2).backward()
+    value, grad, _ = balance_value_and_grad(w, idx, M)
+    assert not value.requires_grad and not grad.requires_grad and torch.equal(value, loss.detach())
+    p = w.detach().double()
+    up = 2 * value.double() * grad.double()
+    want = p * (up - (p * up).sum(dim=1, keepdim=True))
+    assert float((a.grad.double() - want).abs().max()) <= 16 * E * float((p * up.abs()).max())
+    b = z.clone().requires_grad_()
+    loss, _ = table_balance_loss(b * 1.0, idx)
+    (3.0 * loss).backward()
+    _, grad, _ = table_balance_value_and_grad(z, idx)
+    assert float((b.grad - 3.0 * grad).abs().max()) <= 4 * E * 3.0 * float(grad.abs().max())
+    with torch.no_grad():
+        assert not table_balance_loss(b, idx)[0].requires_grad and not balance_loss(a, idx, M)[0].requires_grad
+    c = (z.clone().requires_grad_() * 1.0)
+    loss, _ = table_balance_loss(c, idx)
+    with torch.no_grad():
+        c += 1.0
+    with pytest.raises(RuntimeError, match="modified"):
+        loss.backward()
+    d = z.clone().requires_grad_()
+    loss, _ = table_balance_loss(d, idx)
+    g, = torch.autograd.grad(loss ** 2, d, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        g.sum().backward()
