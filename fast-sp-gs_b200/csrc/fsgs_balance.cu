@@ -21,52 +21,64 @@ constexpr int kBalSharedPoints = 8192;    // superpoints whose histogram or shar
 constexpr int kCountThreads = 1024;
 constexpr int kPairThreads = 512;
 constexpr int kTableThreads = 256;
-constexpr int kBalSlots = 1184;           // partial sums of the pairs form
+constexpr int kBalSlots = 296;            // partial sums
 
-// The workspace: this, the share of every superpoint as float32, then the codes of the pairs (pairs form) or the sums of
-// the thread blocks (table form).
+// The workspace: this, then the codes of the pairs (pairs form) or four copies of the shares, copy s moved up by s places
+// (table form).
 struct BalanceHead {
-  int closed, pad;          // ticket: blocks that have finished summing
-  double total, rows;       // T and n
-  double slots[kBalSlots];
+  int closed, bad;          // pairs: blocks that have finished summing; table: a sum that is not finite
+  long long dead;           // table: rows that count and have no probabilities
+  double slots[kBalSlots];  // pairs: the blocks' sums; table: kFixedSlots sums in fixed point
 };
+constexpr int kFixedSlots = 32;
+
+// floats of one copy of the shares
+static inline __host__ __device__ size_t share_copy(int M) { return ((size_t) M + 3 + 3) & ~(size_t) 3; }
 
 static inline size_t pad16(size_t n) { return (n + 15) & ~(size_t) 15; }
 static inline size_t code_bytes(int M) { return M < 65536 ? 2 : 4; }
 
 struct BalanceSpace {
   BalanceHead *head;
-  float *share;
-  void *codes;     // [N K]
-  double *sums;    // [blocks]
+  float *share;    // table form
+  void *codes;     // pairs form: [N K]
 };
 
-static BalanceSpace balance_space(void *ws, int M) {
+static BalanceSpace balance_space(void *ws) {
   BalanceSpace w;
   w.head = (BalanceHead *) ws;
-  w.share = (float *) ((char *) ws + pad16(sizeof(BalanceHead)));
-  w.codes = (char *) w.share + pad16(sizeof(float) * (size_t) M);
-  w.sums = (double *) w.codes;
+  w.codes = (char *) ws + pad16(sizeof(BalanceHead));
+  w.share = (float *) w.codes;
   return w;
+}
+
+// Table form: the sum over the rows of inner = sum_m p_m share_m is at most M + 1 in magnitude, any part of it too, and is
+// added in whole numbers of 2^-fixed_bits: the order of the additions does not change it.
+static inline __host__ __device__ int fixed_bits(int M) {
+  int bits = 1;
+  while (bits < 31 && (M >> bits) != 0) ++bits;
+  return 60 - bits;
 }
 
 // ---- counts -----------------------------------------------------------------------------------------------
 
 template <typename T>
-__device__ __forceinline__ T block_total(T v, T *scratch) {  // valid in thread 0
+__device__ __forceinline__ T block_total(T v, T *scratch) {  // valid in the first warp
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) scratch[threadIdx.x >> 5] = v;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  if (threadIdx.x == 0)
-    for (int w = 1; w < (int) (blockDim.x >> 5); ++w) v += scratch[w];
+  if (threadIdx.x < 32) {
+    v = lane < warps ? scratch[lane] : T(0);
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
   return v;
 }
 
 // One pass over the indices: a histogram per block in shared memory, added to the 64-bit counts at the end.  In the pairs
 // form the superpoint of every pair is kept as a 16- or 32-bit code (all ones: does not count) for the pass that needs the
-// complete counts, which then reads 2 bytes per pair instead of 8 and no mask.  The block that finishes last turns the
-// counts into shares.  Bound by the read of the indices and, beside it, by one shared-memory atomic per pair.
+// complete counts, which then reads 2 bytes per pair instead of 8 and no mask.  In the table form the block that finishes
+// last turns the counts into shares.  Bound by the read of the indices and, beside it, by one shared-memory atomic per pair.
 template <typename Code>
 __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long long N, int K, int M, const int64_t *__restrict__ idx,
     const uint8_t *__restrict__ mask, int wide, unsigned long long *__restrict__ counts, BalanceHead *__restrict__ head,
@@ -125,13 +137,15 @@ __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long lo
       if (c) atomicAdd(counts + m, (unsigned long long) c);
       named += c;
     }
-  named = block_total(named, s_red);
-  rows = block_total(rows, s_red);
+  // both sums in one: below 2^31 each in a block
+  const long long both = block_total((named << 32) + rows, s_red);
   if (threadIdx.x == 0) {
-    if (named) atomicAdd(counts + M, (unsigned long long) named);
-    if (!mask && blockIdx.x == 0) rows = N;
-    if (rows) atomicAdd(counts + M + 1, (unsigned long long) rows);
+    const unsigned long long n = !mask ? blockIdx.x == 0 ? (unsigned long long) N : 0 : (unsigned long long) (both & 0xffffffffll);
+    if (both >> 32) atomicAdd(counts + M, (unsigned long long) (both >> 32));
+    if (n) atomicAdd(counts + M + 1, n);
+    if (blockIdx.x == 0) head->closed = 0;
   }
+  if (codes) return;
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) s_last = atomicAdd(counts + M + 2, 1ull) == gridDim.x - 1;
@@ -139,12 +153,20 @@ __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long lo
   if (!s_last) return;
   __threadfence();
   const long long total = (long long) __ldcg(counts + M), n = (long long) __ldcg(counts + M + 1);
-  const bool any = total > 0 && n > 0;
-  const double unit = any ? 1.0 / ((double) total * (double) n) : 0.0;
-  const double mean = codes ? 0.0 : (double) total;
-  for (int m = threadIdx.x; m < M; m += kCountThreads)
-    share[m] = (float) (((double) M * (double) (long long) __ldcg(counts + m) - mean) * unit);
-  if (threadIdx.x == 0) head->closed = 0, head->total = any ? (double) total : 0.0, head->rows = any ? (double) n : 0.0;
+  const double unit = total > 0 && n > 0 ? 1.0 / ((double) total * (double) n) : 0.0;
+  const size_t copy = share_copy(M);
+  for (int m = threadIdx.x; m < M; m += kCountThreads) {
+    const float f = (float) (((double) M * (double) (long long) __ldcg(counts + m) - (double) total) * unit);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) share[k * copy + m + k] = f;
+  }
+  if (threadIdx.x < 4) {  // what a whole group reads beside its row's shares
+    float *c = share + threadIdx.x * copy;
+    for (int m = 0; m < (int) threadIdx.x; ++m) c[m] = 0.0f;
+    for (size_t m = (size_t) M + threadIdx.x; m < copy; ++m) c[m] = 0.0f;
+  }
+  if (threadIdx.x < kFixedSlots) ((long long *) head->slots)[threadIdx.x] = 0;
+  if (threadIdx.x == 0) head->bad = 0, head->dead = 0;
 }
 
 // ---- pairs form ---------------------------------------------------------------------------------------------
@@ -158,45 +180,49 @@ struct PairsArgs {
   float *loss, *g;                   // either may be null
   int accumulate;
   BalanceHead *head;
-  const float *share;
+  const long long *counts;
 };
 
 // Eight pairs per thread and turn: 16 bytes of codes, 32 of weights in, 32 of gradients out, the shares from shared memory.
 template <typename Code>
-__global__ void __launch_bounds__(kPairThreads, 3) balance_pairs_kernel(PairsArgs a, const Code *__restrict__ codes) {
+__global__ void __launch_bounds__(kPairThreads, 2) balance_pairs_kernel(PairsArgs a, const Code *__restrict__ codes) {
   extern __shared__ float s_share[];
   __shared__ double s_sum[kPairThreads / 32];
   __shared__ int s_last;
   const bool in_shared = a.M <= kBalSharedPoints;
+  const long long stride = (long long) gridDim.x * kPairThreads, first = (long long) blockIdx.x * kPairThreads + threadIdx.x;
+  const long long eights = a.wide ? a.pairs / 8 : 0;
+  constexpr int kWords = sizeof(Code) / 2;  // 16-byte words of eight codes
+  uint4 nc[kWords];
+  float4 nw[2] = {};
+  auto fetch = [&](long long q) {
+#pragma unroll
+    for (int u = 0; u < kWords; ++u) nc[u] = reinterpret_cast<const uint4 *>(codes)[kWords * q + u];
+    if (a.loss) nw[0] = reinterpret_cast<const float4 *>(a.w)[2 * q], nw[1] = reinterpret_cast<const float4 *>(a.w)[2 * q + 1];
+  };
+  if (first < eights) fetch(first);
+  const double parts = (double) a.counts[a.M] * (double) a.counts[a.M + 1], unit = parts > 0.0 ? (double) a.M / parts : 0.0;
   if (in_shared) {
-    for (int m = threadIdx.x; m < a.M; m += kPairThreads) s_share[m] = a.share[m];
+    for (int m = threadIdx.x; m < a.M; m += kPairThreads) s_share[m] = (float) ((double) a.counts[m] * unit);
     __syncthreads();
   }
   const float up = a.scale * (a.upstream ? *a.upstream : 1.0f);
   double sum = 0.0;
-  const long long stride = (long long) gridDim.x * kPairThreads, first = (long long) blockIdx.x * kPairThreads + threadIdx.x;
   // a weight that does not count is not read into the sum: it may be anything, a NaN too
   auto one = [&](Code c, float w, float &part) {
     const bool on = c != (Code) ~(Code) 0;
-    const float share = !on ? 0.0f : in_shared ? s_share[c] : a.share[c];
+    const float share = !on ? 0.0f : in_shared ? s_share[c] : (float) ((double) a.counts[c] * unit);
     if (on) part = fmaf(w, share, part);
     return up * share;
   };
-  const long long eights = a.wide ? a.pairs / 8 : 0;
   for (long long q = first; q < eights; q += stride) {
+    if (q != first) fetch(q);
     alignas(16) Code c[8];
-    if (sizeof(Code) == 2) {
-      *reinterpret_cast<uint4 *>(c) = reinterpret_cast<const uint4 *>(codes)[q];
-    } else {
-      reinterpret_cast<uint4 *>(c)[0] = reinterpret_cast<const uint4 *>(codes)[2 * q];
-      reinterpret_cast<uint4 *>(c)[1] = reinterpret_cast<const uint4 *>(codes)[2 * q + 1];
-    }
-    alignas(16) float w[8] = {};
+    alignas(16) float w[8];
+#pragma unroll
+    for (int u = 0; u < kWords; ++u) reinterpret_cast<uint4 *>(c)[u] = nc[u];
+    reinterpret_cast<float4 *>(w)[0] = nw[0], reinterpret_cast<float4 *>(w)[1] = nw[1];
     float g[8], part = 0.0f;
-    if (a.loss) {
-      *reinterpret_cast<float4 *>(w) = reinterpret_cast<const float4 *>(a.w)[2 * q];
-      *reinterpret_cast<float4 *>(w + 4) = reinterpret_cast<const float4 *>(a.w)[2 * q + 1];
-    }
 #pragma unroll
     for (int u = 0; u < 8; ++u) g[u] = one(c[u], w[u], part);
     sum += (double) part;
@@ -244,8 +270,7 @@ struct TableArgs {
   const float *upstream;
   void *g;
   const float *share;
-  double *sums;                      // null: no loss; one per block: sum of inner + rows / n
-  const BalanceHead *head;
+  BalanceHead *head;                 // null: no loss
 };
 
 __device__ __forceinline__ float get(const float *p) { return *p; }
@@ -272,10 +297,14 @@ __device__ __forceinline__ void put4(H *p, const float *x) {
   *reinterpret_cast<uint2 *>(p) = v;
 }
 
-// max / sum over the G threads that share a row (part of a warp, a warp, or the block)
+// max / sum over the G threads that share a row (part of a warp, a warp, or the block); NaN are passed over by the max
 template <int G>
 __device__ __forceinline__ float row_max(float v, float *scratch) {
-  for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if (G < 32) {
+    for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  }
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(v) : "f"(v));
   if (G > 32) {
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
     __syncthreads();
@@ -299,40 +328,65 @@ __device__ __forceinline__ float2 row_sum(float2 v, float2 *scratch) {
   return v;
 }
 
-// G threads per row, one row each, V neighbouring columns per access and PER columns per thread in all (PER 0: any number
-// of columns, the row is read again for each of three passes).  The row stays in registers from its one read to the write
-// of its gradient; the grid covers the rows and leaves the order to the hardware.
-template <typename T, int G, int V, int PER>
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// G threads per row, one row each, PER columns per thread in groups of four neighbours (PER 0: any number of columns, the
+// row is read again for each of three passes).  The groups are those of memory: where a row starts s elements past a
+// boundary of four, group k holds columns 4 k - s .. 4 k - s + 3, so that groups are one access whatever the width of the
+// table, and the shares come from the copy that is moved up by s.  What a group holds beside its row belongs to the
+// neighbouring rows; it is read and not used (the first and the last rows read element by element where there is no such
+// neighbour).  exp(z - max) is the hardware's exp2 of (z - max) log2(e); the difference is taken first, because z log2(e)
+// overflows for the type's lowest value, which stands for masked columns in places.  The row stays in registers from its
+// one read to the write of its gradient; the grid covers the rows and leaves the order to the hardware.
+template <typename T, int G, int PER>
 __global__ void __launch_bounds__(kTableThreads) balance_table_kernel(TableArgs a) {
+  constexpr float kLog2e = 1.44269504f;
+  constexpr int kRows = kTableThreads / G;
   __shared__ float s_max[kTableThreads / 32];
   __shared__ float2 s_sum[kTableThreads / 32];
-  __shared__ double s_total[kTableThreads / 32];
+  __shared__ float s_inner[kRows];  // of the block's rows; NaN and infinities pass through
+  __shared__ int s_dead[kRows];
   const int t = threadIdx.x % G;
-  const long long i = (long long) blockIdx.x * (kTableThreads / G) + threadIdx.x / G;
+  const long long i = (long long) blockIdx.x * kRows + threadIdx.x / G;
   const bool here = i < a.N, on = here && (!a.mask || a.mask[i] != 0);
-  const T *z = (const T *) a.table + (here ? i : 0) * a.stride;
+  const long long start = (here ? i : 0) * a.stride;
+  const T *z = (const T *) a.table + start;
   T *g = a.g && here ? (T *) a.g + i * a.g_stride : nullptr;
-  constexpr int R = PER > 0 ? PER : V;
+  const int moved = (int) ((uintptr_t) z / sizeof(T) & 3);
+  const float *copy = a.share + moved * share_copy(a.M);  // copy[m + moved] = share of m
+  const bool inside = start >= 3 && start + a.M + 3 <= (a.N - 1) * a.stride + a.M;  // groups may reach past the row
+  constexpr int R = PER > 0 ? PER : 4;
   alignas(16) float x[R], sh[R];  // values, then exponentials; shares
   float top = -INFINITY;
   if (PER > 0) {
 #pragma unroll
-    for (int u = 0; u < PER; u += V) {
-      const int m = (u / V * G + t) * V;
-      if (V == 4 && on && m + V <= a.M) {
+    for (int u = 0; u < PER; u += 4) {
+      const int k = u * G + 4 * t, m = k - moved;
+      const bool part = m < 0 || m + 4 > a.M;
+      if (!on || m >= a.M) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[u + j] = -INFINITY, sh[u + j] = 0.0f;
+        continue;
+      }
+      get4(copy + k, sh + u);
+      if (inside || !part) {
         get4(z + m, x + u);
-        get4(a.share + m, sh + u);
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const bool in = on && m + j < a.M;
-          x[u + j] = in ? get(z + m + j) : -INFINITY;
-          sh[u + j] = in ? a.share[m + j] : 0.0f;
-        }
+        for (int j = 0; j < 4; ++j) x[u + j] = m + j >= 0 && m + j < a.M ? get(z + m + j) : -INFINITY;
+      }
+      if (part) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (m + j < 0 || m + j >= a.M) x[u + j] = -INFINITY;
       }
     }
 #pragma unroll
-    for (int u = 0; u < PER; ++u) top = fmaxf(top, x[u]);  // passes over a NaN; the row's sum below does not
+    for (int u = 0; u < PER; ++u) top = fmaxf(top, x[u]);
   } else if (on) {
     for (int m = t; m < a.M; m += G) top = fmaxf(top, get(z + m));
   }
@@ -343,75 +397,91 @@ __global__ void __launch_bounds__(kTableThreads) balance_table_kernel(TableArgs 
   if (PER > 0) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      x[u] = expf(x[u] - base);
+      x[u] = fast_exp2((x[u] - base) * kLog2e);
       s.x += x[u], s.y = fmaf(x[u], sh[u], s.y);
     }
   } else if (on) {
     for (int m = t; m < a.M; m += G) {
-      const float e = expf(get(z + m) - base);
-      s.x += e, s.y = fmaf(e, a.share[m], s.y);
+      const float e = fast_exp2((get(z + m) - base) * kLog2e);
+      s.x += e, s.y = fmaf(e, copy[m + moved], s.y);
     }
   }
   s = row_sum<G>(s, s_sum);
-  const float inv = s.x == 0.0f ? 0.0f : 1.0f / s.x, inner = s.y * inv;
+  const float inv = s.x == 0.0f ? 0.0f : __fdividef(1.0f, s.x), inner = s.y * inv;
   if (g) {
-    const float k = a.scale * (a.upstream ? *a.upstream : 1.0f) * inv;
+    const float k = a.scale * (a.upstream ? *a.upstream : 1.0f) * inv, less = -k * inner;
+    const bool alike = (int) ((uintptr_t) g / sizeof(T) & 3) == moved;  // the gradient's groups lie as the table's
     if (PER > 0) {
 #pragma unroll
-      for (int u = 0; u < PER; u += V) {
-        const int m = (u / V * G + t) * V;
-        if (V == 4 && m + V <= a.M) {
+      for (int u = 0; u < PER; u += 4) {
+        const int m = u * G + 4 * t - moved;
+        if (m >= a.M) continue;
 #pragma unroll
-          for (int j = 0; j < V; ++j) x[u + j] = on ? k * x[u + j] * (sh[u + j] - inner) : 0.0f;
+        for (int j = 0; j < 4; ++j) x[u + j] = on ? x[u + j] * fmaf(k, sh[u + j], less) : 0.0f;
+        if (alike && m >= 0 && m + 4 <= a.M) {
           put4(g + m, x + u);
         } else {
 #pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (m + j < a.M) put(g + m + j, on ? k * x[u + j] * (sh[u + j] - inner) : 0.0f);
+          for (int j = 0; j < 4; ++j)
+            if (m + j >= 0 && m + j < a.M) put(g + m + j, x[u + j]);
         }
       }
     } else {
-      for (int m = t; m < a.M; m += G) put(g + m, on ? k * expf(get(z + m) - base) * (a.share[m] - inner) : 0.0f);
+      for (int m = t; m < a.M; m += G)
+        put(g + m, on ? fast_exp2((get(z + m) - base) * kLog2e) * fmaf(k, copy[m + moved], less) : 0.0f);
     }
   }
-  if (!a.sums) return;
-  double sum = 0.0;
-  if (t == 0 && on && s.x != 0.0f && a.head->rows > 0.0) sum = 1.0 / a.head->rows + (double) inner;
-  sum = block_total(sum, s_total);
-  if (threadIdx.x == 0) a.sums[blockIdx.x] = sum;
+  if (!a.head) return;
+  if (t == 0) s_inner[threadIdx.x / G] = on ? inner : 0.0f, s_dead[threadIdx.x / G] = on && s.x == 0.0f;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double sum = 0.0;
+    int dead = 0;
+    for (int r = 0; r < kRows; ++r) sum += (double) s_inner[r], dead += s_dead[r];
+    const bool fine = fabs(sum) <= 2.0 * a.M;
+    if (fine) atomicAdd((unsigned long long *) a.head->slots + blockIdx.x % kFixedSlots,
+                        (unsigned long long) __double2ll_rn(ldexp(sum, fixed_bits(a.M))));
+    else atomicOr(&a.head->bad, 1);
+    if (dead) atomicAdd((unsigned long long *) &a.head->dead, (unsigned long long) dead);
+  }
 }
 
-// The blocks' sums in a fixed order.
-__global__ void __launch_bounds__(1024) balance_close_kernel(int n, const double *__restrict__ sums, float scale,
+// The loss from the sums; rows with probabilities add 1 / n each, what the shares were centred by.  Leaves the sums at zero.
+__global__ void __launch_bounds__(32) balance_close_kernel(BalanceHead *head, const long long *__restrict__ counts, int M, float scale,
     const float *__restrict__ upstream, float *__restrict__ loss) {
-  __shared__ double s_sum[32];
-  double sum = 0.0;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n; i += 1024) sum += sums[i];
-  sum = block_total(sum, s_sum);
-  if (threadIdx.x == 0) *loss = (float) (sum * (double) (scale * (upstream ? *upstream : 1.0f)));
+  long long *slot = (long long *) head->slots + threadIdx.x, sum = *slot;
+  *slot = 0;
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (threadIdx.x != 0) return;
+  const double n = (double) counts[M + 1], up = (double) (scale * (upstream ? *upstream : 1.0f));
+  const double value = n > 0.0 && counts[M] > 0 ? ldexp((double) sum, -fixed_bits(M)) + (n - (double) head->dead) / n : 0.0;
+  *loss = head->bad ? NAN : (float) (value * up);
+  head->bad = 0, head->dead = 0;
 }
+static_assert(kFixedSlots == 32, "one warp closes the sum");
 
-static int rows_per_block(int M) { return M <= 64 ? kTableThreads / 8 : M <= 512 ? kTableThreads / 32 : 1; }
+// `reach`: columns from the first group of four to the row's end, M where every row starts on a boundary of four elements
+static int rows_per_block(int reach) { return reach <= 64 ? kTableThreads / 8 : reach <= 512 ? kTableThreads / 32 : 1; }
 
-template <typename T, int G, int V, int PER>
-static int table_launch(const TableArgs &a, cudaStream_t st) {
-  balance_table_kernel<T, G, V, PER><<<(int) ((a.N + kTableThreads / G - 1) / (kTableThreads / G)), kTableThreads, 0, st>>>(a);
+template <typename T, int G, int PER>
+static int table_launch(const TableArgs &a, int64_t blocks, cudaStream_t st) {
+  balance_table_kernel<T, G, PER><<<(int) blocks, kTableThreads, 0, st>>>(a);
   FSGS_LAUNCH_CHECK();
   return FSGS_OK;
 }
 
-template <typename T, int V>
-static int table_pick(const TableArgs &a, cudaStream_t st) {
-  if (a.M <= 64) return table_launch<T, 8, V, 8>(a, st);
-  if (a.M <= 128) return table_launch<T, 32, V, 4>(a, st);
-  if (a.M <= 256) return table_launch<T, 32, V, 8>(a, st);
-  if (a.M <= 512) return table_launch<T, 32, V, 16>(a, st);
-  if (a.M <= 1024) return table_launch<T, 256, V, 4>(a, st);
-  if (a.M <= 2048) return table_launch<T, 256, V, 8>(a, st);
-  if (a.M <= 4096) return table_launch<T, 256, V, 16>(a, st);
-  if (a.M <= 8192) return table_launch<T, 256, V, 32>(a, st);
-  return table_launch<T, 256, 1, 0>(a, st);
+template <typename T>
+static int table_pick(const TableArgs &a, int reach, int64_t blocks, cudaStream_t st) {
+  if (reach <= 64) return table_launch<T, 8, 8>(a, blocks, st);
+  if (reach <= 128) return table_launch<T, 32, 4>(a, blocks, st);
+  if (reach <= 256) return table_launch<T, 32, 8>(a, blocks, st);
+  if (reach <= 384) return table_launch<T, 32, 12>(a, blocks, st);
+  if (reach <= 512) return table_launch<T, 32, 16>(a, blocks, st);
+  if (reach <= 1024) return table_launch<T, 256, 4>(a, blocks, st);
+  if (reach <= 2048) return table_launch<T, 256, 8>(a, blocks, st);
+  if (reach <= 4096) return table_launch<T, 256, 16>(a, blocks, st);
+  if (reach <= 8192) return table_launch<T, 256, 32>(a, blocks, st);
+  return table_launch<T, 256, 0>(a, blocks, st);
 }
 
 static bool balance_sizes(int64_t N, int64_t per_row) { return N <= (1ll << 36) / per_row; }
@@ -426,10 +496,9 @@ static int balance_blocks(int64_t work, int threads, int most) {
 using namespace fsgs;
 
 extern "C" size_t fsgs_balance_workspace_bytes(int64_t N, int K, int M, int form) {
-  if (N < 0 || K <= 0 || M <= 0 || !balance_sizes(N, form == FSGS_BALANCE_TABLE && M > K ? M : K) || (form != FSGS_BALANCE_PAIRS && form != FSGS_BALANCE_TABLE)) return 0;
-  const size_t more = form == FSGS_BALANCE_PAIRS ? (size_t) N * K * code_bytes(M)
-                                                 : sizeof(double) * ((size_t) N / rows_per_block(M) + 1);
-  return pad16(sizeof(BalanceHead)) + pad16(sizeof(float) * (size_t) M) + pad16(more);
+  const bool table = form == FSGS_BALANCE_TABLE;
+  if (N < 0 || K <= 0 || M <= 0 || !balance_sizes(N, table && M > K ? M : K) || (!table && form != FSGS_BALANCE_PAIRS)) return 0;
+  return pad16(sizeof(BalanceHead)) + (table ? 4 * sizeof(float) * share_copy(M) : pad16((size_t) N * K * code_bytes(M)));
 }
 
 static bool balance_workspace(int64_t N, int K, int M, int form, const void *workspace, size_t bytes) {
@@ -442,7 +511,7 @@ extern "C" int fsgs_balance_count(int64_t N, int K, int M, const int64_t *idx, c
   if (!balance_sizes(N, form == FSGS_BALANCE_TABLE && M > K ? M : K)) return FSGS_ERR_LIMIT;
   if (!balance_workspace(N, K, M, form, workspace, workspace_bytes)) return FSGS_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t) stream;
-  const BalanceSpace w = balance_space(workspace, M);
+  const BalanceSpace w = balance_space(workspace);
   if (cudaMemsetAsync(counts, 0, sizeof(int64_t) * ((size_t) M + 4), st) != cudaSuccess) return FSGS_ERR_LAUNCH;
   const int grid = balance_blocks((N * K + 3) / 4, kCountThreads, 2 * 148);
   const size_t smem = M <= kBalSharedPoints ? sizeof(int) * ((size_t) M + 1) : 0;
@@ -455,17 +524,17 @@ extern "C" int fsgs_balance_count(int64_t N, int K, int M, const int64_t *idx, c
   return FSGS_OK;
 }
 
-extern "C" int fsgs_balance_pairs(int64_t N, int K, int M, const float *weights, void *workspace, size_t workspace_bytes,
-    float scale, const float *upstream, float *loss, float *g_weights, int accumulate, fsgs_stream_t stream) {
-  FSGS_REQUIRE(N >= 0 && K > 0 && M > 0 && (weights || !loss || N == 0));
+extern "C" int fsgs_balance_pairs(int64_t N, int K, int M, const float *weights, const int64_t *counts, void *workspace,
+    size_t workspace_bytes, float scale, const float *upstream, float *loss, float *g_weights, int accumulate, fsgs_stream_t stream) {
+  FSGS_REQUIRE(N >= 0 && K > 0 && M > 0 && counts && (weights || !loss || N == 0));
   if (!balance_sizes(N, K)) return FSGS_ERR_LIMIT;
   if (!balance_workspace(N, K, M, FSGS_BALANCE_PAIRS, workspace, workspace_bytes)) return FSGS_ERR_WORKSPACE;
   if (!loss && (!g_weights || N == 0)) return FSGS_OK;
   cudaStream_t st = (cudaStream_t) stream;
-  const BalanceSpace w = balance_space(workspace, M);
+  const BalanceSpace w = balance_space(workspace);
   const int wide = (((uintptr_t) weights | (uintptr_t) g_weights) & 15) == 0;
-  const PairsArgs a = {N * K, M, wide, weights, scale, upstream, loss, g_weights, accumulate, w.head, w.share};
-  const int grid = balance_blocks((N * K + 7) / 8, kPairThreads, 3 * 148);
+  const PairsArgs a = {N * K, M, wide, weights, scale, upstream, loss, g_weights, accumulate, w.head, (const long long *) counts};
+  const int grid = balance_blocks((N * K + 7) / 8, kPairThreads, kBalSlots);
   const size_t smem = M <= kBalSharedPoints ? sizeof(float) * (size_t) M : 0;
   if (code_bytes(M) == 2) balance_pairs_kernel<uint16_t><<<grid, kPairThreads, smem, st>>>(a, (const uint16_t *) w.codes);
   else balance_pairs_kernel<uint32_t><<<grid, kPairThreads, smem, st>>>(a, (const uint32_t *) w.codes);
@@ -474,28 +543,27 @@ extern "C" int fsgs_balance_pairs(int64_t N, int K, int M, const float *weights,
 }
 
 extern "C" int fsgs_balance_table(int64_t N, int M, int type, const void *table, int64_t row_stride, const uint8_t *mask,
-    void *workspace, size_t workspace_bytes, float scale, const float *upstream, float *loss, void *g_table,
+    const int64_t *counts, void *workspace, size_t workspace_bytes, float scale, const float *upstream, float *loss, void *g_table,
     int64_t g_row_stride, fsgs_stream_t stream) {
-  FSGS_REQUIRE(N >= 0 && M > 0 && (table || N == 0) && row_stride >= M && (!g_table || g_row_stride >= M));
+  FSGS_REQUIRE(N >= 0 && M > 0 && counts && (table || N == 0) && row_stride >= M && (!g_table || g_row_stride >= M));
   FSGS_REQUIRE(type == FSGS_F32 || type == FSGS_BF16 || type == FSGS_F16);
   if (!balance_sizes(N, M)) return FSGS_ERR_LIMIT;
   if (!balance_workspace(N, 1, M, FSGS_BALANCE_TABLE, workspace, workspace_bytes)) return FSGS_ERR_WORKSPACE;
   if (!loss && (!g_table || N == 0)) return FSGS_OK;
   cudaStream_t st = (cudaStream_t) stream;
-  if (N == 0) return cudaMemsetAsync(loss, 0, sizeof(float), st) == cudaSuccess ? FSGS_OK : FSGS_ERR_LAUNCH;
-  const BalanceSpace w = balance_space(workspace, M);
-  const int64_t blocks = (N + rows_per_block(M) - 1) / rows_per_block(M);
+  const BalanceSpace w = balance_space(workspace);
+  const bool plain = row_stride % 4 == 0 && (uintptr_t) table % (type == FSGS_F32 ? 16 : 8) == 0;
+  const int reach = M + (plain ? 0 : 3), rows = rows_per_block(reach);
+  const int64_t blocks = (N + rows - 1) / rows;
   if (blocks > INT32_MAX) return FSGS_ERR_LIMIT;
-  const TableArgs a = {N, row_stride, g_row_stride, M, table, mask, scale, upstream, g_table, w.share, loss ? w.sums : nullptr, w.head};
-  // four columns per access where every row of both tables starts on a boundary of four elements
-  const size_t four = type == FSGS_F32 ? 16 : 8;
-  const bool wide = row_stride % 4 == 0 && (uintptr_t) table % four == 0 && (!g_table || (g_row_stride % 4 == 0 && (uintptr_t) g_table % four == 0));
-  int rc;
-  if (type == FSGS_F32) rc = wide ? table_pick<float, 4>(a, st) : table_pick<float, 1>(a, st);
-  else if (type == FSGS_BF16) rc = wide ? table_pick<__nv_bfloat16, 4>(a, st) : table_pick<__nv_bfloat16, 1>(a, st);
-  else rc = wide ? table_pick<__half, 4>(a, st) : table_pick<__half, 1>(a, st);
-  if (rc != FSGS_OK || !loss) return rc;
-  balance_close_kernel<<<1, 1024, 0, st>>>((int) blocks, w.sums, scale, upstream, loss);
+  if (blocks > 0) {
+    const TableArgs a = {N, row_stride, g_row_stride, M, table, mask, scale, upstream, g_table, w.share, loss ? w.head : nullptr};
+    const int rc = type == FSGS_F32 ? table_pick<float>(a, reach, blocks, st) : type == FSGS_BF16 ? table_pick<__nv_bfloat16>(a, reach, blocks, st)
+                                                                                              : table_pick<__half>(a, reach, blocks, st);
+    if (rc != FSGS_OK) return rc;
+  }
+  if (!loss) return FSGS_OK;
+  balance_close_kernel<<<1, kFixedSlots, 0, st>>>(w.head, (const long long *) counts, M, scale, upstream, loss);
   FSGS_LAUNCH_CHECK();
   return FSGS_OK;
 }

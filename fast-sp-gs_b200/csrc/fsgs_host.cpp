@@ -30,9 +30,10 @@ struct {
   NormFn norm;
   size_t (*balance_bytes)(int64_t, int, int, int);
   int (*balance_count)(int64_t, int, int, const int64_t *, const uint8_t *, int, int64_t *, void *, size_t, fsgs_stream_t);
-  int (*balance_pairs)(int64_t, int, int, const float *, void *, size_t, float, const float *, float *, float *, int, fsgs_stream_t);
-  int (*balance_table)(int64_t, int, int, const void *, int64_t, const uint8_t *, void *, size_t, float, const float *, float *,
-      void *, int64_t, fsgs_stream_t);
+  int (*balance_pairs)(int64_t, int, int, const float *, const int64_t *, void *, size_t, float, const float *, float *, float *,
+      int, fsgs_stream_t);
+  int (*balance_table)(int64_t, int, int, const void *, int64_t, const uint8_t *, const int64_t *, void *, size_t, float,
+      const float *, float *, void *, int64_t, fsgs_stream_t);
   const char *(*status_string)(int);
 } lib;
 
@@ -307,18 +308,18 @@ Counted count(const char *what, const Tensor &idx, int64_t M, const std::optiona
   return c;
 }
 
-void pairs(int64_t N, int64_t K, int64_t M, const float *weights, const Tensor &ws, float scale, const float *upstream, float *loss,
-    float *grad, bool accumulate) {
-  check(lib.balance_pairs(N, (int) K, (int) M, weights, ws.data_ptr(), (size_t) ws.numel(), scale, upstream, loss, grad, accumulate,
-                          stream_of(ws)),
+void pairs(int64_t N, int64_t K, const Counted &c, const float *weights, float scale, const float *upstream, float *loss, float *grad,
+    bool accumulate) {
+  check(lib.balance_pairs(N, (int) K, (int) c.counts.numel() - 4, weights, c.counts.data_ptr<int64_t>(), c.ws.data_ptr(),
+                          (size_t) c.ws.numel(), scale, upstream, loss, grad, accumulate, stream_of(c.ws)),
         "fsgs_balance_pairs");
 }
 
-void table_pass(const Tensor &t, int type, const std::optional<Tensor> &mask, const Tensor &ws, float scale, const float *upstream,
+void table_pass(const Tensor &t, int type, const std::optional<Tensor> &mask, const Counted &c, float scale, const float *upstream,
     float *loss, void *grad) {
   const int64_t N = t.size(0), M = t.size(1);
-  check(lib.balance_table(N, (int) M, type, t.data_ptr(), N > 1 ? t.stride(0) : M, bytes_of(mask), ws.data_ptr(), (size_t) ws.numel(),
-                          scale, upstream, loss, grad, M, stream_of(ws)),
+  check(lib.balance_table(N, (int) M, type, t.data_ptr(), N > 1 ? t.stride(0) : M, bytes_of(mask), c.counts.data_ptr<int64_t>(),
+                          c.ws.data_ptr(), (size_t) c.ws.numel(), scale, upstream, loss, grad, M, stream_of(c.ws)),
         "fsgs_balance_table");
 }
 
@@ -340,19 +341,20 @@ struct PairsLoss : torch::autograd::Function<PairsLoss> {
     const Tensor w = weights.contiguous();
     const Counted c = count(kPairs, idx, M, dense(mask), FSGS_BALANCE_PAIRS);
     Tensor loss = at::empty({}, w.options().requires_grad(false)), counts = c.counts.narrow(0, 0, M);
-    pairs(idx.size(0), idx.size(1), M, w.data_ptr<float>(), c.ws, 1.0f, nullptr, loss.data_ptr<float>(), nullptr, false);
-    ctx->save_for_backward({c.ws});
-    ctx->saved_data["N"] = idx.size(0), ctx->saved_data["K"] = idx.size(1), ctx->saved_data["M"] = M;
+    pairs(idx.size(0), idx.size(1), c, w.data_ptr<float>(), 1.0f, nullptr, loss.data_ptr<float>(), nullptr, false);
+    ctx->save_for_backward({c.counts, c.ws});
+    ctx->saved_data["N"] = idx.size(0), ctx->saved_data["K"] = idx.size(1);
     ctx->mark_non_differentiable({counts});
     return {loss, counts};
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    const Tensor ws = ctx->get_saved_variables()[0];
-    const c10::cuda::CUDAGuard guard(ws.device());
+    const auto saved = ctx->get_saved_variables();
+    const Counted c{saved[0], saved[1]};
+    const c10::cuda::CUDAGuard guard(c.ws.device());
     const int64_t N = ctx->saved_data["N"].toInt(), K = ctx->saved_data["K"].toInt();
     Tensor grad = at::empty({N, K}, g[0].options().requires_grad(false));
-    pairs(N, K, ctx->saved_data["M"].toInt(), nullptr, ws, 1.0f, g[0].data_ptr<float>(), nullptr, grad.data_ptr<float>(), false);
+    pairs(N, K, c, nullptr, 1.0f, g[0].data_ptr<float>(), nullptr, grad.data_ptr<float>(), false);
     return {once(grad, g[0]), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -364,8 +366,8 @@ struct TableLoss : torch::autograd::Function<TableLoss> {
     const auto m = dense(mask);
     const Counted c = count(kTable, idx, t.size(1), m, FSGS_BALANCE_TABLE);
     Tensor loss = at::empty({}, t.options().dtype(at::kFloat).requires_grad(false)), counts = c.counts.narrow(0, 0, t.size(1));
-    table_pass(t, type_of(t.scalar_type()), m, c.ws, 1.0f, nullptr, loss.data_ptr<float>(), nullptr);
-    ctx->save_for_backward({t, m ? *m : Tensor(), c.ws});
+    table_pass(t, type_of(t.scalar_type()), m, c, 1.0f, nullptr, loss.data_ptr<float>(), nullptr);
+    ctx->save_for_backward({t, m ? *m : Tensor(), c.counts, c.ws});
     ctx->mark_non_differentiable({counts});
     return {loss, counts};
   }
@@ -375,8 +377,8 @@ struct TableLoss : torch::autograd::Function<TableLoss> {
     const Tensor &t = saved[0];
     const c10::cuda::CUDAGuard guard(t.device());
     Tensor grad = at::empty(t.sizes(), t.options().requires_grad(false));
-    table_pass(t, type_of(t.scalar_type()), saved[1].defined() ? std::optional<Tensor>(saved[1]) : std::nullopt, saved[2], 1.0f,
-               g[0].data_ptr<float>(), nullptr, grad.data_ptr());
+    table_pass(t, type_of(t.scalar_type()), saved[1].defined() ? std::optional<Tensor>(saved[1]) : std::nullopt,
+               Counted{saved[2], saved[3]}, 1.0f, g[0].data_ptr<float>(), nullptr, grad.data_ptr());
     return {once(grad, g[0]), Tensor(), Tensor()};
   }
 };
@@ -426,7 +428,7 @@ PyObject *balance_pairs(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Counted c = count(kPairs, idx, M, dense(mask), FSGS_BALANCE_PAIRS);
     Tensor loss = at::empty({}, w.options().requires_grad(false));
     if (!add) grad = at::empty(w.sizes(), w.options().requires_grad(false));
-    pairs(idx.size(0), idx.size(1), M, w.data_ptr<float>(), c.ws, weight, nullptr, loss.data_ptr<float>(), grad.data_ptr<float>(), add);
+    pairs(idx.size(0), idx.size(1), c, w.data_ptr<float>(), weight, nullptr, loss.data_ptr<float>(), grad.data_ptr<float>(), add);
     return tuple_of({loss, grad, c.counts.narrow(0, 0, M)});
   } catch (const std::exception &e) {
     return refuse(e.what());
@@ -454,7 +456,7 @@ PyObject *balance_table(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Counted c = count(kTable, idx, t.size(1), m, FSGS_BALANCE_TABLE);
     Tensor loss = at::empty({}, t.options().dtype(at::kFloat).requires_grad(false));
     Tensor grad = at::empty(t.sizes(), t.options().requires_grad(false));
-    table_pass(t, type, m, c.ws, weight, nullptr, loss.data_ptr<float>(), grad.data_ptr());
+    table_pass(t, type, m, c, weight, nullptr, loss.data_ptr<float>(), grad.data_ptr());
     return tuple_of({loss, grad, c.counts.narrow(0, 0, t.size(1))});
   } catch (const std::exception &e) {
     return refuse(e.what());

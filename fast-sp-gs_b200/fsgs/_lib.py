@@ -137,9 +137,9 @@ SYMBOLS = {
     "fsgs_grad_norm": (c_int, [c_int, _vp, c_float, _vp, c_size_t, _vp, _vp]),
     "fsgs_balance_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
     "fsgs_balance_count": (c_int, [c_int64, c_int, c_int, _vp, _vp, c_int, _vp, _vp, c_size_t, _vp]),
-    "fsgs_balance_pairs": (c_int, [c_int64, c_int, c_int, _vp, _vp, c_size_t, c_float, _vp, _vp, _vp, c_int, _vp]),
-    "fsgs_balance_table": (c_int, [c_int64, c_int, c_int, _vp, c_int64, _vp, _vp, c_size_t, c_float, _vp, _vp, _vp, c_int64,
-                                   _vp]),
+    "fsgs_balance_pairs": (c_int, [c_int64, c_int, c_int, _vp, _vp, _vp, c_size_t, c_float, _vp, _vp, _vp, c_int, _vp]),
+    "fsgs_balance_table": (c_int, [c_int64, c_int, c_int, _vp, c_int64, _vp, _vp, _vp, c_size_t, c_float, _vp, _vp, _vp,
+                                   c_int64, _vp]),
     "fsgs_view_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int64, c_int, c_int]),
     "fsgs_motion_param_count": (c_int64, [POINTER(MotionCfg)]),
     "fsgs_motion_param_offsets": (c_int, [POINTER(MotionCfg), POINTER(c_int64), POINTER(c_int32)]),

@@ -601,22 +601,23 @@ int fsgs_lbs_weights_backward(int P, int K, int M, const float *d2, const int64_
  *
  * fsgs_balance_count: counts [M+4] = c, T, n and two words of its own, and into the workspace (16-byte aligned, needs no preparation) what the other
  * two calls need: FSGS_BALANCE_PAIRS for fsgs_balance_pairs, FSGS_BALANCE_TABLE for fsgs_balance_table, which may then be
- * called any number of times, one after another, with the same workspace.  scale and *upstream (device, optional)
+ * called any number of times, one after another, with the same counts and workspace.  scale and *upstream (device, optional)
  * multiply the loss and the gradient.  loss (device, one float) and the gradient are both optional.  accumulate: the
  * gradient is added to g_weights.  fsgs_balance_table: rows of M elements of `type`, row_stride / g_row_stride elements
- * apart; g_table has the table's type; its workspace is that of any K.  Sums are added in a fixed order: the same inputs
- * give the same bits.  N K <= 2^36, and N M <= 2^36 in the table form.
+ * apart; g_table has the table's type; its workspace is that of any K.  The order in which blocks finish does not change
+ * the sums: the same inputs give the same bits.  N K <= 2^36, and N M <= 2^36 in the table form.
  * ---------------------------------------------------------------------------------------------- */
 #define FSGS_BALANCE_PAIRS 0
 #define FSGS_BALANCE_TABLE 1
 size_t fsgs_balance_workspace_bytes(int64_t N, int K, int M, int form);
 int fsgs_balance_count(int64_t N, int K, int M, const int64_t *idx, const uint8_t *mask, int form, int64_t *counts,
     void *workspace, size_t workspace_bytes, fsgs_stream_t stream);
-int fsgs_balance_pairs(int64_t N, int K, int M, const float *weights, void *workspace, size_t workspace_bytes, float scale,
-    const float *upstream, float *loss, float *g_weights, int accumulate, fsgs_stream_t stream);
+int fsgs_balance_pairs(int64_t N, int K, int M, const float *weights, const int64_t *counts, void *workspace,
+    size_t workspace_bytes, float scale, const float *upstream, float *loss, float *g_weights, int accumulate,
+    fsgs_stream_t stream);
 int fsgs_balance_table(int64_t N, int M, int type, const void *table, int64_t row_stride, const uint8_t *mask,
-    void *workspace, size_t workspace_bytes, float scale, const float *upstream, float *loss, void *g_table,
-    int64_t g_row_stride, fsgs_stream_t stream);
+    const int64_t *counts, void *workspace, size_t workspace_bytes, float scale, const float *upstream, float *loss,
+    void *g_table, int64_t g_row_stride, fsgs_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
  * One view of a training iteration in two calls (forward, backward), all intermediates in one workspace.

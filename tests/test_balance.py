@@ -36,16 +36,16 @@ def test_entry_points_check_their_arguments():
         assert count(**bad) == -1, bad
     assert count(ws=0) == -3 and count(ws=4100) == -3 and count(n=pairs_ws - 1) == -3 and count(N=1 << 40) == -5
 
-    def pairs(N=4, K=2, M=3, w=4096, ws=4096, n=pairs_ws, loss=4096, g=0):
-        return L.fsgs_balance_pairs(N, K, M, w, ws, n, 1.0, None, loss, g, 0, None)
+    def pairs(N=4, K=2, M=3, w=4096, c=4096, ws=4096, n=pairs_ws, loss=4096, g=0):
+        return L.fsgs_balance_pairs(N, K, M, w, c, ws, n, 1.0, None, loss, g, 0, None)
 
-    assert pairs(w=0) == -1 and pairs(N=-1) == -1 and pairs(ws=0) == -3 and pairs(n=8) == -3 and pairs(N=1 << 40) == -5
+    assert pairs(w=0) == -1 and pairs(c=0) == -1 and pairs(N=-1) == -1 and pairs(ws=0) == -3 and pairs(n=8) == -3 and pairs(N=1 << 40) == -5
     assert pairs(loss=0) == 0                                      # nothing asked for
 
-    def table(N=4, M=3, type=0, t=4096, rs=3, ws=4096, n=table_ws, loss=4096, g=0, gs=3):
-        return L.fsgs_balance_table(N, M, type, t, rs, None, ws, n, 1.0, None, loss, g, gs, None)
+    def table(N=4, M=3, type=0, t=4096, rs=3, c=4096, ws=4096, n=table_ws, loss=4096, g=0, gs=3):
+        return L.fsgs_balance_table(N, M, type, t, rs, None, c, ws, n, 1.0, None, loss, g, gs, None)
 
-    for bad in (dict(N=-1), dict(M=0), dict(type=3), dict(t=0), dict(rs=2), dict(g=4096, gs=2)):
+    for bad in (dict(N=-1), dict(M=0), dict(type=3), dict(t=0), dict(rs=2), dict(c=0), dict(g=4096, gs=2)):
         assert table(**bad) == -1, bad
     assert table(ws=0) == -3 and table(n=5) == -3 and table(loss=0) == 0 and table(N=1 << 40) == -5
 

@@ -3,9 +3,10 @@
 Tolerances, e = 2^-24.  Pairs form: a share is rounded once, its product with the scale once: 2 e relative on a gradient
 (3 e where it is added to another, of both); the loss sums exact products of rounded terms in double: 3 e of the sum of
 their magnitudes, and e for itself.  Table form, a row with R the range of its values and d the length of a thread's
-column sum and the tree behind it: an exponential is 4 e + R e off (its argument is rounded to R e), sums d e more, so
-`inner` = sum p share is (R + d + 8) e sum p |share| off and a gradient k p (share - inner) is
-(R + d + 12) e k p (|share| + 2 sum p |share|) off, plus half a unit of a 16-bit type."""
+column sum and the tree behind it: an exponential is 4 e + 2 R e off (the difference to the row's largest value and its
+product with log2(e) are rounded to R e together, half of each), sums d e more, so `inner` = sum p share is
+(2 R + d + 8) e sum p |share| off and a gradient k p (share - inner) is (2 R + d + 12) e k p (|share| + 2 sum p |share|)
+off, plus half a unit of a 16-bit type."""
 import math
 
 import pytest
@@ -85,7 +86,7 @@ def _table_reference(z, idx, mask):
     fin = torch.where(torch.isfinite(z), z, z.new_tensor(0.0))
     R = (z.amax(dim=1, keepdim=True).clamp(min=-1e30) - torch.where(torch.isfinite(z), z, z.new_tensor(1e30)).amin(dim=1, keepdim=True)).clamp(0, 200)
     del fin
-    return c, float((p @ f).sum()), grad, (R + M / 32 + 16 + 12) * E * p * (centred.abs() + 2 * spread)
+    return c, float((p @ f).sum()), grad, (2 * R + M / 32 + 16 + 12) * E * p * (centred.abs() + 2 * spread)
 
 
 TABLES = [(1, 1, 1, None), (1, 1, 2, None), (5, 2, 3, 0.5), (100, 3, 128, None), (100, 3, 129, 0.3), (77, 2, 333, 0.1),
