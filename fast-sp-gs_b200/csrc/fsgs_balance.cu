@@ -271,6 +271,7 @@ struct TableArgs {
   void *g;
   const float *share;
   BalanceHead *head;                 // null: no loss
+  bool eager;
 };
 
 __device__ __forceinline__ float get(const float *p) { return *p; }
@@ -352,7 +353,10 @@ __global__ void __launch_bounds__(kTableThreads) balance_table_kernel(TableArgs 
   __shared__ int s_dead[kRows];
   const int t = threadIdx.x % G;
   const long long i = (long long) blockIdx.x * kRows + threadIdx.x / G;
-  const bool here = i < a.N, on = here && (!a.mask || a.mask[i] != 0);
+  const bool here = i < a.N;
+  bool on = here && (!a.mask || a.mask[i] != 0);
+  const bool read = a.eager ? here : on;  // a few waves of blocks: not wait for the mask before the row
+  const float up = a.scale * (a.upstream ? *a.upstream : 1.0f);
   const long long start = (here ? i : 0) * a.stride;
   const T *z = (const T *) a.table + start;
   T *g = a.g && here ? (T *) a.g + i * a.g_stride : nullptr;
@@ -360,19 +364,18 @@ __global__ void __launch_bounds__(kTableThreads) balance_table_kernel(TableArgs 
   const float *copy = a.share + moved * share_copy(a.M);  // copy[m + moved] = share of m
   const bool inside = start >= 3 && start + a.M + 3 <= (a.N - 1) * a.stride + a.M;  // groups may reach past the row
   constexpr int R = PER > 0 ? PER : 4;
-  alignas(16) float x[R], sh[R];  // values, then exponentials; shares
+  alignas(16) float x[R];  // values, then exponentials
   float top = -INFINITY;
   if (PER > 0) {
 #pragma unroll
     for (int u = 0; u < PER; u += 4) {
-      const int k = u * G + 4 * t, m = k - moved;
+      const int m = u * G + 4 * t - moved;
       const bool part = m < 0 || m + 4 > a.M;
-      if (!on || m >= a.M) {
+      if (!read || m >= a.M) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[u + j] = -INFINITY, sh[u + j] = 0.0f;
+        for (int j = 0; j < 4; ++j) x[u + j] = -INFINITY;
         continue;
       }
-      get4(copy + k, sh + u);
       if (inside || !part) {
         get4(z + m, x + u);
       } else {
@@ -386,7 +389,7 @@ __global__ void __launch_bounds__(kTableThreads) balance_table_kernel(TableArgs 
       }
     }
 #pragma unroll
-    for (int u = 0; u < PER; ++u) top = fmaxf(top, x[u]);
+    for (int u = 0; u < PER; ++u) top = fmaxf(top, on ? x[u] : -INFINITY);
   } else if (on) {
     for (int m = t; m < a.M; m += G) top = fmaxf(top, get(z + m));
   }
@@ -396,9 +399,15 @@ __global__ void __launch_bounds__(kTableThreads) balance_table_kernel(TableArgs 
   float2 s = make_float2(0.0f, 0.0f);
   if (PER > 0) {
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      x[u] = fast_exp2((x[u] - base) * kLog2e);
-      s.x += x[u], s.y = fmaf(x[u], sh[u], s.y);
+    for (int u = 0; u < PER; u += 4) {
+      if (u * G + 4 * t - moved >= a.M) continue;
+      alignas(16) float sh[4];
+      get4(copy + u * G + 4 * t, sh);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[u + j] = on ? fast_exp2((x[u + j] - base) * kLog2e) : 0.0f;
+        s.x += x[u + j], s.y = fmaf(x[u + j], sh[j], s.y);
+      }
     }
   } else if (on) {
     for (int m = t; m < a.M; m += G) {
@@ -409,15 +418,17 @@ __global__ void __launch_bounds__(kTableThreads) balance_table_kernel(TableArgs 
   s = row_sum<G>(s, s_sum);
   const float inv = s.x == 0.0f ? 0.0f : __fdividef(1.0f, s.x), inner = s.y * inv;
   if (g) {
-    const float k = a.scale * (a.upstream ? *a.upstream : 1.0f) * inv, less = -k * inner;
+    const float k = up * inv, less = -k * inner;
     const bool alike = (int) ((uintptr_t) g / sizeof(T) & 3) == moved;  // the gradient's groups lie as the table's
     if (PER > 0) {
 #pragma unroll
       for (int u = 0; u < PER; u += 4) {
         const int m = u * G + 4 * t - moved;
         if (m >= a.M) continue;
+        alignas(16) float sh[4];
+        get4(copy + u * G + 4 * t, sh);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[u + j] = on ? x[u + j] * fmaf(k, sh[u + j], less) : 0.0f;
+        for (int j = 0; j < 4; ++j) x[u + j] = on ? x[u + j] * fmaf(k, sh[j], less) : 0.0f;
         if (alike && m >= 0 && m + 4 <= a.M) {
           put4(g + m, x + u);
         } else {
@@ -557,7 +568,7 @@ extern "C" int fsgs_balance_table(int64_t N, int M, int type, const void *table,
   const int64_t blocks = (N + rows - 1) / rows;
   if (blocks > INT32_MAX) return FSGS_ERR_LIMIT;
   if (blocks > 0) {
-    const TableArgs a = {N, row_stride, g_row_stride, M, table, mask, scale, upstream, g_table, w.share, loss ? w.head : nullptr};
+    const TableArgs a = {N, row_stride, g_row_stride, M, table, mask, scale, upstream, g_table, w.share, loss ? w.head : nullptr, blocks <= 4096};
     const int rc = type == FSGS_F32 ? table_pick<float>(a, reach, blocks, st) : type == FSGS_BF16 ? table_pick<__nv_bfloat16>(a, reach, blocks, st)
                                                                                               : table_pick<__half>(a, reach, blocks, st);
     if (rc != FSGS_OK) return rc;
