@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 
 #include "fsgs_common.cuh"
+#include "fsgs_two.cuh"
 
 namespace fsgs {
 
@@ -280,22 +281,34 @@ __device__ __forceinline__ float get(const __half *p) { return __half2float(*p);
 __device__ __forceinline__ void put(float *p, float x) { *p = x; }
 __device__ __forceinline__ void put(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 __device__ __forceinline__ void put(__half *p, float x) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void get4(const float *p, float *x) { *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(p); }
-template <typename H>
-__device__ __forceinline__ void get4(const H *p, float *x) {
-  const uint2 v = *reinterpret_cast<const uint2 *>(p);
-  const H *h = reinterpret_cast<const H *>(&v);
-#pragma unroll
-  for (int u = 0; u < 4; ++u) x[u] = get(h + u);
+// four neighbouring elements, as they lie in memory and as float32
+template <typename T>
+struct Four {
+  uint2 a;
+};
+template <>
+struct Four<float> {
+  float4 a;
+};
+template <typename T>
+__device__ __forceinline__ Four<T> load4(const T *p) { return *reinterpret_cast<const Four<T> *>(p); }
+__device__ __forceinline__ void open4(const Four<float> &v, float *x) { x[0] = v.a.x, x[1] = v.a.y, x[2] = v.a.z, x[3] = v.a.w; }
+__device__ __forceinline__ void open4(const Four<__nv_bfloat16> &v, float *x) {
+  x[0] = __uint_as_float(v.a.x << 16), x[1] = __uint_as_float(v.a.x & 0xffff0000u);
+  x[2] = __uint_as_float(v.a.y << 16), x[3] = __uint_as_float(v.a.y & 0xffff0000u);
+}
+__device__ __forceinline__ void open4(const Four<__half> &v, float *x) {
+  const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.a.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&v.a.y));
+  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
 }
 __device__ __forceinline__ void put4(float *p, const float *x) { *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]); }
-template <typename H>
-__device__ __forceinline__ void put4(H *p, const float *x) {
-  uint2 v;
-  H *h = reinterpret_cast<H *>(&v);
-#pragma unroll
-  for (int u = 0; u < 4; ++u) put(h + u, x[u]);
-  *reinterpret_cast<uint2 *>(p) = v;
+__device__ __forceinline__ void put4(__nv_bfloat16 *p, const float *x) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
+}
+__device__ __forceinline__ void put4(__half *p, const float *x) {
+  const __half2 a = __floats2half2_rn(x[0], x[1]), b = __floats2half2_rn(x[2], x[3]);
+  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
 }
 
 // max / sum over the G threads that share a row (part of a warp, a warp, or the block); NaN are passed over by the max
@@ -329,6 +342,11 @@ __device__ __forceinline__ float2 row_sum(float2 v, float2 *scratch) {
   return v;
 }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {  // passes over NaN, as fmaxf does
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 __device__ __forceinline__ float fast_exp2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -343,112 +361,135 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // neighbour).  exp(z - max) is the hardware's exp2 of (z - max) log2(e); the difference is taken first, because z log2(e)
 // overflows for the type's lowest value, which stands for masked columns in places.  The row stays in registers from its
 // one read to the write of its gradient; the grid covers the rows and leaves the order to the hardware.
-template <typename T, int G, int PER>
+template <typename T, int G, int PER, int ROWS>
 __global__ void __launch_bounds__(kTableThreads) balance_table_kernel(TableArgs a) {
   constexpr float kLog2e = 1.44269504f;
-  constexpr int kRows = kTableThreads / G;
+  constexpr int kGroups = kTableThreads / G;
   __shared__ float s_max[kTableThreads / 32];
   __shared__ float2 s_sum[kTableThreads / 32];
-  __shared__ float s_inner[kRows];  // of the block's rows; NaN and infinities pass through
-  __shared__ int s_dead[kRows];
+  __shared__ float s_inner[kGroups * ROWS];  // of the block's rows; NaN and infinities pass through
+  __shared__ int s_dead[kGroups * ROWS];
   const int t = threadIdx.x % G;
-  const long long i = (long long) blockIdx.x * kRows + threadIdx.x / G;
-  const bool here = i < a.N;
-  bool on = here && (!a.mask || a.mask[i] != 0);
-  const bool read = a.eager ? here : on;  // a few waves of blocks: not wait for the mask before the row
   const float up = a.scale * (a.upstream ? *a.upstream : 1.0f);
-  const long long start = (here ? i : 0) * a.stride;
-  const T *z = (const T *) a.table + start;
-  T *g = a.g && here ? (T *) a.g + i * a.g_stride : nullptr;
-  const int moved = (int) ((uintptr_t) z / sizeof(T) & 3);
-  const float *copy = a.share + moved * share_copy(a.M);  // copy[m + moved] = share of m
-  const bool inside = start >= 3 && start + a.M + 3 <= (a.N - 1) * a.stride + a.M;  // groups may reach past the row
-  constexpr int R = PER > 0 ? PER : 4;
-  alignas(16) float x[R];  // values, then exponentials
-  float top = -INFINITY;
-  if (PER > 0) {
+  auto row_of = [&](int r) { return ((long long) blockIdx.x * ROWS + r) * kGroups + threadIdx.x / G; };
+  // groups of this row may reach past it into its neighbours
+  auto inside = [&](long long i) { return i * a.stride >= 3 && (i + 1 < a.N ? a.stride : (long long) a.M) >= (long long) a.M + 3; };
+  auto moved_of = [&](const T *z) { return (int) ((uintptr_t) z / sizeof(T) & 3); };
+  Four<T> raw[ROWS][PER > 0 ? PER / 4 : 1];
+  bool on[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const long long i = row_of(r);
+    on[r] = i < a.N && (!a.mask || a.mask[i] != 0);
+    const T *z = (const T *) a.table + (i < a.N ? i : 0) * a.stride;
+    const int moved = moved_of(z);
+    const bool past = i < a.N && inside(i), read = a.eager ? i < a.N : on[r];  // eager: not wait for the mask before the row
 #pragma unroll
     for (int u = 0; u < PER; u += 4) {
       const int m = u * G + 4 * t - moved;
-      const bool part = m < 0 || m + 4 > a.M;
-      if (!read || m >= a.M) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[u + j] = -INFINITY;
-        continue;
-      }
-      if (inside || !part) {
-        get4(z + m, x + u);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[u + j] = m + j >= 0 && m + j < a.M ? get(z + m + j) : -INFINITY;
-      }
-      if (part) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (m + j < 0 || m + j >= a.M) x[u + j] = -INFINITY;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < PER; ++u) top = fmaxf(top, on ? x[u] : -INFINITY);
-  } else if (on) {
-    for (int m = t; m < a.M; m += G) top = fmaxf(top, get(z + m));
-  }
-  top = row_max<G>(top, s_max);
-  // a row of nothing but -infinity has no probabilities: it adds nothing and has no gradient
-  const float base = top == -INFINITY ? 0.0f : top;
-  float2 s = make_float2(0.0f, 0.0f);
-  if (PER > 0) {
-#pragma unroll
-    for (int u = 0; u < PER; u += 4) {
-      if (u * G + 4 * t - moved >= a.M) continue;
-      alignas(16) float sh[4];
-      get4(copy + u * G + 4 * t, sh);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[u + j] = on ? fast_exp2((x[u + j] - base) * kLog2e) : 0.0f;
-        s.x += x[u + j], s.y = fmaf(x[u + j], sh[j], s.y);
-      }
-    }
-  } else if (on) {
-    for (int m = t; m < a.M; m += G) {
-      const float e = fast_exp2((get(z + m) - base) * kLog2e);
-      s.x += e, s.y = fmaf(e, copy[m + moved], s.y);
+      if (read && m < a.M && (past || (m >= 0 && m + 4 <= a.M))) raw[r][u / 4] = load4(z + m);
     }
   }
-  s = row_sum<G>(s, s_sum);
-  const float inv = s.x == 0.0f ? 0.0f : __fdividef(1.0f, s.x), inner = s.y * inv;
-  if (g) {
-    const float k = up * inv, less = -k * inner;
-    const bool alike = (int) ((uintptr_t) g / sizeof(T) & 3) == moved;  // the gradient's groups lie as the table's
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const long long i = row_of(r);
+    const T *z = (const T *) a.table + (i < a.N ? i : 0) * a.stride;
+    T *g = a.g && i < a.N ? (T *) a.g + i * a.g_stride : nullptr;
+    const int moved = moved_of(z);
+    const float *copy = a.share + moved * share_copy(a.M);  // copy[m + moved] = share of m
+    float x[PER > 0 ? PER : 1];  // values, then exponentials
+    float top = -INFINITY;
     if (PER > 0) {
+      const bool past = i < a.N && inside(i);
 #pragma unroll
       for (int u = 0; u < PER; u += 4) {
         const int m = u * G + 4 * t - moved;
-        if (m >= a.M) continue;
-        alignas(16) float sh[4];
-        get4(copy + u * G + 4 * t, sh);
+        const bool part = m < 0 || m + 4 > a.M;
+        if (!on[r] || m >= a.M) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[u + j] = on ? x[u + j] * fmaf(k, sh[j], less) : 0.0f;
-        if (alike && m >= 0 && m + 4 <= a.M) {
-          put4(g + m, x + u);
-        } else {
+          for (int j = 0; j < 4; ++j) x[u + j] = -INFINITY;
+          continue;
+        }
+        open4(raw[r][u / 4], x + u);
+        if (part) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (m + j >= 0 && m + j < a.M) put(g + m + j, x[u + j]);
+          for (int j = 0; j < 4; ++j) {
+            const bool in = m + j >= 0 && m + j < a.M;
+            if (in && !past) x[u + j] = get(z + m + j);
+            if (!in) x[u + j] = -INFINITY;
+          }
         }
       }
-    } else {
-      for (int m = t; m < a.M; m += G)
-        put(g + m, on ? fast_exp2((get(z + m) - base) * kLog2e) * fmaf(k, copy[m + moved], less) : 0.0f);
+#pragma unroll
+      for (int u = 0; u < PER; u += 4) top = max3(max3(top, x[u], x[u + 1]), x[u + 2], x[u + 3]);
+    } else if (on[r]) {
+      for (int m = t; m < a.M; m += G) top = fmaxf(top, get(z + m));
     }
+    top = row_max<G>(top, s_max);
+    // a row of nothing but -infinity has no probabilities: it adds nothing and has no gradient
+    const float base = top == -INFINITY ? 0.0f : top;
+    float2 s = make_float2(0.0f, 0.0f);
+    if (PER > 0) {
+      Two sx = both(0.0f), sy = both(0.0f);
+#pragma unroll
+      for (int u = 0; u < PER; u += 4) {
+        if (u * G + 4 * t - moved >= a.M) continue;
+        const float4 sh = *reinterpret_cast<const float4 *>(copy + u * G + 4 * t);
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          split(mul2(add2(two(x[u + j], x[u + j + 1]), both(-base)), both(kLog2e)), x[u + j], x[u + j + 1]);
+          const Two e = two(x[u + j] = fast_exp2(x[u + j]), x[u + j + 1] = fast_exp2(x[u + j + 1]));
+          sx = add2(sx, e), sy = fma2(e, j ? two(sh.z, sh.w) : two(sh.x, sh.y), sy);
+        }
+      }
+      float hx, hy;
+      split(sx, s.x, hx), split(sy, s.y, hy);
+      s.x += hx, s.y += hy;
+    } else if (on[r]) {
+      for (int m = t; m < a.M; m += G) {
+        const float e = fast_exp2((get(z + m) - base) * kLog2e);
+        s.x += e, s.y = fmaf(e, copy[m + moved], s.y);
+      }
+    }
+    s = row_sum<G>(s, s_sum);
+    const float inv = s.x == 0.0f ? 0.0f : __fdividef(1.0f, s.x), inner = s.y * inv;
+    if (g) {
+      const float k = up * inv, less = -k * inner;
+      const bool alike = moved_of(g) == moved;  // the gradient's groups lie as the table's
+      if (PER > 0) {
+#pragma unroll
+        for (int u = 0; u < PER; u += 4) {
+          const int m = u * G + 4 * t - moved;
+          if (m >= a.M) continue;
+          const float4 sh = *reinterpret_cast<const float4 *>(copy + u * G + 4 * t);
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            const Two f = fma2(both(k), j ? two(sh.z, sh.w) : two(sh.x, sh.y), both(less));
+            split(mul2(two(x[u + j], x[u + j + 1]), f), x[u + j], x[u + j + 1]);
+            if (!on[r]) x[u + j] = x[u + j + 1] = 0.0f;
+          }
+          if (alike && m >= 0 && m + 4 <= a.M) {
+            put4(g + m, x + u);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (m + j >= 0 && m + j < a.M) put(g + m + j, x[u + j]);
+          }
+        }
+      } else {
+        for (int m = t; m < a.M; m += G)
+          put(g + m, on[r] ? fast_exp2((get(z + m) - base) * kLog2e) * fmaf(k, copy[m + moved], less) : 0.0f);
+      }
+    }
+    if (a.head && t == 0)
+      s_inner[r * kGroups + threadIdx.x / G] = on[r] ? inner : 0.0f, s_dead[r * kGroups + threadIdx.x / G] = on[r] && s.x == 0.0f;
   }
   if (!a.head) return;
-  if (t == 0) s_inner[threadIdx.x / G] = on ? inner : 0.0f, s_dead[threadIdx.x / G] = on && s.x == 0.0f;
   __syncthreads();
   if (threadIdx.x == 0) {
     double sum = 0.0;
     int dead = 0;
-    for (int r = 0; r < kRows; ++r) sum += (double) s_inner[r], dead += s_dead[r];
+    for (int r = 0; r < kGroups * ROWS; ++r) sum += (double) s_inner[r], dead += s_dead[r];
     const bool fine = fabs(sum) <= 2.0 * a.M;
     if (fine) atomicAdd((unsigned long long *) a.head->slots + blockIdx.x % kFixedSlots,
                         (unsigned long long) __double2ll_rn(ldexp(sum, fixed_bits(a.M))));
@@ -471,28 +512,39 @@ __global__ void __launch_bounds__(32) balance_close_kernel(BalanceHead *head, co
 }
 static_assert(kFixedSlots == 32, "one warp closes the sum");
 
-// `reach`: columns from the first group of four to the row's end, M where every row starts on a boundary of four elements
-static int rows_per_block(int reach) { return reach <= 64 ? kTableThreads / 8 : reach <= 512 ? kTableThreads / 32 : 1; }
-
-template <typename T, int G, int PER>
-static int table_launch(const TableArgs &a, int64_t blocks, cudaStream_t st) {
-  balance_table_kernel<T, G, PER><<<(int) blocks, kTableThreads, 0, st>>>(a);
+// `reach`: columns from the first group of four to the row's end, M where every row starts on a boundary of four elements.
+// `reach`: columns from the first group of four to the row's end, M where every row starts on a boundary of four elements.
+template <typename T, int G, int PER, int ROWS>
+static int table_launch(TableArgs &a, cudaStream_t st) {
+  const int rows = kTableThreads / G * ROWS;
+  const int64_t blocks = (a.N + rows - 1) / rows;
+  if (blocks > INT32_MAX) return FSGS_ERR_LIMIT;
+  if (blocks == 0) return FSGS_OK;
+  a.eager = blocks <= 4096;
+  balance_table_kernel<T, G, PER, ROWS><<<(int) blocks, kTableThreads, 0, st>>>(a);
   FSGS_LAUNCH_CHECK();
   return FSGS_OK;
 }
 
+// Threads per row: as few as the registers allow, so that many columns share a row's reductions and addresses; tables of
+// 16 bits, whose rows are instructions rather than bytes, have the next row's loads under way meanwhile.  Measured, value
+// and gradient (us; one row a thread group | two): 300 k x 512 bf16 177 | 171, 400 k x 256 bf16 140 | 123, 1 M x 100 bf16
+// 148 | 155, 2 M x 40 bf16 209 | 189; float32 is bound by memory (300 k x 512: 190 us, 6.5 TB/s) and takes one.  A warp
+// per row reaches to 1024 columns (100 k x 1000: 138 us, a block per row 244), a block per row lies above.
 template <typename T>
-static int table_pick(const TableArgs &a, int reach, int64_t blocks, cudaStream_t st) {
-  if (reach <= 64) return table_launch<T, 8, 8>(a, blocks, st);
-  if (reach <= 128) return table_launch<T, 32, 4>(a, blocks, st);
-  if (reach <= 256) return table_launch<T, 32, 8>(a, blocks, st);
-  if (reach <= 384) return table_launch<T, 32, 12>(a, blocks, st);
-  if (reach <= 512) return table_launch<T, 32, 16>(a, blocks, st);
-  if (reach <= 1024) return table_launch<T, 256, 4>(a, blocks, st);
-  if (reach <= 2048) return table_launch<T, 256, 8>(a, blocks, st);
-  if (reach <= 4096) return table_launch<T, 256, 16>(a, blocks, st);
-  if (reach <= 8192) return table_launch<T, 256, 32>(a, blocks, st);
-  return table_launch<T, 256, 0>(a, blocks, st);
+static int table_pick(TableArgs &a, int reach, cudaStream_t st) {
+  constexpr int R = sizeof(T) == 2 ? 2 : 1;
+  if (reach <= 64) return table_launch<T, 8, 8, R>(a, st);
+  if (reach <= 128) return table_launch<T, 8, 16, 1>(a, st);
+  if (reach <= 256) return table_launch<T, 16, 16, R>(a, st);
+  if (reach <= 384) return table_launch<T, 32, 12, R>(a, st);
+  if (reach <= 512) return table_launch<T, 32, 16, R>(a, st);
+  if (reach <= 768) return table_launch<T, 32, 24, 1>(a, st);
+  if (reach <= 1024) return table_launch<T, 32, 32, 1>(a, st);
+  if (reach <= 2048) return table_launch<T, 256, 8, 1>(a, st);
+  if (reach <= 4096) return table_launch<T, 256, 16, 1>(a, st);
+  if (reach <= 8192) return table_launch<T, 256, 32, 1>(a, st);
+  return table_launch<T, 256, 0, 1>(a, st);
 }
 
 static bool balance_sizes(int64_t N, int64_t per_row) { return N <= (1ll << 36) / per_row; }
@@ -564,15 +616,11 @@ extern "C" int fsgs_balance_table(int64_t N, int M, int type, const void *table,
   cudaStream_t st = (cudaStream_t) stream;
   const BalanceSpace w = balance_space(workspace);
   const bool plain = row_stride % 4 == 0 && (uintptr_t) table % (type == FSGS_F32 ? 16 : 8) == 0;
-  const int reach = M + (plain ? 0 : 3), rows = rows_per_block(reach);
-  const int64_t blocks = (N + rows - 1) / rows;
-  if (blocks > INT32_MAX) return FSGS_ERR_LIMIT;
-  if (blocks > 0) {
-    const TableArgs a = {N, row_stride, g_row_stride, M, table, mask, scale, upstream, g_table, w.share, loss ? w.head : nullptr, blocks <= 4096};
-    const int rc = type == FSGS_F32 ? table_pick<float>(a, reach, blocks, st) : type == FSGS_BF16 ? table_pick<__nv_bfloat16>(a, reach, blocks, st)
-                                                                                              : table_pick<__half>(a, reach, blocks, st);
-    if (rc != FSGS_OK) return rc;
-  }
+  const int reach = M + (plain ? 0 : 3);
+  TableArgs a = {N, row_stride, g_row_stride, M, table, mask, scale, upstream, g_table, w.share, loss ? w.head : nullptr, false};
+  const int rc = type == FSGS_F32 ? table_pick<float>(a, reach, st) : type == FSGS_BF16 ? table_pick<__nv_bfloat16>(a, reach, st)
+                                                                                  : table_pick<__half>(a, reach, st);
+  if (rc != FSGS_OK) return rc;
   if (!loss) return FSGS_OK;
   balance_close_kernel<<<1, kFixedSlots, 0, st>>>(w.head, (const long long *) counts, M, scale, upstream, loss);
   FSGS_LAUNCH_CHECK();
