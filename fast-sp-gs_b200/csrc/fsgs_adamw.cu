@@ -221,8 +221,8 @@ __device__ __forceinline__ void update(const float *g, float *m, float *v, float
     const Two gs = mul2(two(g[u], g[u + 1]), both(scale));
     Two a = two(m[u], m[u + 1]), b = two(v[u], v[u + 1]);
     if (EIGHT) a = mul2(a, both(ms)), b = mul2(b, both(vs)), b = mul2(b, b);
-    split(add2(mul2(a, both(s.b1)), mul2(gs, both(s.c1))), m[u], m[u + 1]);
-    split(add2(mul2(b, both(-s.b2)), mul2(mul2(gs, gs), both(-s.c2))), v[u], v[u + 1]);  // -v'
+    plain_sum(mul2(a, both(s.b1)), mul2(gs, both(s.c1)), m[u], m[u + 1]);
+    plain_sum(mul2(b, both(-s.b2)), mul2(mul2(gs, gs), both(-s.c2)), v[u], v[u + 1]);  // -v'
   }
   // a NaN among others passes: its own root is a NaN either way.  An infinite v passes with 8-bit moments only, where it
   // spoils its block whatever its root is.
@@ -450,28 +450,41 @@ struct NormArgs {
   int last;    // this launch closes the sum
 };
 
-// Sum of the squares of this thread's elements of a chunk.  Eight squares are added in float32 and the eights in double:
-// the float32 part rounds each eight by 4 x 2^-24 at most, and no sum of squares leaves the range of double unless a
+// Sum of the squares of this thread's elements of a chunk.  Eight squares are added in float32 (two sums of four) and the
+// eights in double: the float32 part rounds each eight by 5 x 2^-24 at most, and no sum of squares leaves the range of double unless a
 // single eight leaves that of float32 (|g| > 6e18: the norm comes out infinite and the step is dropped).
 template <typename T>
 __device__ __forceinline__ double chunk_squares(const T *p, bool vec, long long left, int warp, int lane) {
-  double sum = 0.0;
+  constexpr int parts = kNormChunk / kNormPart;
+  auto squares = [](const float *x) {
+    Two q = both(0.0f);
 #pragma unroll
-  for (int j = 0; j < kNormChunk / kNormPart; ++j) {
-    const long long e0 = (long long) j * kNormPart + warp * kOptBlock + 8 * lane;
-    if (left > e0) {
-      float x[8];
-      if (vec && left - e0 >= 8) {
+    for (int u = 0; u < 8; u += 2) q = fma2(two(x[u], x[u + 1]), two(x[u], x[u + 1]), q);
+    float a, b;
+    split(q, a, b);
+    return (double) (a + b);
+  };
+  double sum = 0.0;
+  float x[8];
+  p += warp * kOptBlock + 8 * lane;
+  if (vec && left >= kNormChunk) {  // all loads out before the first is used
+    Packed<T> w[parts];
+#pragma unroll
+    for (int j = 0; j < parts; ++j) w[j].load(p + j * kNormPart);
+#pragma unroll
+    for (int j = 0; j < parts; ++j) w[j].get(x), sum += squares(x);
+  } else {
+    left -= warp * kOptBlock + 8 * lane;
+#pragma unroll 1
+    for (int j = 0; j < parts && left > 0; ++j, p += kNormPart, left -= kNormPart) {
+      if (vec && left >= 8) {
         Packed<T> w;
-        w.load(p + e0);
+        w.load(p);
         w.get(x);
       } else {
-        load_some(p + e0, left - e0, x);
+        load_some(p, left, x);
       }
-      float q = 0.0f;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) q = fmaf(x[u], x[u], q);
-      sum += (double) q;
+      sum += squares(x);
     }
   }
   return sum;

@@ -82,7 +82,7 @@ __device__ __forceinline__ T block_total(T v, T *scratch) {  // valid in the fir
 // last turns the counts into shares.  Bound by the read of the indices and, beside it, by one shared-memory atomic per pair.
 template <typename Code>
 __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long long N, int K, int M, const int64_t *__restrict__ idx,
-    const uint8_t *__restrict__ mask, int wide, unsigned long long *__restrict__ counts, BalanceHead *__restrict__ head,
+    const uint8_t *__restrict__ mask, int wide, unsigned magic, unsigned long long *__restrict__ counts, BalanceHead *__restrict__ head,
     float *__restrict__ share, Code *__restrict__ codes) {
   extern __shared__ int s_hist[];   // [M + 1]: the last one takes what does not count
   __shared__ long long s_red[kCountThreads / 32];
@@ -110,7 +110,14 @@ __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long lo
     const longlong2 a = reinterpret_cast<const longlong2 *>(idx)[2 * q], b = reinterpret_cast<const longlong2 *>(idx)[2 * q + 1];
     bool on[4] = {true, true, true, true};
     if (mask) {
-      long long row = pairs < (1ll << 32) ? (long long) ((unsigned) (4 * q) / (unsigned) K) : 4 * q / K;
+      long long row;
+      if (magic) {  // 4 q / K for 32-bit values: the high product is the quotient or one less
+        unsigned r = __umulhi((unsigned) (4 * q), magic);
+        if ((unsigned) (4 * q) - r * (unsigned) K >= (unsigned) K) ++r;
+        row = r;
+      } else {
+        row = 4 * q / K;
+      }
       int col = (int) (4 * q - row * K);
       on[0] = mask[row] != 0;
 #pragma unroll
@@ -580,9 +587,10 @@ extern "C" int fsgs_balance_count(int64_t N, int K, int M, const int64_t *idx, c
   const size_t smem = M <= kBalSharedPoints ? sizeof(int) * ((size_t) M + 1) : 0;
   unsigned long long *c = (unsigned long long *) counts;
   const int wide = ((uintptr_t) idx & 15) == 0;
+  const unsigned magic = K > 1 && N * K < (1ll << 32) ? (unsigned) ((1ull << 32) / (unsigned) K) : 0u;
   void *codes = form == FSGS_BALANCE_PAIRS ? w.codes : nullptr;
-  if (code_bytes(M) == 2) balance_count_kernel<uint16_t><<<grid, kCountThreads, smem, st>>>(N, K, M, idx, mask, wide, c, w.head, w.share, (uint16_t *) codes);
-  else balance_count_kernel<uint32_t><<<grid, kCountThreads, smem, st>>>(N, K, M, idx, mask, wide, c, w.head, w.share, (uint32_t *) codes);
+  if (code_bytes(M) == 2) balance_count_kernel<uint16_t><<<grid, kCountThreads, smem, st>>>(N, K, M, idx, mask, wide, magic, c, w.head, w.share, (uint16_t *) codes);
+  else balance_count_kernel<uint32_t><<<grid, kCountThreads, smem, st>>>(N, K, M, idx, mask, wide, magic, c, w.head, w.share, (uint32_t *) codes);
   FSGS_LAUNCH_CHECK();
   return FSGS_OK;
 }

@@ -420,3 +420,48 @@ def test_the_plan_follows_the_optimiser():
         before = _snapshot(opt, params[1:])
         opt.step()
     _check_step(opt, before, params[1:], one_grad)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_moments_are_the_formula_operation_by_operation(bits):
+    """The moments bit for bit as float32 operations one after another give them, roots, scales and 8-bit values too: a
+    moment beside a border between two 8-bit values falls on the formula's side."""
+    from fsgs.optim import AdamW
+    n = 64 * B
+    gen = torch.Generator().manual_seed(11)
+    spread = lambda: (torch.randn(n, generator=gen) * torch.exp(torch.randn(n, generator=gen))).cuda()  # noqa: E731
+    p = torch.nn.Parameter(spread())
+    opt = AdamW([p], state_bits=bits)
+    opt.init_state()
+    st = opt.state[p]
+    rows = lambda t: t.view(-1, B)  # noqa: E731
+
+    def pack(x, positive):
+        top = x.abs().amax(dim=1, keepdim=True)
+        y = x * (448.0 / top)
+        y = torch.where(x > 0, y.clamp_min(2.0 ** -9), y) if positive else y
+        return y.to(torch.float8_e4m3fn), top
+
+    m, s = rows(spread() * 1e-3), rows(spread().abs() * 1e-3)
+    if bits == 8:
+        for x, name, positive in ((m, "exp_avg", False), (s, "exp_avg_sq_root", True)):
+            code, top = pack(x, positive)
+            st[name].copy_(code.view(-1))
+            st[name + "_scale"].copy_(top[:, 0] / 448.0)
+        m, s = (rows(st[k].float()) * st[k + "_scale"][:, None] for k in ("exp_avg", "exp_avg_sq_root"))
+        v = s * s
+    else:
+        v = s * s
+        st["exp_avg"].copy_(m.reshape(-1))
+        st["exp_avg_sq"].copy_(v.reshape(-1))
+    p.grad = spread() * 1e-3
+    g = rows(p.grad)
+    m, v = m * 0.9 + g * (1 - 0.9), v * 0.999 + g * g * (1 - 0.999)
+    opt.step()
+    if bits == 32:
+        assert torch.equal(rows(st["exp_avg"]), m) and torch.equal(rows(st["exp_avg_sq"]), v)
+        return
+    for x, name, positive in ((m, "exp_avg", False), (v.sqrt(), "exp_avg_sq_root", True)):
+        code, top = pack(x, positive)
+        assert torch.equal(rows(st[name]).float(), code.float()), name
+        assert bool(((st[name + "_scale"] - top[:, 0] / 448.0).abs() <= 2 * E * top[:, 0] / 448.0).all()), name
