@@ -11,7 +11,8 @@ import torch.distributed as dist
 
 from . import ops
 from .dist import GradBucket, slot_order
-from .optim import DenseAdam, SparseGaussianAdam
+from .loss import balance_value_and_grad
+from .optim import AdamW, DenseAdam, SparseGaussianAdam
 from .renderer import GS_2D_fast_render, check_overflow, group_pairs_by_superpoint
 
 # learning rates of exps/d_nerf.yaml (position lr at its initial value)
@@ -45,12 +46,15 @@ def lbs_weights(d2, idx, mode="dist", temperature=1.0, radius=None, weight=None,
 
 class DynamicScene:
     def __init__(self, surfels, centres, K=3, eps=1e-15, device="cuda", lrs=None, motion_net=None, kernel_weights=None,
-                 lr_deform=1.6e-4):
+                 lr_deform=1.6e-4, adamw=None, balance=0.0):
         """``motion_net``: a ``fsgs.motion.MotionNet``; views may then give a time ``t`` instead of a precomputed
         ``motion`` and the network is trained with the scene.  ``kernel_weights``: ``(raw_radius [M], raw_weight [M] or
         None)`` switches the LBS weights to the learnable kernel form of the shipped configuration
         (network.py:506-513), re-evaluated every step and trained as well.  Both are optimised by a dense Adam at
-        ``lr_deform`` (the reference's deformation-network group, network.py:296-305)."""
+        ``lr_deform`` (the reference's deformation-network group, network.py:296-305), or, with ``adamw`` -- a dictionary
+        of ``fsgs.optim.AdamW`` settings, empty for its defaults --, by ``AdamW`` (weight decay, 8-bit moments, clipping).
+        ``balance``: weight of ``fsgs.loss.balance_loss`` on the kernel weights, added once per step; ``self.balance_loss``
+        and ``self.superpoint_counts`` are the last step's."""
         P = lambda t: torch.nn.Parameter(t.to(device).contiguous())
         self.xyz = P(surfels["means"])
         self.scaling = P(surfels["log_scales"])
@@ -67,7 +71,14 @@ class DynamicScene:
             self.sp_weight = P(kernel_weights[1]) if kernel_weights[1] is not None else None
         self.dense_params = ([motion_net.params] if motion_net is not None else []) + \
             [p for p in (self.sp_radius, self.sp_weight) if p is not None]
-        self.dense_optimizer = DenseAdam(self.dense_params, lr=lr_deform, eps=eps) if self.dense_params else None
+        if balance and self.sp_radius is None:
+            raise ValueError("balance acts on the kernel weights: pass kernel_weights")
+        self.balance = float(balance)
+        self.balance_loss = self.superpoint_counts = None
+        self.dense_optimizer = None
+        if self.dense_params:
+            self.dense_optimizer = DenseAdam(self.dense_params, lr=lr_deform, eps=eps) if adamw is None else \
+                AdamW(self.dense_params, **{"lr": lr_deform, "eps": eps, **adamw})
         self.refresh_knn()
         LRS = dict(globals()["LRS"], **(lrs or {}))
         groups = [dict(params=[self.xyz], lr=LRS["xyz"]), dict(params=[self.sh_dc], lr=LRS["sh_dc"]),
@@ -205,6 +216,10 @@ class DynamicScene:
         def after_last_view():
             if self.sp_radius is not None:
                 from .motion import kernel_weights_backward
+                if self.balance:  # the ranks' gradients are summed: each adds its part of the one term
+                    loss, _, self.superpoint_counts = balance_value_and_grad(
+                        self.knn_w, self.knn_idx, self.centres.shape[0], weight=self.balance / world, grad=self.g_knn_w)
+                    self.balance_loss = loss * world
                 kernel_weights_backward(self.knn_d2, self.knn_idx, self.sp_radius.data,
                                         None if self.sp_weight is None else self.sp_weight.data, self.g_knn_w,
                                         self.knn_idx.superpoint_pairs, b.view_of(self.sp_radius),
@@ -245,6 +260,9 @@ class DynamicScene:
                     after_last_view()
         if not views:  # a rank without a view this step still takes part in the exchange, with zeros
             b.flat.zero_()
+            if self.balance:   # the balance term does not depend on the views
+                self.g_knn_w.zero_()
+                after_last_view()
             if distributed:
                 first_exchange()
                 late = b.reduce_span(3, last_seg, group)
