@@ -441,15 +441,6 @@ constexpr int kNormPart = kOptWarps * kOptBlock;   // elements of one pass of a 
 constexpr int kNormChunk = 4 * kNormPart;
 constexpr int kNormSlots = FSGS_GRAD_NORM_SLOTS;
 
-struct NormArgs {
-  double *slots;
-  int *ticket;
-  float *out;
-  float max_norm;
-  int filled;  // slots written by earlier launches of the same call
-  int last;    // this launch closes the sum
-};
-
 // Sum of the squares of this thread's elements of a chunk.  Eight squares are added in float32 (two sums of four) and the
 // eights in double: the float32 part rounds each eight by 5 x 2^-24 at most, and no sum of squares leaves the range of double unless a
 // single eight leaves that of float32 (|g| > 6e18: the norm comes out infinite and the step is dropped).
@@ -490,9 +481,9 @@ __device__ __forceinline__ double chunk_squares(const T *p, bool vec, long long 
   return sum;
 }
 
-__global__ void __launch_bounds__(kOptThreads) grad_norm_kernel(const __grid_constant__ NormTable a, const NormArgs s) {
+// `filled`: sums that earlier launches of the same call have left in the slots
+__global__ void __launch_bounds__(kOptThreads) grad_norm_kernel(const __grid_constant__ NormTable a, double *slots, int filled) {
   __shared__ double s_sum[kOptThreads / 32];
-  __shared__ int s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int total = a.chunk_start[a.n];
   double sum = 0.0;
@@ -508,32 +499,30 @@ __global__ void __launch_bounds__(kOptThreads) grad_norm_kernel(const __grid_con
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    double t = 0.0;
-    for (int w = 0; w < kOptThreads / 32; ++w) t += s_sum[w];
-    s.slots[blockIdx.x] = (int) blockIdx.x < s.filled ? s.slots[blockIdx.x] + t : t;
-    __threadfence();
-    s_last = s.last && atomicAdd(s.ticket, 1) == (int) gridDim.x - 1;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  // the last block adds the slots in a fixed order: the same gradients give the same norm, bit for bit
-  const int n = max(s.filled, (int) gridDim.x);
-  sum = 0.0;
-  for (int i = threadIdx.x; i < n; i += kOptThreads) sum += __ldcg(s.slots + i);
+  if (threadIdx.x != 0) return;
+  double t = 0.0;
+  for (int w = 0; w < kOptThreads / 32; ++w) t += s_sum[w];
+  slots[blockIdx.x] = (int) blockIdx.x < filled ? slots[blockIdx.x] + t : t;
+}
+
+// Adds the slots in a fixed order: the same gradients give the same norm, bit for bit.
+__global__ void __launch_bounds__(kOptThreads) grad_norm_close_kernel(const double *__restrict__ slots, int n, float max_norm,
+    float *__restrict__ out) {
+  __shared__ double s_sum[kOptThreads / 32];
+  const int lane = threadIdx.x & 31;
+  double sum = 0.0;
+#pragma unroll 5
+  for (int i = threadIdx.x; i < n; i += kOptThreads) sum += slots[i];
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_sum[warp] = sum;
+  if (lane == 0) s_sum[threadIdx.x >> 5] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    double t = 0.0;
-    for (int w = 0; w < kOptThreads / 32; ++w) t += s_sum[w];
-    const float norm = (float) sqrt(t);
-    // a norm that is not a number or infinite: factor 0, which drops the step that is given it
-    s.out[0] = norm;
-    s.out[1] = norm < INFINITY ? fminf(1.0f, __fmul_rn(__frcp_rn(__fadd_rn(norm, 1e-6f)), s.max_norm)) : 0.0f;
-    *s.ticket = 0;
-  }
+  if (threadIdx.x != 0) return;
+  double t = 0.0;
+  for (int w = 0; w < kOptThreads / 32; ++w) t += s_sum[w];
+  const float norm = (float) sqrt(t);
+  // a norm that is not a number or infinite: factor 0, which drops the step that is given it
+  out[0] = norm;
+  out[1] = norm < INFINITY ? fminf(1.0f, __fmul_rn(__frcp_rn(__fadd_rn(norm, 1e-6f)), max_norm)) : 0.0f;
 }
 
 static bool is_type(int type) { return type == FSGS_F32 || type == FSGS_BF16 || type == FSGS_F16; }
@@ -573,36 +562,37 @@ extern "C" int fsgs_adamw_multi(int n_tensors, const fsgs_adamw_tensor *tensors,
   return grad_type == FSGS_F32 ? adamw_pick<__half, float>(eight, master, c) : adamw_pick<__half, __half>(eight, master, c);
 }
 
-extern "C" size_t fsgs_grad_norm_workspace_bytes(void) { return 16 + sizeof(double) * kNormSlots; }
+extern "C" size_t fsgs_grad_norm_workspace_bytes(void) { return sizeof(double) * kNormSlots; }
 
 extern "C" int fsgs_grad_norm(int n_tensors, const fsgs_norm_tensor *tensors, float max_norm, void *workspace,
     size_t workspace_bytes, float *out, fsgs_stream_t stream) {
   FSGS_REQUIRE(n_tensors >= 0 && (tensors || n_tensors == 0) && out && max_norm > 0.0f);
   if (!workspace || ((uintptr_t) workspace & 15) || workspace_bytes < fsgs_grad_norm_workspace_bytes()) return FSGS_ERR_WORKSPACE;
-  for (int k = 0; k < n_tensors; ++k)
+  for (int k = 0; k < n_tensors; ++k) {
     FSGS_REQUIRE(tensors[k].numel >= 0 && is_type(tensors[k].type) && (tensors[k].data || tensors[k].numel == 0));
-  NormArgs s;
-  s.ticket = (int *) workspace, s.slots = (double *) ((char *) workspace + 16), s.out = out, s.max_norm = max_norm, s.filled = 0;
-  int first = 0;
-  do {  // at least one launch: no tensors have norm 0
+    if (tensors[k].numel / kNormChunk >= INT32_MAX - (1 << 20)) return FSGS_ERR_LIMIT;
+  }
+  double *slots = (double *) workspace;
+  int filled = 0;
+  for (int first = 0; first < n_tensors;) {
     NormTable a;
     a.n = 0, a.chunk_start[0] = 0;
-    int64_t chunks = 0;
     for (; first < n_tensors && a.n < kOptCapacity; ++first) {
       const fsgs_norm_tensor &t = tensors[first];
-      const int64_t c = (t.numel + kNormChunk - 1) / kNormChunk;
-      if (c > INT32_MAX - (1 << 20)) return FSGS_ERR_LIMIT;
-      if (chunks + c > INT32_MAX - (1 << 20)) break;
+      const int64_t chunks = (t.numel + kNormChunk - 1) / kNormChunk;
+      if (a.chunk_start[a.n] + chunks > INT32_MAX - (1 << 20)) break;  // the rest in a launch of its own
       a.t[a.n].data = t.data, a.t[a.n].numel = t.numel, a.type[a.n] = (uint8_t) t.type;
       a.vec[a.n] = ((uintptr_t) t.data & 15) == 0;
-      chunks += c;
-      a.chunk_start[++a.n] = (int) chunks;
+      a.chunk_start[a.n + 1] = a.chunk_start[a.n] + (int) chunks;
+      ++a.n;
     }
-    s.last = first >= n_tensors;
-    const int grid = chunks < kNormSlots ? (chunks > 0 ? (int) chunks : 1) : kNormSlots;
-    grad_norm_kernel<<<grid, kOptThreads, 0, (cudaStream_t) stream>>>(a, s);
+    const int chunks = a.chunk_start[a.n], grid = chunks < kNormSlots ? chunks : kNormSlots;
+    if (grid == 0) continue;
+    grad_norm_kernel<<<grid, kOptThreads, 0, (cudaStream_t) stream>>>(a, slots, filled);
     FSGS_LAUNCH_CHECK();
-    if (grid > s.filled) s.filled = grid;
-  } while (first < n_tensors);
+    if (grid > filled) filled = grid;
+  }
+  grad_norm_close_kernel<<<1, kOptThreads, 0, (cudaStream_t) stream>>>(slots, filled, max_norm, out);
+  FSGS_LAUNCH_CHECK();
   return FSGS_OK;
 }

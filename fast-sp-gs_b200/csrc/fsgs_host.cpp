@@ -88,11 +88,69 @@ PyObject *refuse(const char *what) {
   return nullptr;
 }
 
-// plan(entries, launches): entries [(param, group, state, names, address of its table row)], launches
+void need(bool ok, const char *what, const std::string &message) {
+  if (!ok) throw std::runtime_error(std::string(what) + ": " + message);
+}
+
+// The names of a parameter's state, and where in its table row the address goes.
+struct Slot {
+  const char *name;
+  void *fsgs_adamw_tensor::*untyped;
+  float *fsgs_adamw_tensor::*typed;
+  PyObject *key;
+};
+Slot slots32[] = {{"step", nullptr, &fsgs_adamw_tensor::step, nullptr},
+                  {"exp_avg", &fsgs_adamw_tensor::exp_avg, nullptr, nullptr},
+                  {"exp_avg_sq", &fsgs_adamw_tensor::exp_avg_sq, nullptr, nullptr},
+                  {"master", nullptr, &fsgs_adamw_tensor::master, nullptr}};
+Slot slots8[] = {{"step", nullptr, &fsgs_adamw_tensor::step, nullptr},
+                 {"exp_avg", &fsgs_adamw_tensor::exp_avg, nullptr, nullptr},
+                 {"exp_avg_sq_root", &fsgs_adamw_tensor::exp_avg_sq, nullptr, nullptr},
+                 {"exp_avg_scale", nullptr, &fsgs_adamw_tensor::exp_avg_scale, nullptr},
+                 {"exp_avg_sq_root_scale", nullptr, &fsgs_adamw_tensor::exp_avg_sq_scale, nullptr},
+                 {"master", nullptr, &fsgs_adamw_tensor::master, nullptr}};
+
+// One parameter: checks it, its gradient and its state, and fills its table row (but the rates).
+Entry entry_of(PyObject *param, Py_ssize_t group, PyObject *state, bool master, int bits, fsgs_adamw_tensor *row, c10::Device device) {
+  constexpr const char *what = "AdamW";
+  need(THPVariable_Check(param), what, "parameters are tensors");
+  const at::Tensor &t = THPVariable_Unpack(param);
+  need(t.is_cuda() && t.device() == device, what, "CUDA parameters on one device");
+  need(t.layout() == at::kStrided && t.is_contiguous() && type_of(t.scalar_type()) >= 0, what,
+       "contiguous float32, bfloat16 or float16 parameters");
+  const at::Tensor &g = t.grad();
+  need(g.defined() && g.layout() == at::kStrided && (g.scalar_type() == t.scalar_type() || g.scalar_type() == at::kFloat), what,
+       "a dense gradient of its parameter's type or float32");
+  need(g.numel() == t.numel() && g.device() == device, what, "a gradient has another size or device than its parameter");
+  Entry e{param, state, group, t.data_ptr(), t.numel(), t.scalar_type(), g.scalar_type(), {}, row};
+  row->param = e.data, row->numel = e.numel;
+  Slot *slots = bits == 8 ? slots8 : slots32;
+  const int n = (bits == 8 ? 6 : 4) - (master ? 0 : 1);
+  for (int k = 0; k < n; ++k) {
+    Slot &s = slots[k];
+    if (!s.key) s.key = PyUnicode_InternFromString(s.name);
+    PyObject *v = PyDict_GetItem(state, s.key);
+    need(v && THPVariable_Check(v), what, std::string("a parameter's state has no ") + s.name);
+    const at::Tensor &x = THPVariable_Unpack(v);
+    const bool scale = bits == 8 && (k == 3 || k == 4), moment = k == 1 || k == 2;
+    const int64_t size = k == 0 ? 1 : scale ? (e.numel + FSGS_ADAMW_BLOCK - 1) / FSGS_ADAMW_BLOCK : e.numel;
+    const at::ScalarType kind = bits == 8 && moment ? at::kFloat8_e4m3fn : at::kFloat;
+    need(x.device() == device && x.layout() == at::kStrided && x.scalar_type() == kind && x.numel() == size && x.is_contiguous(), what,
+         std::string("the state ") + s.name + " must be a contiguous " + c10::toString(kind) + " tensor of " + std::to_string(size) +
+             " elements on the parameter's device");
+    if (s.untyped) row->*s.untyped = x.data_ptr();
+    else row->*s.typed = (float *) x.data_ptr();
+    e.held.push_back({s.key, x.data_ptr()});
+  }
+  return e;
+}
+
+// plan(entries, launches, bits): entries [(param, group, state, master, address of its table row)], launches
 // [(n, address of the table, param type, gradient type, bits, beta1, beta2, eps)]
 PyObject *make_plan(PyObject *, PyObject *args) {
   PyObject *entries, *launches;
-  if (!PyArg_ParseTuple(args, "O!O!", &PyList_Type, &entries, &PyList_Type, &launches)) return nullptr;
+  int bits;
+  if (!PyArg_ParseTuple(args, "O!O!i", &PyList_Type, &entries, &PyList_Type, &launches, &bits)) return nullptr;
   auto *plan = new Plan;
   PyObject *capsule = PyCapsule_New(plan, "fsgs.plan", free_plan);
   if (!capsule) {
@@ -101,31 +159,26 @@ PyObject *make_plan(PyObject *, PyObject *args) {
   }
   plan->keep = PyTuple_Pack(2, entries, launches);
   plan->params_key = PyUnicode_InternFromString("params");
+  c10::Device device(at::kCPU);
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(entries); ++i) {
-    PyObject *param, *state, *names;
+    PyObject *param, *state;
     Py_ssize_t group;
+    int master;
     unsigned long long row;
-    if (!PyArg_ParseTuple(PyList_GET_ITEM(entries, i), "OnO!O!K", &param, &group, &PyDict_Type, &state, &PyTuple_Type, &names, &row)) {
+    if (!PyArg_ParseTuple(PyList_GET_ITEM(entries, i), "OnO!pK", &param, &group, &PyDict_Type, &state, &master, &row)) {
       Py_DECREF(capsule);
       return nullptr;
     }
-    if (!THPVariable_Check(param) || !THPVariable_Unpack(param).grad().defined()) {
+    try {
+      if (i == 0 && THPVariable_Check(param)) device = THPVariable_Unpack(param).device();
+      plan->entries.push_back(entry_of(param, group, state, master, bits, (fsgs_adamw_tensor *) row, device));
+    } catch (const std::exception &e) {
       Py_DECREF(capsule);
-      return refuse("AdamW: a parameter without a gradient");
+      return refuse(e.what());
     }
-    const at::Tensor &t = THPVariable_Unpack(param);
-    Entry e{param, state, group, t.data_ptr(), t.numel(), t.scalar_type(), t.grad().scalar_type(), {}, (fsgs_adamw_tensor *) row};
-    for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(names); ++k) {
-      PyObject *name = PyTuple_GET_ITEM(names, k), *v = PyDict_GetItem(state, name);
-      if (!v || !THPVariable_Check(v)) {
-        Py_DECREF(capsule);
-        return refuse("AdamW: a parameter's state is incomplete");
-      }
-      e.held.push_back({name, THPVariable_Unpack(v).data_ptr()});
-    }
-    plan->place.emplace(param, plan->entries.size());
+    const Entry &e = plan->entries.back();
+    plan->place.emplace(param, plan->entries.size() - 1);
     plan->norm.push_back({nullptr, e.numel, type_of(e.grad_type)});
-    plan->entries.push_back(std::move(e));
   }
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(launches); ++i) {
     Launch l;
@@ -217,32 +270,51 @@ PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
-// norm(tensors, max_norm, workspace, its bytes, out, stream)
+fsgs_stream_t stream_of(const at::Tensor &t) { return (fsgs_stream_t) c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+PyObject *tuple_of(std::initializer_list<at::Tensor> list) {
+  PyObject *out = PyTuple_New((Py_ssize_t) list.size());
+  Py_ssize_t i = 0;
+  for (const at::Tensor &t : list) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
+  return out;
+}
+
+// norm(tensors, max_norm, workspace bytes) -> (norm, factor)
 PyObject *norm_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 6 || !PyList_Check(args[0])) return refuse("fsgs_host.norm: wrong arguments");
-  auto at = [&](int k) { return (uintptr_t) PyLong_AsUnsignedLongLong(args[k]); };
+  if (n != 3 || !PyList_Check(args[0])) return refuse("fsgs_host.norm: wrong arguments");
   const float max_norm = (float) PyFloat_AsDouble(args[1]);
-  void *ws = (void *) at(2);
-  const size_t bytes = at(3);
-  float *out = (float *) at(4);
-  const auto stream = (fsgs_stream_t) at(5);
+  const long long bytes = PyLong_AsLongLong(args[2]);
   if (PyErr_Occurred()) return nullptr;
-  static const char *want = "grad_norm: dense float32, bfloat16 or float16 CUDA tensors on one device";
   try {
+    const at::NoGradGuard none;
     const Py_ssize_t count = PyList_GET_SIZE(args[0]);
+    need(count > 0, "grad_norm", "no tensors");
     std::vector<fsgs_norm_tensor> table((size_t) count);
+    std::vector<at::Tensor> kept;
     c10::Device device(at::kCPU);
     for (Py_ssize_t i = 0; i < count; ++i) {
       PyObject *o = PyList_GET_ITEM(args[0], i);
-      if (!THPVariable_Check(o)) return refuse(want);
-      const at::Tensor &t = THPVariable_Unpack(o);
-      if (i == 0) device = t.device();
-      const int type = type_of(t.scalar_type());
-      if (!t.is_cuda() || t.device() != device || t.layout() != at::kStrided || type < 0) return refuse(want);
-      if (!t.is_contiguous()) return PyLong_FromLong(kStrided);
-      table[(size_t) i] = {t.data_ptr(), t.numel(), type};
+      const bool tensor = THPVariable_Check(o);
+      if (tensor && i == 0) device = THPVariable_Unpack(o).device();
+      need(tensor && THPVariable_Unpack(o).is_cuda() && THPVariable_Unpack(o).device() == device &&
+               THPVariable_Unpack(o).layout() == at::kStrided && type_of(THPVariable_Unpack(o).scalar_type()) >= 0,
+           "grad_norm", "dense float32, bfloat16 or float16 CUDA tensors on one device");
     }
-    return PyLong_FromLong(lib.norm((int) count, table.data(), max_norm, ws, bytes, out, stream));
+    const c10::cuda::CUDAGuard guard(device);
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      const at::Tensor &t = THPVariable_Unpack(PyList_GET_ITEM(args[0], i));
+      const at::Tensor *d = &t;
+      if (!t.is_contiguous()) {
+        kept.push_back(t.contiguous());
+        d = &kept.back();
+      }
+      table[(size_t) i] = {d->data_ptr(), d->numel(), type_of(d->scalar_type())};
+    }
+    const auto options = at::TensorOptions().device(device);
+    at::Tensor out = at::empty({2}, options.dtype(at::kFloat)), ws = at::empty({bytes}, options.dtype(at::kByte));
+    const int rc = lib.norm((int) count, table.data(), max_norm, ws.data_ptr(), (size_t) bytes, out.data_ptr<float>(), stream_of(out));
+    need(rc == 0, "fsgs_grad_norm", std::string(lib.status_string(rc)) + " (status " + std::to_string(rc) + ")");
+    return tuple_of({out.select(0, 0), out.select(0, 1)});
   } catch (const std::exception &e) {
     return refuse(e.what());
   }
@@ -253,10 +325,6 @@ PyObject *norm_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
 using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-void need(bool ok, const char *what, const char *message) {
-  if (!ok) throw std::runtime_error(std::string(what) + ": " + message);
-}
 
 void check(int rc, const char *what) {
   if (rc != 0) throw std::runtime_error(std::string(what) + ": " + lib.status_string(rc) + " (status " + std::to_string(rc) + ")");
@@ -291,8 +359,6 @@ int check_table(const Tensor &table, const Tensor &idx, const std::optional<Tens
 
 const uint8_t *bytes_of(const std::optional<Tensor> &mask) { return mask ? (const uint8_t *) mask->data_ptr() : nullptr; }
 std::optional<Tensor> dense(const std::optional<Tensor> &mask) { return mask ? std::optional<Tensor>(mask->contiguous()) : mask; }
-fsgs_stream_t stream_of(const Tensor &t) { return (fsgs_stream_t) c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
-
 struct Counted {
   Tensor counts, ws;  // counts [M + 4]
 };
@@ -393,13 +459,6 @@ std::optional<Tensor> mask_of(const char *what, PyObject *o) {
   if (o == Py_None) return std::nullopt;
   need(THPVariable_Check(o), what, "mask must be bool [N] on the same device");
   return THPVariable_Unpack(o);
-}
-
-PyObject *tuple_of(std::initializer_list<Tensor> list) {
-  PyObject *out = PyTuple_New((Py_ssize_t) list.size());
-  Py_ssize_t i = 0;
-  for (const Tensor &t : list) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
-  return out;
 }
 
 // balance_pairs(weights, idx, M, mask, weight, grad, autograd) -> (loss, counts) or (loss, grad, counts)

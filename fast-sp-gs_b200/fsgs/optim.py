@@ -144,31 +144,15 @@ _table_type = np.dtype([(n, np.float32 if t is ctypes.c_float else np.int64) for
 assert _table_type.itemsize == ctypes.sizeof(_lib.AdamWTensor)
 
 
-def _norm_workspace(device):
-    return torch.zeros(int(lib().fsgs_grad_norm_workspace_bytes()), dtype=torch.uint8, device=device)
-
-
 def grad_norm(tensors, max_norm=None):
     """``(norm, factor)``: the 2-norm of all elements of all ``tensors`` (float32, bfloat16 or float16, on one device)
     and ``min(1, max_norm / (norm + 1e-6))``, the factor that clips them to ``max_norm`` -- 1 without ``max_norm``, 0
-    where the norm is not finite.  Two float32 device scalars, one launch (per 256 tensors) and no synchronisation; the
-    factor can be given to ``AdamW.step(grad_scale=...)``.  Summed in a fixed order: the same gradients give the same
-    bits."""
-    tensors = list(tensors)
-    _need(len(tensors) > 0 and isinstance(tensors[0], torch.Tensor) and tensors[0].is_cuda,
-          "grad_norm: dense float32, bfloat16 or float16 CUDA tensors on one device")
+    where the norm is not finite.  Two float32 device scalars, one pass (a launch per 256 tensors and one that closes the
+    sum) and no synchronisation; the factor can be given to ``AdamW.step(grad_scale=...)``.  Summed in a fixed order: the
+    same gradients give the same bits."""
     _need(max_norm is None or max_norm > 0, "grad_norm: max_norm must be positive")
-    device = tensors[0].device
-    with _on_device(device):
-        out, work = torch.empty(2, device=device), _norm_workspace(device)
-        args = (float("inf") if max_norm is None else float(max_norm), work.data_ptr(),
-                work.numel(), out.data_ptr(), _stream().value or 0)
-        rc = _lib.host().norm(tensors, *args)
-        if rc == _STRIDED:
-            tensors = [t.detach().contiguous() for t in tensors]
-            rc = _lib.host().norm(tensors, *args)
-        check(rc, "fsgs_grad_norm")
-    return out[0], out[1]
+    return _lib.host().norm(list(tensors), float("inf") if max_norm is None else float(max_norm),
+                            int(lib().fsgs_grad_norm_workspace_bytes()))
 
 
 class _Plan:
@@ -177,45 +161,31 @@ class _Plan:
     they are what it was made from."""
 
     def __init__(self, opt):
-        self.params = params = [p for g in opt.param_groups for p in g["params"] if p.grad is not None]
-        self.device = params[0].device
-        group_of = {id(p): k for k, g in enumerate(opt.param_groups) for p in g["params"]}
-        self.groups = [group_of[id(p)] for p in params]
-        for p in params:
-            _need(p.is_cuda and p.device == self.device, "AdamW: CUDA parameters on one device")
-            _need(p.is_contiguous() and p.dtype in _TYPES, "AdamW: contiguous float32, bfloat16 or float16 parameters")
-            _need(p.grad.layout == torch.strided and (p.grad.dtype == p.dtype or p.grad.dtype == torch.float32),
-                  "AdamW: a dense gradient of its parameter's type or float32")
-            _need(p.grad.numel() == p.numel(), "AdamW: a gradient has another size than its parameter")
-        states, names = [opt._state_of(p) for p in params], [opt._names(p) for p in params]
-        for p, st, wanted in zip(params, states, names):
-            for name in wanted:
-                _need(name in st, f"AdamW: a parameter's state has no {name}")
-                t = st[name]
-                size = (p.numel() + _BLOCK - 1) // _BLOCK if name.endswith("_scale") else 1 if name == "step" else p.numel()
-                kind = torch.float8_e4m3fn if opt.state_bits == 8 and name in ("exp_avg", "exp_avg_sq_root") else torch.float32
-                _need(t.device == self.device and t.dtype == kind and t.numel() == size and t.is_contiguous(),
-                      f"AdamW: the state {name} must be a contiguous {kind} tensor of {size} elements on {self.device}")
         self.settings = self.current_settings(opt)
-        kinds = {}
-        for i, (p, k) in enumerate(zip(params, self.groups)):
-            g = opt.param_groups[k]
-            key = (_TYPES[p.dtype], _TYPES[p.grad.dtype], "master" in names[i], tuple(g["betas"]), g["eps"])
-            kinds.setdefault(key, []).append(i)
-        self.launches, entries = [], [None] * len(params)
+        self.params, self.groups, found, kinds = [], [], [], {}
+        for k, group in enumerate(opt.param_groups):
+            tail = (tuple(group["betas"]), group["eps"])
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                _need(p.is_cuda and p.dtype in _TYPES and g.dtype in _TYPES, "AdamW: float32, bfloat16 or float16 CUDA parameters on one device")
+                master = opt.master_weights and p.dtype != torch.float32
+                kinds.setdefault((_TYPES[p.dtype], _TYPES[g.dtype], master) + tail, []).append(len(found))
+                found.append((p, k, opt._state_of(p), master))
+                self.params.append(p)
+                self.groups.append(k)
+        self.device = self.params[0].device
+        self.launches, entries = [], [None] * len(found)
         for (param_type, grad_type, _, betas, eps), rows in kinds.items():
             t = np.zeros(len(rows), _table_type)
-            address = lambda name: [states[i][name].data_ptr() if name in names[i] else 0 for i in rows]  # noqa: E731
-            t["param"], t["numel"] = [params[i].data_ptr() for i in rows], [params[i].numel() for i in rows]
-            t["step"], t["exp_avg"], t["master"] = address("step"), address("exp_avg"), address("master")
-            t["exp_avg_sq"] = address("exp_avg_sq" if opt.state_bits == 32 else "exp_avg_sq_root")
-            t["exp_avg_scale"], t["exp_avg_sq_scale"] = address("exp_avg_scale"), address("exp_avg_sq_root_scale")
-            self.launches.append((rows, t, (len(rows), t.ctypes.data, param_type, grad_type, opt.state_bits, float(betas[0]),
+            start = t.ctypes.data
+            self.launches.append((rows, t, (len(rows), start, param_type, grad_type, opt.state_bits, float(betas[0]),
                                             float(betas[1]), float(eps))))
             for k, i in enumerate(rows):
-                entries[i] = (params[i], self.groups[i], states[i], names[i], t.ctypes.data + k * _table_type.itemsize)
+                entries[i] = found[i] + (start + k * _table_type.itemsize,)
         self.rates(opt)
-        self.handle = _lib.host().plan(entries, [l[2] for l in self.launches])
+        self.handle = _lib.host().plan(entries, [l[2] for l in self.launches], opt.state_bits)
 
     @staticmethod
     def current_settings(opt):
@@ -425,7 +395,8 @@ class AdamW(torch.optim.Optimizer):
         for name, wanted, make in (("_work", True, lambda: (torch.empty(int(lib().fsgs_adamw_workspace_bytes()),
                                                                        dtype=torch.uint8, device=device),)),
                                    ("_norm", self.max_grad_norm is not None,
-                                    lambda: (torch.zeros(2, device=device), _norm_workspace(device)))):
+                                    lambda: (torch.zeros(2, device=device), torch.empty(int(lib().fsgs_grad_norm_workspace_bytes()),
+                                                                                       dtype=torch.uint8, device=device)))):
             have = getattr(self, name)
             if wanted and (have is None or have[0].device != device):
                 _need(not torch.cuda.is_current_stream_capturing(),
