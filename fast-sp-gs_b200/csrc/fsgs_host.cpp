@@ -71,6 +71,7 @@ struct Plan {
   std::vector<Launch> launches;
   std::unordered_map<PyObject *, size_t> place;
   std::vector<fsgs_norm_tensor> norm;
+  c10::Device device{at::kCPU};
   PyObject *keep = nullptr;   // the Python objects behind every pointer
   PyObject *params_key = nullptr;
 };
@@ -159,7 +160,6 @@ PyObject *make_plan(PyObject *, PyObject *args) {
   }
   plan->keep = PyTuple_Pack(2, entries, launches);
   plan->params_key = PyUnicode_InternFromString("params");
-  c10::Device device(at::kCPU);
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(entries); ++i) {
     PyObject *param, *state;
     Py_ssize_t group;
@@ -170,8 +170,8 @@ PyObject *make_plan(PyObject *, PyObject *args) {
       return nullptr;
     }
     try {
-      if (i == 0 && THPVariable_Check(param)) device = THPVariable_Unpack(param).device();
-      plan->entries.push_back(entry_of(param, group, state, master, bits, (fsgs_adamw_tensor *) row, device));
+      if (i == 0 && THPVariable_Check(param)) plan->device = THPVariable_Unpack(param).device();
+      plan->entries.push_back(entry_of(param, group, state, master, bits, (fsgs_adamw_tensor *) row, plan->device));
     } catch (const std::exception &e) {
       Py_DECREF(capsule);
       return refuse(e.what());
@@ -237,37 +237,39 @@ int walk(Plan &plan, PyObject *groups, PyObject *state) {
   return found != plan.entries.size() ? kStale : strided ? kStrided : 0;
 }
 
-// step(plan, groups, state, max_norm, norm workspace, its bytes, norm out, grad_scale, gate, workspace, its bytes, stream):
-// addresses as integers, 0 for none; norm out 0: no norm
+// step(plan, groups, state, max_norm, (norm workspace, its bytes, norm out, workspace, its bytes), grad_scale, gate): on the
+// parameters' device and its current stream; addresses as integers, 0 for none; max_norm None: no norm
 PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 12 || !PyList_Check(args[1]) || !PyDict_Check(args[2])) return refuse("fsgs_host.step: wrong arguments");
+  if (n != 7 || !PyList_Check(args[1]) || !PyDict_Check(args[2]) || !PyTuple_Check(args[4]) || PyTuple_GET_SIZE(args[4]) != 5)
+    return refuse("fsgs_host.step: wrong arguments");
   Plan *plan = (Plan *) PyCapsule_GetPointer(args[0], "fsgs.plan");
   if (!plan) return nullptr;
-  auto at = [&](int k) { return (uintptr_t) PyLong_AsUnsignedLongLong(args[k]); };
-  const float max_norm = (float) PyFloat_AsDouble(args[3]);
-  void *norm_ws = (void *) at(4), *ws = (void *) at(9);
-  const size_t norm_bytes = at(5), bytes = at(10);
-  float *norm_out = (float *) at(6);
-  const float *grad_scale = (const float *) at(7), *gate = (const float *) at(8);
-  const auto stream = (fsgs_stream_t) at(11);
+  auto word = [&](int k) { return (uintptr_t) PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(args[4], k)); };
+  const bool clip = args[3] != Py_None;
+  const float max_norm = clip ? (float) PyFloat_AsDouble(args[3]) : 0.0f;
+  void *norm_ws = (void *) word(0), *ws = (void *) word(3);
+  const size_t norm_bytes = word(1), bytes = word(4);
+  float *norm_out = clip ? (float *) word(2) : nullptr;
+  const float *grad_scale = (const float *) (uintptr_t) PyLong_AsUnsignedLongLong(args[5]);
+  const float *gate = (const float *) (uintptr_t) PyLong_AsUnsignedLongLong(args[6]);
   if (PyErr_Occurred()) return nullptr;
-  int rc;
   try {
-    rc = walk(*plan, args[1], args[2]);
+    int rc = walk(*plan, args[1], args[2]);
+    if (rc != 0) return PyLong_FromLong(rc);
+    const c10::cuda::CUDAGuard guard(plan->device);
+    const auto stream = (fsgs_stream_t) c10::cuda::getCurrentCUDAStream(plan->device.index()).stream();
+    if (norm_out) {
+      rc = lib.norm((int) plan->norm.size(), plan->norm.data(), max_norm, norm_ws, norm_bytes, norm_out, stream);
+      grad_scale = norm_out + 1;
+    }
+    for (const Launch &l : plan->launches) {
+      if (rc != 0) break;
+      rc = lib.adamw(l.n, l.table, l.param_type, l.grad_type, l.bits, l.b1, l.b2, l.eps, grad_scale, gate, ws, bytes, stream);
+    }
+    return PyLong_FromLong(rc);
   } catch (const std::exception &e) {
     return refuse(e.what());
   }
-  if (rc != 0) return PyLong_FromLong(rc);
-  if (norm_out) {
-    rc = lib.norm((int) plan->norm.size(), plan->norm.data(), max_norm, norm_ws, norm_bytes, norm_out, stream);
-    if (rc != 0) return PyLong_FromLong(rc);
-    grad_scale = norm_out + 1;
-  }
-  for (const Launch &l : plan->launches) {
-    rc = lib.adamw(l.n, l.table, l.param_type, l.grad_type, l.bits, l.b1, l.b2, l.eps, grad_scale, gate, ws, bytes, stream);
-    if (rc != 0) break;
-  }
-  return PyLong_FromLong(rc);
 }
 
 fsgs_stream_t stream_of(const at::Tensor &t) { return (fsgs_stream_t) c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }

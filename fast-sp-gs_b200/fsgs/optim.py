@@ -10,7 +10,7 @@ from torch.optim.optimizer import _global_optimizer_post_hooks, _global_optimize
 
 from . import _lib
 from ._lib import lib, check
-from .ops import _need, _on_device, _ptr, _stream
+from .ops import _need, _ptr, _stream
 
 
 class SparseGaussianAdam(torch.optim.Adam):
@@ -277,8 +277,7 @@ class AdamW(torch.optim.Optimizer):
             for p in group["params"]:
                 _need(p.is_cuda, "AdamW: CUDA parameters on one device")
                 self._state_of(p)
-                with _on_device(p.device):
-                    self._workspaces(p.device)
+                self._workspaces(p.device)
 
     def _state_of(self, p):
         st = self.state[p]
@@ -344,10 +343,11 @@ class AdamW(torch.optim.Optimizer):
 
     def step_gated(self, gate=None, grad_scale=None):
         """The body of ``step``, without hooks."""
-        for t in (gate, grad_scale):
-            _need(t is None or (t.is_cuda and t.numel() == 1 and t.dtype == torch.float32),
-                  "AdamW: gate and grad_scale are one-element float32 tensors on the parameters' device")
-        _need(grad_scale is None or self.max_grad_norm is None, "AdamW: grad_scale together with max_grad_norm")
+        if gate is not None or grad_scale is not None:
+            for t in (gate, grad_scale):
+                _need(t is None or (t.is_cuda and t.numel() == 1 and t.dtype == torch.float32),
+                      "AdamW: gate and grad_scale are one-element float32 tensors on the parameters' device")
+            _need(grad_scale is None or self.max_grad_norm is None, "AdamW: grad_scale together with max_grad_norm")
         plan = self._plan
         if plan is None or not plan.follow(self):
             plan = self._new_plan()
@@ -377,31 +377,30 @@ class AdamW(torch.optim.Optimizer):
         return self._plan
 
     def _run(self, plan, gate, grad_scale):
-        device = plan.device
-        for t in (gate, grad_scale):
-            _need(t is None or t.device == device, "AdamW: gate and grad_scale are on the parameters' device")
-        with _on_device(device):
+        device, clip = plan.device, self.max_grad_norm
+        if self._work is None or self._work[0] != device or (clip is not None and self._norm is None):
             self._workspaces(device)
-            work, clip = self._work[0], self.max_grad_norm is not None
-            norm = (float(self.max_grad_norm), self._norm[1].data_ptr(), self._norm[1].numel(), self._norm[0].data_ptr()) \
-                if clip else (0.0, 0, 0, 0)
-            return _lib.host().step(plan.handle, self.param_groups, self.state, *norm,
-                                    0 if grad_scale is None else grad_scale.data_ptr(),
-                                    0 if gate is None else gate.data_ptr(), work.data_ptr(), work.numel(),
-                                    _stream().value or 0)
+        scale = where = 0
+        if grad_scale is not None:
+            _need(grad_scale.device == device, "AdamW: gate and grad_scale are on the parameters' device")
+            scale = grad_scale.data_ptr()
+        if gate is not None:
+            _need(gate.device == device, "AdamW: gate and grad_scale are on the parameters' device")
+            where = gate.data_ptr()
+        return _lib.host().step(plan.handle, self.param_groups, self.state, clip, self._words, scale, where)
 
     def _workspaces(self, device):
         """Created once and never replaced on the same device: a captured step goes on using them."""
-        for name, wanted, make in (("_work", True, lambda: (torch.empty(int(lib().fsgs_adamw_workspace_bytes()),
-                                                                       dtype=torch.uint8, device=device),)),
-                                   ("_norm", self.max_grad_norm is not None,
-                                    lambda: (torch.zeros(2, device=device), torch.empty(int(lib().fsgs_grad_norm_workspace_bytes()),
-                                                                                       dtype=torch.uint8, device=device)))):
-            have = getattr(self, name)
-            if wanted and (have is None or have[0].device != device):
-                _need(not torch.cuda.is_current_stream_capturing(),
-                      "AdamW: take a step, or call init_state(), before a step is captured")
-                setattr(self, name, make())
+        _need(not torch.cuda.is_current_stream_capturing(),
+              "AdamW: take a step, or call init_state(), before a step is captured")
+        space = lambda n: torch.empty(int(n), dtype=torch.uint8, device=device)  # noqa: E731
+        if self._work is None or self._work[0] != device:
+            self._work, self._norm = (device, space(lib().fsgs_adamw_workspace_bytes())), None
+        if self.max_grad_norm is not None and self._norm is None:
+            self._norm = (torch.zeros(2, device=device), space(lib().fsgs_grad_norm_workspace_bytes()))
+        work, norm = self._work[1], self._norm
+        self._words = (norm[1].data_ptr(), norm[1].numel(), norm[0].data_ptr()) if norm is not None else (0, 0, 0)
+        self._words += (work.data_ptr(), work.numel())
 
 
 _hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW.step_gated)
