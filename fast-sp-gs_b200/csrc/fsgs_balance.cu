@@ -78,7 +78,8 @@ __device__ __forceinline__ T block_total(T v, T *scratch) {  // valid in the fir
 
 // One pass over the indices: a histogram per block in shared memory, added to the 64-bit counts at the end.  In the pairs
 // form the superpoint of every pair is kept as a 16- or 32-bit code (all ones: does not count) for the pass that needs the
-// complete counts, which then reads 2 bytes per pair instead of 8 and no mask.  In the table form the block that finishes
+// complete counts, which then reads 2 bytes per pair instead of 8 and no mask, most of it from L2 (the indices are read,
+// and the weights and gradients of that pass streamed, so as not to displace the codes).  In the table form the block that finishes
 // last turns the counts into shares.  Bound by the read of the indices and, beside it, by one shared-memory atomic per pair.
 template <typename Code>
 __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long long N, int K, int M, const int64_t *__restrict__ idx,
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long lo
   };
   const long long quads = wide ? pairs / 4 : 0;
   for (long long q = first; q < quads; q += stride) {
-    const longlong2 a = reinterpret_cast<const longlong2 *>(idx)[2 * q], b = reinterpret_cast<const longlong2 *>(idx)[2 * q + 1];
+    const longlong2 a = __ldcs(reinterpret_cast<const longlong2 *>(idx) + 2 * q), b = __ldcs(reinterpret_cast<const longlong2 *>(idx) + 2 * q + 1);
     bool on[4] = {true, true, true, true};
     if (mask) {
       long long row;
@@ -119,11 +120,17 @@ __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long lo
         row = 4 * q / K;
       }
       int col = (int) (4 * q - row * K);
-      on[0] = mask[row] != 0;
+      if (K >= 4) {  // at most two rows
+        const bool r0 = mask[row] != 0, r1 = col + 3 >= K ? mask[row + 1] != 0 : r0;
 #pragma unroll
-      for (int u = 1; u < 4; ++u) {
-        on[u] = on[u - 1];
-        if (++col == K) col = 0, on[u] = mask[++row] != 0;
+        for (int u = 0; u < 4; ++u) on[u] = col + u < K ? r0 : r1;
+      } else {
+        on[0] = mask[row] != 0;
+#pragma unroll
+        for (int u = 1; u < 4; ++u) {
+          on[u] = on[u - 1];
+          if (++col == K) col = 0, on[u] = mask[++row] != 0;
+        }
       }
     }
     const Code c[4] = {take(a.x, on[0]), take(a.y, on[1]), take(b.x, on[2]), take(b.y, on[3])};
@@ -206,7 +213,7 @@ __global__ void __launch_bounds__(kPairThreads, 2) balance_pairs_kernel(PairsArg
   auto fetch = [&](long long q) {
 #pragma unroll
     for (int u = 0; u < kWords; ++u) nc[u] = reinterpret_cast<const uint4 *>(codes)[kWords * q + u];
-    if (a.loss) nw[0] = reinterpret_cast<const float4 *>(a.w)[2 * q], nw[1] = reinterpret_cast<const float4 *>(a.w)[2 * q + 1];
+    if (a.loss) nw[0] = __ldcs(reinterpret_cast<const float4 *>(a.w) + 2 * q), nw[1] = __ldcs(reinterpret_cast<const float4 *>(a.w) + 2 * q + 1);
   };
   if (first < eights) fetch(first);
   const double parts = (double) a.counts[a.M] * (double) a.counts[a.M + 1], unit = parts > 0.0 ? (double) a.M / parts : 0.0;
@@ -241,7 +248,7 @@ __global__ void __launch_bounds__(kPairThreads, 2) balance_pairs_kernel(PairsArg
         const float4 ox = o[0], oy = o[1];
         x.x += ox.x, x.y += ox.y, x.z += ox.z, x.w += ox.w, y.x += oy.x, y.y += oy.y, y.z += oy.z, y.w += oy.w;
       }
-      o[0] = x, o[1] = y;
+      __stcs(o, x), __stcs(o + 1, y);
     }
   }
   for (long long e = 8 * eights + first; e < a.pairs; e += stride) {
