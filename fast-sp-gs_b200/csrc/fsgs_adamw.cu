@@ -224,9 +224,8 @@ __device__ __forceinline__ void update(const float *g, float *m, float *v, float
     plain_sum(mul2(a, both(s.b1)), mul2(gs, both(s.c1)), m[u], m[u + 1]);
     plain_sum(mul2(b, both(-s.b2)), mul2(mul2(gs, gs), both(-s.c2)), v[u], v[u + 1]);  // -v'
   }
-  // a NaN among others passes: its own root is a NaN either way.  An infinite v passes with 8-bit moments only, where it
-  // spoils its block whatever its root is.
-  const bool plain = high8(v) <= -kSafe && (EIGHT || top8(v) < INFINITY);
+  // a NaN among others passes: its own root is a NaN either way
+  const bool plain = high8(v) <= -kSafe && !(top8(v) == INFINITY);
   float q[8];  // -sqrt(v')
   neg_roots(v, q, plain);
 #pragma unroll

@@ -386,8 +386,8 @@ __global__ void __launch_bounds__(kTableThreads) balance_table_kernel(TableArgs 
   const int t = threadIdx.x % G;
   const float up = a.scale * (a.upstream ? *a.upstream : 1.0f);
   auto row_of = [&](int r) { return ((long long) blockIdx.x * ROWS + r) * kGroups + threadIdx.x / G; };
-  // groups of this row may reach past it into its neighbours
-  auto inside = [&](long long i) { return i * a.stride >= 3 && (i + 1 < a.N ? a.stride : (long long) a.M) >= (long long) a.M + 3; };
+  // the table goes on for three elements before and behind this row
+  auto inside = [&](long long i) { return i * a.stride >= 3 && (a.N - 1 - i) * a.stride >= 3; };
   auto moved_of = [&](const T *z) { return (int) ((uintptr_t) z / sizeof(T) & 3); };
   Four<T> raw[ROWS][PER > 0 ? PER / 4 : 1];
   bool on[ROWS];

@@ -465,3 +465,19 @@ def test_moments_are_the_formula_operation_by_operation(bits):
         code, top = pack(x, positive)
         assert torch.equal(rows(st[name]).float(), code.float()), name
         assert bool(((st[name + "_scale"] - top[:, 0] / 448.0).abs() <= 2 * E * top[:, 0] / 448.0).all()), name
+
+
+def test_a_gradient_whose_square_overflows():
+    """|g| = 1e21: the second moment is infinite, the element's update zero (m / infinity) in 32 and in 8 bits; with 8 bits
+    its block's moments are spoiled, its neighbours' parameters of this step are not."""
+    from fsgs.optim import AdamW
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.ones(600, device="cuda"))
+        g = torch.full((600,), 1e-2, device="cuda")
+        g[300] = 1e21
+        p.grad = g
+        AdamW([p], lr=1e-3, weight_decay=0.0, state_bits=bits).step()
+        assert float(p[300]) == 1.0
+        others = torch.cat([p.detach()[:300], p.detach()[301:]])
+        # first step: m / (1 - b1) = g, sqrt(v / (1 - b2)) = |g|
+        assert float((others - (1.0 - 1e-3 / (1 + 1e-8 / 1e-2))).abs().max()) <= 44 * E
