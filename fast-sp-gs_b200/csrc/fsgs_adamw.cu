@@ -14,7 +14,13 @@
 //
 // The update itself is done in float32 with the roundings of the written formula, one per operation, no contraction of
 // the moments' sums: a moment next to a border between two 8-bit values then falls on the side on which the formula
-// evaluated operation by operation falls.
+// evaluated operation by operation falls.  The quotient m' / (...) alone is approximate (1 unit of the reciprocal).
+//
+// What bounds it: memory.  28 bytes per element in float32 (parameter and moments in and out, gradient in), 16 with 8-bit
+// moments, 10 with bf16 parameters and gradients too.  Measured on one B200 (copy 6.57 TB/s; device time, states larger
+// than L2): 116 M float32 elements 469 us (6.9 TB/s); 17.4 M with 8-bit moments 48 us (5.8 TB/s, of which 4 are launches);
+// 116 M bf16 with 8-bit moments 201 us (5.8 TB/s; 36 instructions per element, half of them packed pairs), the norm of
+// their gradients 50 us before it; 60 k float32 elements 6 us, two launches.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -293,12 +299,12 @@ __global__ void __launch_bounds__(kOptCapacity) adamw_begin_kernel(const __grid_
 // leaves the order to the hardware, which hands out thread blocks as others finish, each reading all that it needs before
 // it writes: the memory in use at any moment is one short stretch of every array, and DRAM pages are opened once.  Measured
 // (us; 116 M elements in float32 with float32 moments | bf16 with 8-bit moments, the norm before it included):
-//   this order                                                                  469 | 258
+//   this order                                                                  469 | 256
 //   a grid that fills the device, blocks interleaved (2 / 3 thread blocks an SM)  507 / 598 | 320
 //   every warp a run of its own                                                 588 | 269
 //   bulk copies through a ring in shared memory, 3 thread blocks an SM            - | 293, and 272 with no arithmetic at all
 //   this order, a warp's second block loaded while the first is computed        592 | 290
-// Two blocks per warp where an element brings 4 bytes of parameter and gradient (258 against 281: half the address and
+// Two blocks per warp where an element brings 4 bytes of parameter and gradient (256 against 281: half the address and
 // argument work per element), one where it brings more (49 against 57 us for 17.4 M float32 elements: the second
 // block's registers push the loads behind the first block's stores).
 template <typename P, typename G, bool EIGHT, bool MASTER>
@@ -424,6 +430,9 @@ static int adamw_pick(bool eight, bool master, const AdamWCall &c) {
 // the norm of all gradients
 // ------------------------------------------------------------------------------------------------
 
+// One pass over all gradients, bound by its read: 464 MB of float32 in 71 us (6.6 TB/s), 232 MB of bf16 in 50 us; a small
+// call is two launches, 5 us.  Every thread block adds its share in double and leaves it in a slot of its own; a block of a
+// second launch adds the slots.  No counter, nothing to prepare: a workspace can be used again as soon as a call is done.
 struct NormEntry {
   const void *data;
   long long numel;
