@@ -22,7 +22,7 @@ constexpr int kBalSharedPoints = 8192;    // superpoints whose histogram or shar
 constexpr int kCountThreads = 1024;
 constexpr int kPairThreads = 512;
 constexpr int kTableThreads = 256;
-constexpr int kBalSlots = 296;            // partial sums
+constexpr int kBalSlots = 296;            // partial sums of the pairs form: two blocks an SM
 
 // The workspace: this, then the codes of the pairs (pairs form) or four copies of the shares, copy s moved up by s places
 // (table form).
@@ -81,15 +81,14 @@ __device__ __forceinline__ T block_total(T v, T *scratch) {  // valid in the fir
 // complete counts, which then reads 2 bytes per pair instead of 8 and no mask, most of it from L2 (the indices are read,
 // and the weights and gradients of that pass streamed, so as not to displace the codes).  In the table form the block that finishes
 // last turns the counts into shares.  Bound by the read of the indices and, beside it, by one shared-memory atomic per pair.
-template <typename Code>
+template <typename Code, bool SHARED>
 __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long long N, int K, int M, const int64_t *__restrict__ idx,
     const uint8_t *__restrict__ mask, int wide, unsigned magic, unsigned long long *__restrict__ counts, BalanceHead *__restrict__ head,
     float *__restrict__ share, Code *__restrict__ codes) {
   extern __shared__ int s_hist[];   // [M + 1]: the last one takes what does not count
   __shared__ long long s_red[kCountThreads / 32];
   __shared__ int s_last;
-  const bool in_shared = M <= kBalSharedPoints;
-  if (in_shared) {
+  if (SHARED) {
     for (int m = threadIdx.x; m <= M; m += kCountThreads) s_hist[m] = 0;
     __syncthreads();
   }
@@ -97,14 +96,14 @@ __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long lo
   const long long first = (long long) blockIdx.x * kCountThreads + threadIdx.x;
   long long named = 0, rows = 0;
   auto take = [&](int64_t m, bool on) -> Code {
-    on = on && (uint64_t) m < (uint64_t) M;
-    if (in_shared) {
-      atomicAdd(s_hist + (on ? (int) m : M), 1);
-    } else if (on) {
+    const unsigned bin = on && (unsigned) (m >> 32) == 0 ? min((unsigned) m, (unsigned) M) : (unsigned) M;
+    if (SHARED) {
+      atomicAdd(s_hist + bin, 1);
+    } else if (bin < (unsigned) M) {
       ++named;
-      atomicAdd(counts + m, 1ull);
+      atomicAdd(counts + bin, 1ull);
     }
-    return on ? (Code) m : (Code) ~(Code) 0;
+    return bin < (unsigned) M ? (Code) bin : (Code) ~(Code) 0;
   };
   const long long quads = wide ? pairs / 4 : 0;
   for (long long q = first; q < quads; q += stride) {
@@ -146,7 +145,7 @@ __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long lo
   if (mask)
     for (long long i = first; i < N; i += stride) rows += mask[i] != 0;
   __syncthreads();
-  if (in_shared)
+  if (SHARED)
     for (int m = threadIdx.x; m < M; m += kCountThreads) {
       const int c = s_hist[m];
       if (c) atomicAdd(counts + m, (unsigned long long) c);
@@ -596,8 +595,10 @@ extern "C" int fsgs_balance_count(int64_t N, int K, int M, const int64_t *idx, c
   const int wide = ((uintptr_t) idx & 15) == 0;
   const unsigned magic = K > 1 && N * K < (1ll << 32) ? (unsigned) ((1ull << 32) / (unsigned) K) : 0u;
   void *codes = form == FSGS_BALANCE_PAIRS ? w.codes : nullptr;
-  if (code_bytes(M) == 2) balance_count_kernel<uint16_t><<<grid, kCountThreads, smem, st>>>(N, K, M, idx, mask, wide, magic, c, w.head, w.share, (uint16_t *) codes);
-  else balance_count_kernel<uint32_t><<<grid, kCountThreads, smem, st>>>(N, K, M, idx, mask, wide, magic, c, w.head, w.share, (uint32_t *) codes);
+  const auto kernel32 = balance_count_kernel<uint32_t, false>;  // 65536 superpoints and more are never in shared memory
+  if (M <= kBalSharedPoints) balance_count_kernel<uint16_t, true><<<grid, kCountThreads, smem, st>>>(N, K, M, idx, mask, wide, magic, c, w.head, w.share, (uint16_t *) codes);
+  else if (code_bytes(M) == 2) balance_count_kernel<uint16_t, false><<<grid, kCountThreads, 0, st>>>(N, K, M, idx, mask, wide, magic, c, w.head, w.share, (uint16_t *) codes);
+  else kernel32<<<grid, kCountThreads, 0, st>>>(N, K, M, idx, mask, wide, magic, c, w.head, w.share, (uint32_t *) codes);
   FSGS_LAUNCH_CHECK();
   return FSGS_OK;
 }
