@@ -19,7 +19,7 @@
 // What bounds it: memory.  28 bytes per element in float32 (parameter and moments in and out, gradient in), 16 with 8-bit
 // moments, 10 with bf16 parameters and gradients too.  Measured on one B200 (copy 6.57 TB/s; device time, states larger
 // than L2): 116 M float32 elements 469 us (6.9 TB/s); 17.4 M with 8-bit moments 48 us (5.8 TB/s, of which 4 are launches);
-// 116 M bf16 with 8-bit moments 201 us (5.8 TB/s; 36 instructions per element, half of them packed pairs), the norm of
+// 116 M bf16 with 8-bit moments 201 us (5.8 TB/s; 41 instructions per element, 69 % of the issue slots), the norm of
 // their gradients 50 us before it; 60 k float32 elements 6 us, two launches.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

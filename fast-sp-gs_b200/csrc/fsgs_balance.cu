@@ -10,6 +10,13 @@
 // off the difference is between small numbers, where M c_m / T are all near 1 and their difference would lose the digits
 // that they have in common.  The counts are integers, so the centred share (M c_m - T) / (T n) is exact up to its one
 // rounding to float32.
+//
+// What bounds it: memory.  Pairs: 8 bytes of index, 4 of weight and 4 of gradient per pair and, between the two passes,
+// 2 bytes of code that mostly stay in L2; table: the table in and its gradient out, once each.  Measured on one B200 (copy
+// 6.57 TB/s; device time): 2 M x 8 pairs over 4096 superpoints 59 us, 30 counting (160 MB at 5.3 TB/s; neither the
+// shared-memory atomics nor their flush show: 30.9 and 29.0 us without them) and 27 for loss and gradient (160 MB at 5.9
+// TB/s); 300 k x 3 over 512 12 us in three nodes; table 300 k x 512 float32, value and gradient, 178 us (6.9 TB/s) and 12
+// of counting and closing; bf16 171 us in all (3.7 TB/s, bound by instructions: 28 per column and lane).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

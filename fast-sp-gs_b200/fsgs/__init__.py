@@ -4,7 +4,8 @@
 ``fsgs.install``   makes the reference's own Python (``fast_2d_gs.renderer``, ``utils.cdist_top``,
                    ``fast_2d_gs.sparse_gaussian_adam``) bind to these operators, unmodified
 ``fsgs.renderer``  ``GS_2D_fast_render`` with the reference's signature and result dictionary
-``fsgs.optim``     ``SparseGaussianAdam`` (single fused launch)
+``fsgs.optim``     ``SparseGaussianAdam`` (single fused launch); ``AdamW`` over many dense tensors, ``grad_norm``
+``fsgs.loss``      L1 + SSIM image loss; balance of the Gaussians over the superpoints
 ``fsgs.dist``      one-view-per-GPU sharding with NCCL all-reduce of per-Gaussian gradients
 """
 from .install import install  # noqa: F401
