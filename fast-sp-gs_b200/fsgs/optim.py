@@ -224,7 +224,8 @@ class AdamW(torch.optim.Optimizer):
       scale.  The rounding is to nearest: second moments of elements that move against their block by less than a
       sixteenth per step stay where they are.  A gradient that is not finite spoils its block of 256.
     * ``master_weights=True``: 16-bit parameters are updated through a float32 copy in the state (``master``); without
-      it an update below half a unit of the parameter's last place is lost.
+      it an update below half a unit of the parameter's last place is lost.  The copy is then the parameter: who sets
+      parameters from outside sets it too (or clears the state).
     * ``max_grad_norm``: every step is preceded by the norm of all its gradients and clips by it; ``self.grad_norm``
       is the last norm (a device scalar, overwritten by the next step).  A step whose norm is not finite is dropped.
 

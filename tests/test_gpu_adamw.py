@@ -481,3 +481,56 @@ def test_a_gradient_whose_square_overflows():
         others = torch.cat([p.detach()[:300], p.detach()[301:]])
         # first step: m / (1 - b1) = g, sqrt(v / (1 - b2)) = |g|
         assert float((others - (1.0 - 1e-3 / (1 + 1e-8 / 1e-2))).abs().max()) <= 44 * E
+
+
+def test_two_graphs_of_one_optimiser():
+    """Two captured steps of the same optimiser, each with gradients of its own, replayed in turn beside eager steps: they
+    share its state, counts and workspaces."""
+    from fsgs.optim import AdamW
+    a, _ = _make((3000, 40), torch.float32, torch.float32)
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    oa, ob = (AdamW(x, lr=1e-2, state_bits=8, max_grad_norm=0.2) for x in (a, b))
+    oa.init_state()
+    sets = [_make((3000, 40), torch.float32, torch.float32, seed=s)[1] for s in (31, 32, 33)]
+    graphs = []
+    for grads in sets[:2]:
+        for p, g in zip(a, grads):
+            p.grad = g
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            oa.step()
+        graphs.append(graph)
+    for k in (0, 1, 2, 1, 0, 2, 0):
+        for p, q, g in zip(a, b, sets[k]):
+            p.grad, q.grad = g, g
+        if k < 2:
+            graphs[k].replay()
+        else:
+            oa.step()
+        ob.step()
+        assert torch.equal(oa.grad_norm, ob.grad_norm)
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+            assert all(torch.equal(oa.state[p][n].float(), t.float()) for n, t in ob.state[q].items())
+
+
+def test_tensors_beyond_32_bits_of_elements():
+    """2^31 + 777 bf16 elements with 8-bit moments, clipped: the ends against the formula, the norm against a double sum."""
+    from fsgs.optim import AdamW
+    n = 2 ** 31 + 777
+    p = torch.nn.Parameter(torch.full((n,), 0.5, dtype=torch.bfloat16, device="cuda"))
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g[:5000] = 1.0
+    g[-5000:] = -2.0
+    g[n // 2] = 4.0
+    p.grad = g
+    opt = AdamW([p], lr=0.25, weight_decay=0.0, state_bits=8, max_grad_norm=1e9)
+    opt.step()
+    assert abs(float(opt.grad_norm) - math.sqrt(5000 + 20000 + 16)) <= 5 * E * 160
+    # the first step is lr sign(g): m / (1 - b1) = g, sqrt(v / (1 - b2)) = |g|; bf16 at 0.25 and 0.75 rounds to 2^-8 of them
+    assert float((p[:5000].float() - 0.25).abs().max()) <= 0.25 * 2.0 ** -8
+    assert float((p[-5000:].float() - 0.75).abs().max()) <= 0.75 * 2.0 ** -8
+    assert float((p[n // 2].float() - 0.25).abs()) <= 0.25 * 2.0 ** -8
+    assert bool((p[5000:10_000] == 0.5).all()) and bool((p[-10_000:-5000] == 0.5).all())
+    st = opt.state[p]
+    assert st["exp_avg_scale"].numel() == (n + B - 1) // B and float(st["exp_avg_scale"][-1]) > 0

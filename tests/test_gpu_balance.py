@@ -256,3 +256,40 @@ def test_autograd_of_the_losses():
     g, = torch.autograd.grad(loss ** 2, d, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivative"):
         g.sum().backward()
+
+
+def test_pairs_at_odd_addresses():
+    """Indices, weights and the gradient that is added to, each one element off an aligned start: the same results."""
+    from fsgs.loss import balance_value_and_grad
+    gen = torch.Generator().manual_seed(8)
+    N, K, M = 3001, 3, 77
+    idx, w = _indices(N, K, M, gen, 0.05).cuda(), torch.rand(N, K, generator=gen).cuda()
+    mask = (torch.rand(N, generator=gen) > 0.2).cuda()
+    loss, grad, counts = balance_value_and_grad(w, idx, M, mask=mask)
+    odd = lambda t: torch.cat([t.reshape(-1)[:1], t.reshape(-1)])[1:].view(t.shape)  # noqa: E731
+    into = odd(torch.ones_like(w))
+    loss2, same, counts2 = balance_value_and_grad(odd(w), odd(idx), M, mask=odd(mask), grad=into)
+    assert torch.equal(counts, counts2) and same is into
+    assert abs(float(loss) - float(loss2)) <= 4 * E * float(loss)
+    assert torch.equal(into, 1.0 + grad)
+
+
+def test_tables_beyond_32_bits_of_elements():
+    """600 k x 4000 bf16, 2.4e9 elements: the first and the last rows against the formula."""
+    from fsgs.loss import table_balance_value_and_grad
+    N, M = 600_000, 4000
+    gen = torch.Generator("cuda").manual_seed(1)
+    z = torch.empty(N, M, dtype=torch.bfloat16, device="cuda")
+    z.normal_(generator=gen)
+    idx = (torch.rand(N, 2, device="cuda", generator=gen) ** 2 * M).long().clamp_(max=M - 1)
+    weight = 2.0 ** 20                      # brings the gradients into the range in which bf16 keeps its precision
+    loss, grad, counts = table_balance_value_and_grad(z, idx, weight=weight)
+    assert torch.equal(counts, torch.bincount(idx.reshape(-1), minlength=M))
+    f = M * counts.double() / (2 * N) / N
+    for rows in (slice(0, 50), slice(N - 50, N)):
+        p = torch.softmax(z[rows].double(), dim=1)
+        want = weight * p * (f - (p @ f)[:, None])
+        centred = (M * counts.double() - 2 * N) / (2 * N) / N
+        tol = weight * (2 * 12 + M / 32 + 28) * E * p * (centred.abs() + 2 * (p * centred.abs()).sum(dim=1, keepdim=True))
+        assert bool(((grad[rows].double() - want).abs() <= tol + HALF[torch.bfloat16] * (want.abs() + tol)).all())
+    assert math.isfinite(float(loss))
