@@ -28,6 +28,7 @@ using NormFn = int (*)(int, const fsgs_norm_tensor *, float, void *, size_t, flo
 struct {
   AdamWFn adamw;
   NormFn norm;
+  size_t (*norm_bytes)(void);
   size_t (*balance_bytes)(int64_t, int, int, int);
   int (*balance_count)(int64_t, int, int, const int64_t *, const uint8_t *, int, int64_t *, void *, size_t, fsgs_stream_t);
   int (*balance_pairs)(int64_t, int, int, const float *, const int64_t *, void *, size_t, float, const float *, float *, float *,
@@ -281,11 +282,10 @@ PyObject *tuple_of(std::initializer_list<at::Tensor> list) {
   return out;
 }
 
-// norm(tensors, max_norm, workspace bytes) -> (norm, factor)
+// norm(tensors, max_norm) -> (norm, factor)
 PyObject *norm_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 3 || !PyList_Check(args[0])) return refuse("fsgs_host.norm: wrong arguments");
+  if (n != 2 || !PyList_Check(args[0])) return refuse("fsgs_host.norm: wrong arguments");
   const float max_norm = (float) PyFloat_AsDouble(args[1]);
-  const long long bytes = PyLong_AsLongLong(args[2]);
   if (PyErr_Occurred()) return nullptr;
   try {
     const at::NoGradGuard none;
@@ -313,6 +313,7 @@ PyObject *norm_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
       table[(size_t) i] = {d->data_ptr(), d->numel(), type_of(d->scalar_type())};
     }
     const auto options = at::TensorOptions().device(device);
+    const int64_t bytes = (int64_t) lib.norm_bytes();
     at::Tensor out = at::empty({2}, options.dtype(at::kFloat)), ws = at::empty({bytes}, options.dtype(at::kByte));
     const int rc = lib.norm((int) count, table.data(), max_norm, ws.data_ptr(), (size_t) bytes, out.data_ptr<float>(), stream_of(out));
     need(rc == 0, "fsgs_grad_norm", std::string(lib.status_string(rc)) + " (status " + std::to_string(rc) + ")");

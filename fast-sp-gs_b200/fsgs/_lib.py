@@ -217,8 +217,8 @@ def host():
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         module.bind(*(ctypes.cast(getattr(lib(), name), c_void_p).value for name in (
-            "fsgs_adamw_multi", "fsgs_grad_norm", "fsgs_balance_workspace_bytes", "fsgs_balance_count", "fsgs_balance_pairs",
-            "fsgs_balance_table", "fsgs_status_string")))
+            "fsgs_adamw_multi", "fsgs_grad_norm", "fsgs_grad_norm_workspace_bytes", "fsgs_balance_workspace_bytes",
+            "fsgs_balance_count", "fsgs_balance_pairs", "fsgs_balance_table", "fsgs_status_string")))
         _host = module
     return _host
 

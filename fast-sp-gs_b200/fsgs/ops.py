@@ -6,7 +6,6 @@ pybind11 function of the same name in the reference extension ``fast_2d_gs/_C`` 
 pointers and the current CUDA stream go to the C ABI.  Errors surface as ``RuntimeError`` like the
 reference's ``TORCH_CHECK``s.  There is no CPU path.
 """
-import contextlib
 import ctypes
 
 import torch
@@ -40,14 +39,6 @@ def _stream():
     if _raw_stream is not None:
         return ctypes.c_void_p(_raw_stream(torch.cuda.current_device()))
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-_same_device = contextlib.nullcontext()
-
-
-def _on_device(device):
-    """Context in which ``device`` is torch's current device: launches then go to it and to its current stream."""
-    return _same_device if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _ptr(t):

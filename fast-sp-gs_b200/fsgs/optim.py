@@ -151,8 +151,7 @@ def grad_norm(tensors, max_norm=None):
     sum) and no synchronisation; the factor can be given to ``AdamW.step(grad_scale=...)``.  Summed in a fixed order: the
     same gradients give the same bits."""
     _need(max_norm is None or max_norm > 0, "grad_norm: max_norm must be positive")
-    return _lib.host().norm(list(tensors), float("inf") if max_norm is None else float(max_norm),
-                            int(lib().fsgs_grad_norm_workspace_bytes()))
+    return _lib.host().norm(list(tensors), float("inf") if max_norm is None else float(max_norm))
 
 
 class _Plan:
@@ -309,12 +308,16 @@ class AdamW(torch.optim.Optimizer):
                 _need(value.numel() == fresh.numel() and (value.dtype == fresh.dtype or name == "step"),
                       f"AdamW: the loaded {name} has another size or type")
                 loaded.setdefault(p, {})[name] = fresh.copy_(value.reshape(fresh.shape))
-        before = {p: self.state[p] for p in own if p in self.state}
+        before = {p: self.state[p] for p in own if self.state.get(p)}
         super().load_state_dict(dict(state_dict, state={}))
-        for p, new in loaded.items():
-            st = before.get(p, {})
-            if set(st) == set(new) and all(st[n].shape == t.shape and st[n].dtype == t.dtype and st[n].device == t.device
-                                           for n, t in new.items()):
+        for p in own:
+            st, new = before.get(p), loaded.get(p)
+            if st is not None and new is None:      # no state: as before the first step
+                new = {n: self._fresh(p, n) for n in self._names(p)}
+            if new is None:
+                continue
+            if st is not None and set(st) == set(new) and all(st[n].shape == t.shape and st[n].dtype == t.dtype and
+                                                              st[n].device == t.device for n, t in new.items()):
                 for n, t in new.items():   # into the tensors that are there: a captured step goes on using them
                     st[n].copy_(t)
                 new = st

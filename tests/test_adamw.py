@@ -95,3 +95,15 @@ def test_copies_keep_their_settings():
     b = copy.deepcopy(a)
     assert (b.state_bits, b.master_weights, b.max_grad_norm) == (8, True, 2.0) and b.grad_norm is None
     assert {len(s) for s in b.state.values()} == {6}
+
+
+def test_loading_a_state_that_has_none_starts_again_in_place():
+    """What a fresh optimiser saves has no state: a loaded one starts again as new, in the tensors that it had (a captured
+    step may be using them)."""
+    a = _with_state(AdamW(_params(torch.bfloat16), state_bits=8, master_weights=True))
+    held = {p: dict(st) for p, st in a.state.items()}
+    a.load_state_dict(AdamW(_params(torch.bfloat16), state_bits=8, master_weights=True).state_dict())
+    for p, before in held.items():
+        st = a.state[p]
+        assert all(st[n] is t for n, t in before.items()) and torch.equal(st["master"], p.detach().float())
+        assert all(not bool(st[n].float().any()) for n in st if n != "master")
