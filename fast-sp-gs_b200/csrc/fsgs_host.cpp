@@ -8,6 +8,7 @@
 // A CPython extension compiled against torch's headers; it holds no CUDA code and calls libfsgs.so through the function
 // pointers that bind() gives it.
 #include <Python.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -404,6 +405,24 @@ Tensor once(const Tensor &grad, const Tensor &upstream) {
   return (*error)({grad.detach().set_requires_grad(true)})[0];
 }
 
+// The engine hands a gradient over on the stream on which the node that takes it was made, and a leaf keeps one node as long
+// as any graph of it lives.  Under capture, with that node from a stream outside the capture, the hand-over would end the
+// capture with an error; so it is refused before, and the capture stays good.
+void hand_over(const char *what) {
+  const auto stream = c10::cuda::getCurrentCUDAStream();
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  const auto next = node && node->num_outputs() ? node->next_edge(0).function : nullptr;
+  const auto theirs = next ? next->stream() : std::nullopt;
+  if (!theirs || *theirs == stream.unwrap()) return;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  const bool known = cudaStreamIsCapturing(c10::cuda::CUDAStream(*theirs).stream(), &status) == cudaSuccess;
+  if (!known) (void) cudaGetLastError();
+  need(known && status == cudaStreamCaptureStatusActive, what,
+       "a backward pass is being captured, but a graph made earlier on another stream still holds the input: let go of its "
+       "loss first, or capture the value_and_grad form");
+}
+
 struct PairsLoss : torch::autograd::Function<PairsLoss> {
   static variable_list forward(AutogradContext *ctx, const Tensor &weights, const Tensor &idx, int64_t M, const std::optional<Tensor> &mask) {
     const c10::cuda::CUDAGuard guard(weights.device());
@@ -421,6 +440,7 @@ struct PairsLoss : torch::autograd::Function<PairsLoss> {
     const auto saved = ctx->get_saved_variables();
     const Counted c{saved[0], saved[1]};
     const c10::cuda::CUDAGuard guard(c.ws.device());
+    hand_over(kPairs);
     const int64_t N = ctx->saved_data["N"].toInt(), K = ctx->saved_data["K"].toInt();
     Tensor grad = at::empty({N, K}, g[0].options().requires_grad(false));
     pairs(N, K, c, nullptr, 1.0f, g[0].data_ptr<float>(), nullptr, grad.data_ptr<float>(), false);
@@ -445,6 +465,7 @@ struct TableLoss : torch::autograd::Function<TableLoss> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &t = saved[0];
     const c10::cuda::CUDAGuard guard(t.device());
+    hand_over(kTable);
     Tensor grad = at::empty(t.sizes(), t.options().requires_grad(false));
     table_pass(t, type_of(t.scalar_type()), saved[1].defined() ? std::optional<Tensor>(saved[1]) : std::nullopt,
                Counted{saved[2], saved[3]}, 1.0f, g[0].data_ptr<float>(), nullptr, grad.data_ptr());

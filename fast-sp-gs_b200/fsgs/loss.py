@@ -84,7 +84,11 @@ def balance_loss(weights, idx, M, mask=None):
 
     is 1 when every superpoint has its share.  Differentiable in ``weights`` (the counts carry no gradient).  ``mask``
     (bool [N]): the Gaussians that count, ``n`` of them; an index outside 0 .. M-1 is a pair that does not count.  No
-    Gaussian or no pair that counts: loss 0.  No synchronisation; the same inputs give the same bits."""
+    Gaussian or no pair that counts: loss 0.  No synchronisation; the same inputs give the same bits.
+
+    Forward and backward can be captured into a CUDA graph.  While an earlier graph of ``weights``, made on a stream outside
+    the capture, is still alive (a loss that somebody holds), the captured backward pass raises: its gradient could not be
+    handed over.  ``balance_value_and_grad`` has no such limit."""
     return host().balance_pairs(weights, idx, int(M), mask, 1.0, None, True)
 
 
@@ -102,7 +106,8 @@ def table_balance_loss(table, idx, mask=None):
 
     ``balance_loss`` with the probabilities of all superpoints in the place of the K blend weights, differentiable in
     ``table`` (gradient in its type).  A row of nothing but -infinity adds nothing.  ``mask``, indices outside 0 .. M-1
-    and ``counts`` as in ``balance_loss``."""
+    and ``counts`` as in ``balance_loss``; a captured backward pass too.  The gradient of a table
+    of N rows is of the order of a probability times M / N: below 6e-8 a float16 table loses it, so scale the loss."""
     return host().balance_table(table, idx, mask, 1.0, True)
 
 

@@ -293,3 +293,74 @@ def test_tables_beyond_32_bits_of_elements():
         tol = weight * (2 * 12 + M / 32 + 28) * E * p * (centred.abs() + 2 * (p * centred.abs()).sum(dim=1, keepdim=True))
         assert bool(((grad[rows].double() - want).abs() <= tol + HALF[torch.bfloat16] * (want.abs() + tol)).all())
     assert math.isfinite(float(loss))
+
+
+def test_a_captured_backward_pass():
+    """Forward and backward of both losses in one graph, no other graph of the leaves alive; replayed with other inputs."""
+    from fsgs.loss import balance_loss, balance_value_and_grad, table_balance_loss, table_balance_value_and_grad
+    gen = torch.Generator().manual_seed(9)
+    N, K, M = 700, 2, 40
+    idx = _indices(N, K, M, gen).cuda()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        z, w = torch.randn(N, M, device="cuda").requires_grad_(), torch.rand(N, K, device="cuda").requires_grad_()
+
+        def both():
+            a, b = table_balance_loss(z, idx)[0], balance_loss(w, idx, M)[0]
+            return torch.autograd.grad(a + b, (z, w))
+
+        both()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            held = both()
+        for k in range(2):
+            with torch.no_grad():
+                z.copy_(torch.randn(N, M, device="cuda"))
+            idx.copy_((idx + 7) % M)
+            graph.replay()
+            assert torch.equal(held[0], table_balance_value_and_grad(z, idx)[1])
+            assert torch.equal(held[1], balance_value_and_grad(w, idx, M)[1])
+    torch.cuda.current_stream().wait_stream(stream)
+
+
+@pytest.mark.parametrize("of", ["pairs", "table"])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_a_captured_backward_pass_beside_a_living_graph(of, accumulate):
+    """A loss of the same leaf is held, made on another stream: refused, and the same capture goes on without the backward."""
+    from fsgs.loss import balance_loss, balance_value_and_grad, table_balance_loss, table_balance_value_and_grad
+    gen = torch.Generator().manual_seed(10)
+    N, K, M = 300, 2, 20
+    idx = _indices(N, K, M, gen).cuda()
+    x = (torch.rand(N, K, generator=gen) if of == "pairs" else torch.randn(N, M, generator=gen)).cuda().requires_grad_()
+    loss = (lambda: balance_loss(x, idx, M)[0]) if of == "pairs" else (lambda: table_balance_loss(x, idx)[0])
+    values = (lambda: balance_value_and_grad(x, idx, M)) if of == "pairs" else (lambda: table_balance_value_and_grad(x, idx))
+    held = loss()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        values()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            captured = loss()
+            with pytest.raises(RuntimeError, match="value_and_grad"):
+                captured.backward() if accumulate else torch.autograd.grad(captured, x)
+            out = values()
+        graph.replay()
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    want = values()
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]) and torch.equal(captured.detach(), want[0])
+    assert x.grad is None
+    (grad,) = torch.autograd.grad(held, x)                          # the held graph works as before
+    assert torch.equal(grad, want[1])
+    del captured, held                                              # let go of: the same capture now holds its backward pass
+    with torch.cuda.stream(stream):
+        torch.autograd.grad(loss(), x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            (again,) = torch.autograd.grad(loss(), x)
+        graph.replay()
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(again, want[1])
