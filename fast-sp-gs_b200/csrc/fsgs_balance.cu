@@ -532,8 +532,6 @@ __global__ void __launch_bounds__(32) balance_close_kernel(BalanceHead *head, co
 }
 static_assert(kFixedSlots == 32, "one warp closes the sum");
 
-// `reach`: columns from the first group of four to the row's end, M where every row starts on a boundary of four elements.
-// `reach`: columns from the first group of four to the row's end, M where every row starts on a boundary of four elements.
 template <typename T, int G, int PER, int ROWS>
 static int table_launch(TableArgs &a, cudaStream_t st) {
   const int rows = kTableThreads / G * ROWS;
@@ -551,6 +549,8 @@ static int table_launch(TableArgs &a, cudaStream_t st) {
 // and gradient (us; one row a thread group | two): 300 k x 512 bf16 177 | 171, 400 k x 256 bf16 140 | 123, 1 M x 100 bf16
 // 148 | 155, 2 M x 40 bf16 209 | 189; float32 is bound by memory (300 k x 512: 190 us, 6.5 TB/s) and takes one.  A warp
 // per row reaches to 1024 columns (100 k x 1000: 138 us, a block per row 244), a block per row lies above.
+//
+// `reach`: columns from the first group of four to the row's end, M where every row starts on a boundary of four elements.
 template <typename T>
 static int table_pick(TableArgs &a, int reach, cudaStream_t st) {
   constexpr int R = sizeof(T) == 2 ? 2 : 1;

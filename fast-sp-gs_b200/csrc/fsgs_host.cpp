@@ -15,7 +15,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 #include "../../include/fsgs.h"
@@ -148,6 +150,15 @@ Entry entry_of(PyObject *param, Py_ssize_t group, PyObject *state, bool master, 
   return e;
 }
 
+// All tensors of a launch are updated at once, so none may be part of another.
+void need_apart(const std::vector<Entry> &entries) {
+  std::vector<std::pair<const char *, const char *>> spans;
+  for (const Entry &e : entries)
+    if (e.numel > 0) spans.emplace_back((const char *) e.data, (const char *) e.data + e.numel * c10::elementSize(e.type));
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i) need(spans[i].first >= spans[i - 1].second, "AdamW", "two parameters share memory");
+}
+
 // plan(entries, launches, bits): entries [(param, group, state, master, address of its table row)], launches
 // [(n, address of the table, param type, gradient type, bits, beta1, beta2, eps)]
 PyObject *make_plan(PyObject *, PyObject *args) {
@@ -181,6 +192,12 @@ PyObject *make_plan(PyObject *, PyObject *args) {
     const Entry &e = plan->entries.back();
     plan->place.emplace(param, plan->entries.size() - 1);
     plan->norm.push_back({nullptr, e.numel, type_of(e.grad_type)});
+  }
+  try {
+    need_apart(plan->entries);
+  } catch (const std::exception &e) {
+    Py_DECREF(capsule);
+    return refuse(e.what());
   }
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(launches); ++i) {
     Launch l;

@@ -212,8 +212,8 @@ class AdamW(torch.optim.Optimizer):
         ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
         ``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)``.
 
-    Parameters are contiguous CUDA tensors of float32, bfloat16 or float16 on one device, gradients of the parameter's
-    type or (``param.grad_dtype``) float32.  ``lr``, ``betas``, ``eps`` and ``weight_decay`` are per group and may be
+    Parameters are contiguous CUDA tensors of float32, bfloat16 or float16 on one device that share no memory, gradients
+    of the parameter's type or (``param.grad_dtype``) float32.  ``lr``, ``betas``, ``eps`` and ``weight_decay`` are per group and may be
     changed between steps.
 
     * ``state_bits=32``: state ``step`` (float32 device scalar), ``exp_avg``, ``exp_avg_sq`` (float32): the layout of
@@ -245,6 +245,8 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, group):
         super().add_param_group(group)
         g = self.param_groups[-1]
+        _need(not any(torch.is_tensor(v) and v.is_cuda for v in (g["lr"], g["weight_decay"], g["eps"], *g["betas"])),
+              "AdamW: lr, betas, eps and weight_decay are numbers on the host (a step would wait for the device to read them)")
         _need(float(g["lr"]) >= 0 and g["eps"] >= 0 and g["weight_decay"] >= 0 and
               all(0 <= b < 1 for b in g["betas"]), "AdamW: lr, eps, weight_decay >= 0 and 0 <= beta < 1")
         for p in g["params"]:
@@ -292,7 +294,12 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As ``torch.optim.Optimizer.load_state_dict``, with every state tensor kept in its own type (the base class
         casts them to the parameter's) and copied to the parameter's device.  A state in another number of bits, or
-        without the master copy that this optimiser keeps, is refused."""
+        without the master copy that this optimiser keeps, is refused, and so are groups of another rule (``amsgrad``,
+        ``maximize``, a weight decay that is added to the gradient)."""
+        for g in state_dict["param_groups"]:
+            _need(not g.get("amsgrad") and not g.get("maximize") and
+                  (g.get("decoupled_weight_decay", True) or not g.get("weight_decay")),
+                  "AdamW: the loaded state is of amsgrad, maximize or a weight decay that is not decoupled")
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         own = [p for g in self.param_groups for p in g["params"]]
         _need(len(ids) == len(own), "AdamW: the loaded state has another number of parameters")

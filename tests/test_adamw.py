@@ -107,3 +107,22 @@ def test_loading_a_state_that_has_none_starts_again_in_place():
         st = a.state[p]
         assert all(st[n] is t for n, t in before.items()) and torch.equal(st["master"], p.detach().float())
         assert all(not bool(st[n].float().any()) for n in st if n != "master")
+
+
+@pytest.mark.parametrize("of", [lambda p: torch.optim.AdamW(p, amsgrad=True), lambda p: torch.optim.AdamW(p, maximize=True),
+                                lambda p: torch.optim.Adam(p, weight_decay=0.1)])
+def test_state_dicts_of_another_rule_are_refused(of):
+    opt = AdamW(_params())
+    with pytest.raises(RuntimeError, match="amsgrad"):
+        opt.load_state_dict(of(_params()).state_dict())
+    opt.load_state_dict(torch.optim.Adam(_params()).state_dict())    # without weight decay the two are one
+
+
+def test_a_schedule_follows_the_steps():
+    opt = AdamW(_params(), lr=1.0)
+    schedule = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.5)
+    for _ in range(2):
+        opt.step()                             # nothing has a gradient
+        schedule.step()
+    assert opt.param_groups[0]["lr"] == 0.25 and schedule.get_last_lr() == [0.25]
+    AdamW(_params(), lr=torch.tensor(0.5))     # on the host: read at each step

@@ -534,3 +534,29 @@ def test_tensors_beyond_32_bits_of_elements():
     assert bool((p[5000:10_000] == 0.5).all()) and bool((p[-10_000:-5000] == 0.5).all())
     st = opt.state[p]
     assert st["exp_avg_scale"].numel() == (n + B - 1) // B and float(st["exp_avg_scale"][-1]) > 0
+
+
+def test_parameters_that_share_memory_are_refused():
+    from fsgs.optim import AdamW
+    base = torch.zeros(1000, device="cuda")
+    for a, b in ((base, base), (base[:500], base[499:]), (base[100:101], base)):
+        params = [torch.nn.Parameter(a), torch.nn.Parameter(b)]
+        for p in params:
+            p.grad = torch.ones_like(p)
+        with pytest.raises(RuntimeError, match="share memory"):
+            AdamW(params).step()
+    assert not bool(base.any())
+    params = [torch.nn.Parameter(x) for x in (base[500:], base[:500], base[500:500])]   # neighbours, and an empty one inside
+    for p in params:
+        p.grad = torch.ones_like(p)
+    AdamW(params, lr=0.5, weight_decay=0.0).step()
+    # the first step is lr g / (|g| + eps), 40 E U off
+    assert float((base + 0.5 / (1 + 1e-8)).abs().max()) <= 40 * E * 0.5
+
+
+def test_numbers_on_the_device_are_refused():
+    from fsgs.optim import AdamW
+    p = [torch.nn.Parameter(torch.zeros(8, device="cuda"))]
+    for kw in (dict(lr=torch.tensor(1e-3, device="cuda")), dict(weight_decay=torch.tensor(0.1, device="cuda"))):
+        with pytest.raises(RuntimeError, match="numbers on the host"):
+            AdamW(p, **kw)
