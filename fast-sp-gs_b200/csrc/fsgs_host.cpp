@@ -51,6 +51,13 @@ int type_of(at::ScalarType t) {
 struct StateTensor {
   PyObject *name;
   void *data;
+  int64_t numel;
+  at::ScalarType type;
+  // still a dense tensor of that length and type there: the kernels trust all of it
+  bool is(const at::Tensor &x, c10::Device device) const {
+    return x.layout() == at::kStrided && x.device() == device && x.scalar_type() == type && x.numel() == numel && x.is_contiguous() &&
+           x.data_ptr() == data;
+  }
 };
 
 struct Entry {
@@ -145,7 +152,7 @@ Entry entry_of(PyObject *param, Py_ssize_t group, PyObject *state, bool master, 
              " elements on the parameter's device");
     if (s.untyped) row->*s.untyped = x.data_ptr();
     else row->*s.typed = (float *) x.data_ptr();
-    e.held.push_back({s.key, x.data_ptr()});
+    e.held.push_back({s.key, x.data_ptr(), size, kind});
   }
   return e;
 }
@@ -237,7 +244,7 @@ int walk(Plan &plan, PyObject *groups, PyObject *state) {
       strided = strided || !grad.is_contiguous();
       for (const StateTensor &h : e.held) {
         PyObject *v = PyDict_GetItem(e.state, h.name);
-        if (!v || !THPVariable_Check(v) || THPVariable_Unpack(v).data_ptr() != h.data) return kStale;
+        if (!v || !THPVariable_Check(v) || !h.is(THPVariable_Unpack(v), plan.device)) return kStale;
       }
       e.row->grad = grad.data_ptr();
       plan.norm[i].data = e.row->grad;

@@ -160,7 +160,7 @@ class _Plan:
     they are what it was made from."""
 
     def __init__(self, opt):
-        self.settings = self.current_settings(opt)
+        self.settings, self.form = self.current_settings(opt), self.current_form(opt)
         self.params, self.groups, found, kinds = [], [], [], {}
         for k, group in enumerate(opt.param_groups):
             tail = (tuple(group["betas"]), group["eps"])
@@ -190,8 +190,14 @@ class _Plan:
     def current_settings(opt):
         return [(float(g["lr"]), float(g["weight_decay"]), *g["betas"], g["eps"]) for g in opt.param_groups]
 
+    @staticmethod
+    def current_form(opt):
+        return opt.state_bits, opt.master_weights
+
     def follow(self, opt):
-        """Take over changed learning rates and weight decays; False where betas or eps changed."""
+        """Take over changed learning rates and weight decays; False where betas, eps or the form of the state changed."""
+        if self.current_form(opt) != self.form:
+            return False
         now = self.current_settings(opt)
         if now != self.settings:
             if [s[2:] for s in now] != [s[2:] for s in self.settings]:

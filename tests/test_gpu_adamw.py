@@ -560,3 +560,58 @@ def test_numbers_on_the_device_are_refused():
     for kw in (dict(lr=torch.tensor(1e-3, device="cuda")), dict(weight_decay=torch.tensor(0.1, device="cuda"))):
         with pytest.raises(RuntimeError, match="numbers on the host"):
             AdamW(p, **kw)
+
+
+def test_states_that_changed_where_they_lie_are_refused():
+    """A state tensor cut, of another type, transposed or replaced at the same address since the last step, and another form
+    of the state asked for: refused before anything is launched; put back, the next step is the formula's."""
+    from fsgs.optim import AdamW
+    for bits, dtype, master in ((32, torch.float32, False), (8, torch.bfloat16, True)):
+        params, grads = _make((600, 24), dtype, torch.float32)
+        for p, g in zip(params, grads):
+            p.grad = g
+        opt = AdamW(params, state_bits=bits, master_weights=master)
+        opt.step()
+        st = opt.state[params[1]]
+
+        def refused(what):
+            frozen = [t.clone() for p in params for t in [p.detach()] + list(opt.state[p].values())]
+            with pytest.raises(RuntimeError, match=what):
+                opt.step()
+            after = [t for p in params for t in [p.detach()] + list(opt.state[p].values())]
+            assert all(torch.equal(a.float(), b.float()) for a, b in zip(frozen, after))
+
+        for name in [n for n in st if n != "step"]:
+            whole = st[name]
+            there = whole.data_ptr()
+            changed = [whole.view(torch.int8).view(-1)[:whole.numel()], whole.view(-1)[:whole.numel() // 2]]
+            if whole.numel() == 24:
+                changed.append(whole.view(6, 4).t())
+            for other in changed:
+                assert other.data_ptr() == there or other.numel() == 0
+                st[name] = other
+                refused(name)
+                st[name] = whole
+            whole.data, kept = whole.data.view(-1)[:0], whole.data        # the same tensor, cut in place
+            refused(name)
+            whole.data = kept
+        # given back and replaced by a shorter one, for which the allocator may hand out the same address
+        name = "exp_avg"
+        kept = st[name].clone()
+        del whole, changed, other, st[name]
+        st[name] = torch.zeros(7, dtype=kept.dtype, device="cuda")
+        refused(name)
+        st[name] = kept
+        opt.state_bits = 40 - bits
+        refused("state")
+        opt.state_bits = bits
+        if dtype != torch.float32:
+            del st["master"]
+            opt.master_weights = False
+            opt.step()                                                   # a state that has what is asked for
+            opt.master_weights = True
+            refused("master")
+            st["master"] = params[1].detach().float()
+        before = _snapshot(opt, params)
+        opt.step()
+        _check_step(opt, before, params, grads)
