@@ -53,6 +53,7 @@ struct StateTensor {
   void *data;
   int64_t numel;
   at::ScalarType type;
+  PyObject *now;   // the tensor that the last walk found
   // still a dense tensor of that length and type there: the kernels trust all of it
   bool is(const at::Tensor &x, c10::Device device) const {
     return x.layout() == at::kStrided && x.device() == device && x.scalar_type() == type && x.numel() == numel && x.is_contiguous() &&
@@ -152,7 +153,7 @@ Entry entry_of(PyObject *param, Py_ssize_t group, PyObject *state, bool master, 
              " elements on the parameter's device");
     if (s.untyped) row->*s.untyped = x.data_ptr();
     else row->*s.typed = (float *) x.data_ptr();
-    e.held.push_back({s.key, x.data_ptr(), size, kind});
+    e.held.push_back({s.key, x.data_ptr(), size, kind, v});
   }
   return e;
 }
@@ -242,9 +243,10 @@ int walk(Plan &plan, PyObject *groups, PyObject *state) {
       if (grad.scalar_type() != e.grad_type || grad.layout() != at::kStrided || grad.device() != t.device() || grad.numel() != e.numel)
         return kStale;
       strided = strided || !grad.is_contiguous();
-      for (const StateTensor &h : e.held) {
+      for (StateTensor &h : e.held) {
         PyObject *v = PyDict_GetItem(e.state, h.name);
         if (!v || !THPVariable_Check(v) || !h.is(THPVariable_Unpack(v), plan.device)) return kStale;
+        h.now = v;
       }
       e.row->grad = grad.data_ptr();
       plan.norm[i].data = e.row->grad;
@@ -261,6 +263,18 @@ int walk(Plan &plan, PyObject *groups, PyObject *state) {
     ++found;
   }
   return found != plan.entries.size() ? kStale : strided ? kStrided : 0;
+}
+
+// What a kernel writes counts as modified in place: a graph that has saved it then raises instead of using the new values.
+void written(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+void written(const Plan &plan) {
+  for (const Entry &e : plan.entries) {
+    written(THPVariable_Unpack(e.param));
+    for (const StateTensor &h : e.held) written(THPVariable_Unpack(h.now));
+  }
 }
 
 // step(plan, groups, state, max_norm, (norm workspace, its bytes, norm out, workspace, its bytes), grad_scale, gate): on the
@@ -282,6 +296,7 @@ PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   try {
     int rc = walk(*plan, args[1], args[2]);
     if (rc != 0) return PyLong_FromLong(rc);
+    written(*plan);
     const c10::cuda::CUDAGuard guard(plan->device);
     const auto stream = (fsgs_stream_t) c10::cuda::getCurrentCUDAStream(plan->device.index()).stream();
     if (norm_out) {

@@ -615,3 +615,29 @@ def test_states_that_changed_where_they_lie_are_refused():
         before = _snapshot(opt, params)
         opt.step()
         _check_step(opt, before, params, grads)
+
+
+def test_a_step_marks_what_it_writes():
+    """A graph that has saved a parameter before a step raises in its backward pass, as after torch's optimisers; every
+    state that a step writes counts as modified, gradients do not, and tensors without a version are left alone."""
+    from fsgs.loss import table_balance_loss
+    from fsgs.optim import AdamW
+    for bits, dtype, master in ((32, torch.float32, False), (8, torch.bfloat16, True)):
+        z = torch.nn.Parameter(torch.randn(60, 40, device="cuda").to(dtype))
+        z.grad = torch.ones_like(z)
+        opt = AdamW([z], state_bits=bits, master_weights=master)
+        opt.step()
+        table, _ = table_balance_loss(z, torch.zeros(60, 2, dtype=torch.int64, device="cuda"))
+        square = (z * z).sum()
+        held = [z] + list(opt.state[z].values())
+        before, grad = [t._version for t in held], z.grad._version
+        opt.step()
+        assert all(t._version > v for t, v in zip(held, before)) and z.grad._version == grad
+        for loss in (table, square):
+            with pytest.raises(RuntimeError, match="modified"):
+                loss.backward()
+        with torch.inference_mode():
+            p = torch.zeros(5, device="cuda")
+            p.grad = torch.ones(5, device="cuda")
+            AdamW([p], lr=0.5, weight_decay=0.0, state_bits=bits).step()
+        assert float((p + 0.5 / (1 + 1e-8)).abs().max()) <= 40 * E * 0.5     # the first step is lr g / (|g| + eps)
