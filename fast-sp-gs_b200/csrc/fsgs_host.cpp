@@ -105,6 +105,11 @@ void need(bool ok, const char *what, const std::string &message) {
   if (!ok) throw std::runtime_error(std::string(what) + ": " + message);
 }
 
+// What a kernel writes counts as modified in place: a graph that has saved it then raises instead of using the new values.
+void written(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // The names of a parameter's state, and where in its table row the address goes.
 struct Slot {
   const char *name;
@@ -263,11 +268,6 @@ int walk(Plan &plan, PyObject *groups, PyObject *state) {
     ++found;
   }
   return found != plan.entries.size() ? kStale : strided ? kStrided : 0;
-}
-
-// What a kernel writes counts as modified in place: a graph that has saved it then raises instead of using the new values.
-void written(const at::Tensor &t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 void written(const Plan &plan) {
@@ -551,6 +551,7 @@ PyObject *balance_pairs(PyObject *, PyObject *const *args, Py_ssize_t n) {
     Tensor loss = at::empty({}, w.options().requires_grad(false));
     if (!add) grad = at::empty(w.sizes(), w.options().requires_grad(false));
     pairs(idx.size(0), idx.size(1), c, w.data_ptr<float>(), weight, nullptr, loss.data_ptr<float>(), grad.data_ptr<float>(), add);
+    if (add) written(grad);
     return tuple_of({loss, grad, c.counts.narrow(0, 0, M)});
   } catch (const std::exception &e) {
     return refuse(e.what());

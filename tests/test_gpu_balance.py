@@ -364,3 +364,20 @@ def test_a_captured_backward_pass_beside_a_living_graph(of, accumulate):
         graph.replay()
     torch.cuda.current_stream().wait_stream(stream)
     assert torch.equal(again, want[1])
+
+
+def test_the_gradient_added_to_counts_as_modified():
+    from fsgs.loss import balance_value_and_grad
+    into = torch.zeros(50, 2, device="cuda")
+    factor = torch.ones(50, 2, device="cuda", requires_grad=True)
+    loss = (factor * into).sum()                   # saves `into`
+    version = into._version
+    w, idx = torch.rand(50, 2, device="cuda"), torch.zeros(50, 2, dtype=torch.int64, device="cuda")
+    balance_value_and_grad(w, idx, 5, grad=into)
+    assert into._version > version and w._version == 0 and idx._version == 0
+    with pytest.raises(RuntimeError, match="modified"):
+        loss.backward()
+    with torch.inference_mode():
+        plain = torch.zeros(50, 2, device="cuda")
+        balance_value_and_grad(w, idx, 5, grad=plain)
+    assert torch.equal(plain, into)
