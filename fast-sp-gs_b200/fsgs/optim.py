@@ -250,7 +250,14 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, group):
         super().add_param_group(group)
-        g = self.param_groups[-1]
+        try:
+            self._check_group(self.param_groups[-1])
+        except RuntimeError:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check_group(g):
         _need(not any(torch.is_tensor(v) and v.is_cuda for v in (g["lr"], g["weight_decay"], g["eps"], *g["betas"])),
               "AdamW: lr, betas, eps and weight_decay are numbers on the host (a step would wait for the device to read them)")
         _need(float(g["lr"]) >= 0 and g["eps"] >= 0 and g["weight_decay"] >= 0 and

@@ -126,3 +126,14 @@ def test_a_schedule_follows_the_steps():
         schedule.step()
     assert opt.param_groups[0]["lr"] == 0.25 and schedule.get_last_lr() == [0.25]
     AdamW(_params(), lr=torch.tensor(0.5))     # on the host: read at each step
+
+
+@pytest.mark.parametrize("bad", [dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(weight_decay=float("nan")),
+                                 dict(params=[torch.zeros(3, dtype=torch.float64)])])
+def test_a_refused_group_is_not_kept(bad):
+    opt = AdamW(_params(), lr=1e-3)
+    with pytest.raises(RuntimeError):
+        opt.add_param_group(dict(dict(params=[torch.zeros(3)]), **bad))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[torch.zeros(3)], lr=0.5))
+    assert [g["lr"] for g in opt.param_groups] == [1e-3, 0.5]
