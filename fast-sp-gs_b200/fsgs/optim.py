@@ -252,7 +252,7 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(group)
         try:
             self._check_group(self.param_groups[-1])
-        except RuntimeError:
+        except Exception:
             self.param_groups.pop()
             raise
 

@@ -137,3 +137,11 @@ def test_a_refused_group_is_not_kept(bad):
     assert len(opt.param_groups) == 1
     opt.add_param_group(dict(params=[torch.zeros(3)], lr=0.5))
     assert [g["lr"] for g in opt.param_groups] == [1e-3, 0.5]
+
+
+def test_a_group_with_settings_of_another_kind_is_not_kept():
+    opt = AdamW(_params(), lr=1e-3)
+    for bad in (dict(betas=0.9), dict(lr="fast"), dict(eps=None)):
+        with pytest.raises((TypeError, ValueError)):
+            opt.add_param_group(dict(params=[torch.zeros(3)], **bad))
+    assert len(opt.param_groups) == 1
