@@ -265,6 +265,12 @@ class AdamW(torch.optim.Optimizer):
         for p in g["params"]:
             _need(p.dtype in _TYPES and p.layout == torch.strided, "AdamW: dense float32, bfloat16 or float16 parameters")
 
+    @staticmethod
+    def _on_host(g):
+        number = lambda v: float(v) if torch.is_tensor(v) and v.is_cuda else v  # noqa: E731
+        return dict(g, **{k: type(g[k])(map(number, g[k])) if k == "betas" else number(g[k])
+                          for k in ("lr", "betas", "eps", "weight_decay") if k in g})
+
     @property
     def grad_norm(self):
         """Norm of all gradients of the last step (``max_grad_norm``), before clipping; a device scalar."""
@@ -308,12 +314,16 @@ class AdamW(torch.optim.Optimizer):
         """As ``torch.optim.Optimizer.load_state_dict``, with every state tensor kept in its own type (the base class
         casts them to the parameter's) and copied to the parameter's device.  A state in another number of bits, or
         without the master copy that this optimiser keeps, is refused, and so are groups of another rule (``amsgrad``,
-        ``maximize``, a weight decay that is added to the gradient)."""
+        ``maximize``, a weight decay that is added to the gradient) and settings that the constructor refuses; numbers
+        that lie on a device are read."""
         for g in state_dict["param_groups"]:
             _need(not g.get("amsgrad") and not g.get("maximize") and
                   (g.get("decoupled_weight_decay", True) or not g.get("weight_decay")),
                   "AdamW: the loaded state is of amsgrad, maximize or a weight decay that is not decoupled")
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        groups = [self._on_host(g) for g in state_dict["param_groups"]]
+        for g in groups:
+            self._check_group(dict(self.defaults, **dict(g, params=())))
+        ids = [i for g in groups for i in g["params"]]
         own = [p for g in self.param_groups for p in g["params"]]
         _need(len(ids) == len(own), "AdamW: the loaded state has another number of parameters")
         loaded = {}
@@ -329,7 +339,7 @@ class AdamW(torch.optim.Optimizer):
                       f"AdamW: the loaded {name} has another size or type")
                 loaded.setdefault(p, {})[name] = fresh.copy_(value.reshape(fresh.shape))
         before = {p: self.state[p] for p in own if self.state.get(p)}
-        super().load_state_dict(dict(state_dict, state={}))
+        super().load_state_dict(dict(state_dict, state={}, param_groups=groups))
         for p in own:
             st, new = before.get(p), loaded.get(p)
             if st is not None and new is None:      # no state: as before the first step

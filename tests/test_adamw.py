@@ -145,3 +145,16 @@ def test_a_group_with_settings_of_another_kind_is_not_kept():
         with pytest.raises((TypeError, ValueError)):
             opt.add_param_group(dict(params=[torch.zeros(3)], **bad))
     assert len(opt.param_groups) == 1
+
+
+@pytest.mark.parametrize("bad", [dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=float("nan")), dict(weight_decay=-0.5)])
+def test_loaded_settings_are_checked(bad):
+    """What the constructor refuses is refused in a state dictionary too, before anything has changed."""
+    opt = _with_state(AdamW(_params(), lr=1e-3))
+    held = {p: {n: t.clone() for n, t in st.items()} for p, st in opt.state.items()}
+    sd = _with_state(AdamW(_params(), lr=0.25)).state_dict()
+    sd["param_groups"][0].update(bad)
+    with pytest.raises(RuntimeError):
+        opt.load_state_dict(sd)
+    assert opt.param_groups[0]["lr"] == 1e-3 and opt.param_groups[0]["betas"] == (0.9, 0.999)
+    assert all(torch.equal(opt.state[p][n], t) for p, st in held.items() for n, t in st.items())

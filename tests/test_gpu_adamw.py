@@ -641,3 +641,19 @@ def test_a_step_marks_what_it_writes():
             p.grad = torch.ones(5, device="cuda")
             AdamW([p], lr=0.5, weight_decay=0.0, state_bits=bits).step()
         assert float((p + 0.5 / (1 + 1e-8)).abs().max()) <= 40 * E * 0.5     # the first step is lr g / (|g| + eps)
+
+
+def test_loaded_numbers_on_the_device_are_read():
+    """A state of torch's AdamW with its learning rate on the device: read once, when it is loaded; a step can be captured."""
+    from fsgs.optim import AdamW
+    params, grads = _make((300,), torch.float32, torch.float32)
+    params[0].grad = grads[0]
+    ref = torch.optim.AdamW(params, lr=torch.tensor(2.0 ** -7, device="cuda"), capturable=True)
+    ref.step()
+    opt = AdamW(params)
+    opt.load_state_dict(ref.state_dict())
+    assert type(opt.param_groups[0]["lr"]) is float and opt.param_groups[0]["lr"] == 2.0 ** -7
+    assert torch.is_tensor(ref.param_groups[0]["lr"])
+    before = _snapshot(opt, params)
+    opt.step()
+    _check_step(opt, before, params, grads)
