@@ -154,6 +154,15 @@ def grad_norm(tensors, max_norm=None):
     return _lib.host().norm(list(tensors), float("inf") if max_norm is None else float(max_norm))
 
 
+def _number(v):
+    """A setting as a number; a tensor on a device would make every step wait for it."""
+    if v.__class__ is float:
+        return v
+    _need(not (torch.is_tensor(v) and v.is_cuda),
+          "AdamW: lr, betas, eps and weight_decay are numbers on the host (a step would wait for the device to read them)")
+    return float(v)
+
+
 class _Plan:
     """The argument tables of a step for one list of parameters, and what the host extension compares them with: it reads
     every address, length and type of the parameters, gradients and states anew each step, and a plan is used only while
@@ -163,7 +172,7 @@ class _Plan:
         self.settings, self.form = self.current_settings(opt), self.current_form(opt)
         self.params, self.groups, found, kinds = [], [], [], {}
         for k, group in enumerate(opt.param_groups):
-            tail = (tuple(group["betas"]), group["eps"])
+            tail = self.settings[k][2:]
             for p in group["params"]:
                 g = p.grad
                 if g is None:
@@ -176,19 +185,20 @@ class _Plan:
                 self.groups.append(k)
         self.device = self.params[0].device
         self.launches, entries = [], [None] * len(found)
-        for (param_type, grad_type, _, betas, eps), rows in kinds.items():
+        for (param_type, grad_type, _, *numbers), rows in kinds.items():
             t = np.zeros(len(rows), _table_type)
             start = t.ctypes.data
-            self.launches.append((rows, t, (len(rows), start, param_type, grad_type, opt.state_bits, float(betas[0]),
-                                            float(betas[1]), float(eps))))
+            self.launches.append((rows, t, (len(rows), start, param_type, grad_type, opt.state_bits, *numbers)))
             for k, i in enumerate(rows):
                 entries[i] = found[i] + (start + k * _table_type.itemsize,)
-        self.rates(opt)
+        self.rates()
         self.handle = _lib.host().plan(entries, [l[2] for l in self.launches], opt.state_bits)
 
     @staticmethod
     def current_settings(opt):
-        return [(float(g["lr"]), float(g["weight_decay"]), *g["betas"], g["eps"]) for g in opt.param_groups]
+        """Learning rate, weight decay, both betas and eps of every group."""
+        return [(_number(g["lr"]), _number(g["weight_decay"]), *map(_number, g["betas"]), _number(g["eps"]))
+                for g in opt.param_groups]
 
     @staticmethod
     def current_form(opt):
@@ -203,13 +213,12 @@ class _Plan:
             if [s[2:] for s in now] != [s[2:] for s in self.settings]:
                 return False
             self.settings = now
-            self.rates(opt)
+            self.rates()
         return True
 
-    def rates(self, opt):
-        lr, wd = ([float(g[k]) for g in opt.param_groups] for k in ("lr", "weight_decay"))
+    def rates(self):
         for rows, table, _ in self.launches:
-            table["lr"], table["weight_decay"] = ([v[self.groups[i]] for i in rows] for v in (lr, wd))
+            table["lr"], table["weight_decay"] = ([self.settings[self.groups[i]][k] for i in rows] for k in (0, 1))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -258,10 +267,8 @@ class AdamW(torch.optim.Optimizer):
 
     @staticmethod
     def _check_group(g):
-        _need(not any(torch.is_tensor(v) and v.is_cuda for v in (g["lr"], g["weight_decay"], g["eps"], *g["betas"])),
-              "AdamW: lr, betas, eps and weight_decay are numbers on the host (a step would wait for the device to read them)")
-        _need(float(g["lr"]) >= 0 and g["eps"] >= 0 and g["weight_decay"] >= 0 and
-              all(0 <= b < 1 for b in g["betas"]), "AdamW: lr, eps, weight_decay >= 0 and 0 <= beta < 1")
+        _need(all(_number(g[k]) >= 0 for k in ("lr", "eps", "weight_decay")) and
+              all(0 <= _number(b) < 1 for b in g["betas"]), "AdamW: lr, eps, weight_decay >= 0 and 0 <= beta < 1")
         for p in g["params"]:
             _need(p.dtype in _TYPES and p.layout == torch.strided, "AdamW: dense float32, bfloat16 or float16 parameters")
 

@@ -657,3 +657,25 @@ def test_loaded_numbers_on_the_device_are_read():
     before = _snapshot(opt, params)
     opt.step()
     _check_step(opt, before, params, grads)
+
+
+def test_numbers_put_on_the_device_between_steps_are_refused():
+    from fsgs.optim import AdamW
+    params, grads = _make((300,), torch.float32, torch.float32)
+    params[0].grad = grads[0]
+    opt = AdamW(params, lr=1e-2)
+    group = opt.param_groups[0]
+    opt.step()
+    for key, bad, good in (("lr", torch.tensor(0.1, device="cuda"), 1e-3), ("weight_decay", torch.tensor(0.1, device="cuda"), 0.0),
+                           ("eps", torch.tensor(0.1, device="cuda"), torch.tensor(1e-6)),
+                           ("betas", (torch.tensor(0.5, device="cuda"), 0.9), (0, 0.9))):
+        group[key] = bad
+        with pytest.raises(RuntimeError, match="numbers on the host"):
+            opt.step()
+        group[key] = good
+    group["eps"] = float(group["eps"])
+    before = _snapshot(opt, params)
+    group["eps"] = torch.tensor(group["eps"], dtype=torch.float64)         # a tensor on the host is read at each step
+    opt.step()
+    group["eps"] = float(group["eps"])
+    _check_step(opt, before, params, grads)
