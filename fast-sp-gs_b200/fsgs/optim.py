@@ -323,6 +323,18 @@ class AdamW(torch.optim.Optimizer):
         without the master copy that this optimiser keeps, is refused, and so are groups of another rule (``amsgrad``,
         ``maximize``, a weight decay that is added to the gradient) and settings that the constructor refuses; numbers
         that lie on a device are read."""
+        loaded, before = {}, {p: st for p, st in self.state.items() if st}
+        # after the user's hooks, which may give another dictionary, and before those that want the loaded state
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, sd: self._take_states(sd, loaded, before)),
+                 self.register_load_state_dict_post_hook(lambda _: self._put_states(loaded, before), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
+
+    def _take_states(self, state_dict, loaded, before):
+        """Checks a state dictionary, moves its states into ``loaded`` and returns what is left for the base class."""
         for g in state_dict["param_groups"]:
             _need(not g.get("amsgrad") and not g.get("maximize") and
                   (g.get("decoupled_weight_decay", True) or not g.get("weight_decay")),
@@ -333,7 +345,6 @@ class AdamW(torch.optim.Optimizer):
         ids = [i for g in groups for i in g["params"]]
         own = [p for g in self.param_groups for p in g["params"]]
         _need(len(ids) == len(own), "AdamW: the loaded state has another number of parameters")
-        loaded = {}
         for i, p in zip(ids, own):
             st = state_dict["state"].get(i)
             if not st:
@@ -345,14 +356,14 @@ class AdamW(torch.optim.Optimizer):
                 _need(value.numel() == fresh.numel() and (value.dtype == fresh.dtype or name == "step"),
                       f"AdamW: the loaded {name} has another size or type")
                 loaded.setdefault(p, {})[name] = fresh.copy_(value.reshape(fresh.shape))
-        before = {p: self.state[p] for p in own if self.state.get(p)}
-        super().load_state_dict(dict(state_dict, state={}, param_groups=groups))
         for p in own:
-            st, new = before.get(p), loaded.get(p)
-            if st is not None and new is None:      # no state: as before the first step
-                new = {n: self._fresh(p, n) for n in self._names(p)}
-            if new is None:
-                continue
+            if p in before and p not in loaded:      # no state: as before the first step
+                loaded[p] = {n: self._fresh(p, n) for n in self._names(p)}
+        return dict(state_dict, state={}, param_groups=groups)
+
+    def _put_states(self, loaded, before):
+        for p, new in loaded.items():
+            st = before.get(p)
             if st is not None and set(st) == set(new) and all(st[n].shape == t.shape and st[n].dtype == t.dtype and
                                                               st[n].device == t.device for n, t in new.items()):
                 for n, t in new.items():   # into the tensors that are there: a captured step goes on using them

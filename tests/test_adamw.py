@@ -158,3 +158,36 @@ def test_loaded_settings_are_checked(bad):
         opt.load_state_dict(sd)
     assert opt.param_groups[0]["lr"] == 1e-3 and opt.param_groups[0]["betas"] == (0.9, 0.999)
     assert all(torch.equal(opt.state[p][n], t) for p, st in held.items() for n, t in st.items())
+
+
+def test_hooks_of_loading():
+    """A pre-hook sees the whole state dictionary and may return another one, a post-hook sees the loaded state; afterwards
+    the optimiser has the hooks that it had."""
+    src = _with_state(AdamW(_params(), lr=0.25))
+    opt, seen = AdamW(_params(), lr=1.0), []
+
+    def before(o, sd):
+        seen.append(len(sd["state"]))
+        sd["state"] = {k: dict(v, step=torch.tensor(7.0)) for k, v in sd["state"].items()}
+        sd["param_groups"] = [dict(g, lr=0.5) for g in sd["param_groups"]]
+        return sd
+
+    opt.register_load_state_dict_pre_hook(before)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append([float(o.state[p]["step"]) for p in o.param_groups[0]["params"]]))
+    for n in (1, 2):
+        given = src.state_dict()
+        opt.load_state_dict(given)
+        assert seen == [2, [7.0, 7.0]] * n and opt.param_groups[0]["lr"] == 0.5
+        assert given["param_groups"][0]["lr"] == 0.25
+        for p, q in zip(src.param_groups[0]["params"], opt.param_groups[0]["params"]):
+            assert torch.equal(src.state[p]["exp_avg"], opt.state[q]["exp_avg"])
+
+    def refuse(o, sd):
+        return dict(sd, state={k: {n: t for n, t in v.items() if n != "exp_avg"} for k, v in sd["state"].items()})
+
+    handle = opt.register_load_state_dict_pre_hook(refuse)
+    with pytest.raises(RuntimeError, match="exp_avg"):
+        opt.load_state_dict(src.state_dict())
+    handle.remove()
+    opt.load_state_dict(src.state_dict())
+    assert seen == [2, [7.0, 7.0]] * 2 + [2] + [2, [7.0, 7.0]]
