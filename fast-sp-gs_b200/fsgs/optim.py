@@ -397,7 +397,7 @@ class AdamW(torch.optim.Optimizer):
         """The body of ``step``, without hooks."""
         if gate is not None or grad_scale is not None:
             for t in (gate, grad_scale):
-                _need(t is None or (t.is_cuda and t.numel() == 1 and t.dtype == torch.float32),
+                _need(t is None or (torch.is_tensor(t) and t.is_cuda and t.numel() == 1 and t.dtype == torch.float32),
                       "AdamW: gate and grad_scale are one-element float32 tensors on the parameters' device")
             _need(grad_scale is None or self.max_grad_norm is None, "AdamW: grad_scale together with max_grad_norm")
         plan = self._plan

@@ -191,3 +191,12 @@ def test_hooks_of_loading():
     handle.remove()
     opt.load_state_dict(src.state_dict())
     assert seen == [2, [7.0, 7.0]] * 2 + [2] + [2, [7.0, 7.0]]
+
+
+@pytest.mark.parametrize("bad", [lambda: 0.0, 1.0, [1.0], "open"])
+def test_a_gate_that_is_no_tensor_is_refused(bad):
+    """A closure too: the step of this optimiser takes a gate in the first place."""
+    opt = AdamW(_params())
+    for call in (lambda: opt.step(bad), lambda: opt.step(gate=bad), lambda: opt.step(grad_scale=bad)):
+        with pytest.raises(RuntimeError, match="one-element float32 tensors"):
+            call()
