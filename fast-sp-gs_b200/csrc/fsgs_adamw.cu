@@ -65,6 +65,14 @@ struct Packed<float> {
   __device__ __forceinline__ void get(float *x) const {
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
   }
+  __device__ __forceinline__ unsigned bits() const {  // zero where all eight are (as below)
+    float x[8];
+    get(x);
+    unsigned r = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) r |= __float_as_uint(x[u]);
+    return r;
+  }
   static __device__ __forceinline__ void store(float *p, const float *x) {
     reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
     reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
@@ -79,6 +87,7 @@ struct Packed<__nv_bfloat16> {
 #pragma unroll
     for (int u = 0; u < 4; ++u) x[2 * u] = __uint_as_float(w[u] << 16), x[2 * u + 1] = __uint_as_float(w[u] & 0xffff0000u);
   }
+  __device__ __forceinline__ unsigned bits() const { return a.x | a.y | a.z | a.w; }
   static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float *x) {
     *reinterpret_cast<uint4 *>(p) = make_uint4(bits_of(__floats2bfloat162_rn(x[0], x[1])), bits_of(__floats2bfloat162_rn(x[2], x[3])),
                                                bits_of(__floats2bfloat162_rn(x[4], x[5])), bits_of(__floats2bfloat162_rn(x[6], x[7])));
@@ -96,6 +105,7 @@ struct Packed<__half> {
       x[2 * u] = f.x, x[2 * u + 1] = f.y;
     }
   }
+  __device__ __forceinline__ unsigned bits() const { return a.x | a.y | a.z | a.w; }
   static __device__ __forceinline__ void store(__half *p, const float *x) {
     *reinterpret_cast<uint4 *>(p) = make_uint4(bits_of(__floats2half2_rn(x[0], x[1])), bits_of(__floats2half2_rn(x[2], x[3])),
                                                bits_of(__floats2half2_rn(x[4], x[5])), bits_of(__floats2half2_rn(x[6], x[7])));
@@ -442,8 +452,8 @@ static int adamw_pick(bool eight, bool master, const AdamWCall &c) {
 // the norm of all gradients
 // ------------------------------------------------------------------------------------------------
 
-// One pass over all gradients, bound by its read: 464 MB of float32 in 71 us (6.6 TB/s), 232 MB of bf16 in 50 us; a small
-// call is two launches, 5 us.  Every thread block adds its share in double and leaves it in a slot of its own; a block of a
+// One pass over all gradients, bound by its read: 464 MB of float32 in 70 us (6.6 TB/s), 232 MB of bf16 in 39 us call after
+// call (part of them from L2), 50 us in front of a step; a small call is two launches, 4 us.  Every thread block adds its share in double and leaves it in a slot of its own; a block of a
 // second launch adds the slots.  No counter, nothing to prepare: a workspace can be used again as soon as a call is done.
 struct NormEntry {
   const void *data;
@@ -460,12 +470,14 @@ struct NormTable {
 constexpr int kNormPart = kOptWarps * kOptBlock;   // elements of one pass of a thread block
 constexpr int kNormChunk = 4 * kNormPart;
 constexpr int kNormSlots = FSGS_GRAD_NORM_SLOTS;
+constexpr double kLost = 1.0 / (1ull << 56) / (1ull << 56);  // 2^-112
 
 // Sum of the squares of this thread's elements of a chunk.  Eight squares are added in float32 (two sums of four) and the
-// eights in double: the float32 part rounds each eight by 5 x 2^-24 at most, and no sum of squares leaves the range of double unless a
-// single eight leaves that of float32 (|g| > 6e18: the norm comes out infinite and the step is dropped).
+// eights in double: the float32 part rounds each eight by 5 x 2^-24 at most.  An eight overflows above |g| = 6e18, and what
+// its squares lose below 2^-126, 2^-150 each, shows where nearly all gradients are below 1e-18: the kernel looks at its sum
+// for both.  `bits`: all elements' bits, zero where the gradients are.
 template <typename T>
-__device__ __forceinline__ double chunk_squares(const T *p, bool vec, long long left, int warp, int lane) {
+__device__ __forceinline__ double chunk_squares(const T *p, bool vec, long long left, int warp, int lane, unsigned &bits) {
   constexpr int parts = kNormChunk / kNormPart;
   auto squares = [](const float *x) {
     Two q = both(0.0f);
@@ -478,12 +490,12 @@ __device__ __forceinline__ double chunk_squares(const T *p, bool vec, long long 
   double sum = 0.0;
   float x[8];
   p += warp * kOptBlock + 8 * lane;
-  if (vec && left >= kNormChunk) {  // all loads out before the first is used
+  if (vec && left >= kNormChunk) {  // as many loads under way as the registers take
     Packed<T> w[parts];
 #pragma unroll
     for (int j = 0; j < parts; ++j) w[j].load(p + j * kNormPart);
 #pragma unroll
-    for (int j = 0; j < parts; ++j) w[j].get(x), sum += squares(x);
+    for (int j = 0; j < parts; ++j) w[j].get(x), bits |= w[j].bits(), sum += squares(x);
   } else {
     left -= warp * kOptBlock + 8 * lane;
 #pragma unroll 1
@@ -495,9 +507,30 @@ __device__ __forceinline__ double chunk_squares(const T *p, bool vec, long long 
       } else {
         load_some(p, left, x);
       }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) bits |= __float_as_uint(x[u]);
       sum += squares(x);
     }
   }
+  return sum;
+}
+
+// The same over a warp's elements of a chunk, every square in double, whose range holds that of every float32.
+template <typename T>
+__device__ __noinline__ double warp_squares(const T *p, long long left, int warp, int lane) {
+  double sum = 0.0;
+#pragma unroll 1
+  for (int e = warp * kOptBlock; e < kNormChunk; e += kNormPart)
+#pragma unroll 1
+    for (int i = e + lane; i < e + kOptBlock && i < left; i += 32) {
+      const double x = (double) to_f32(p[i]);
+      sum += x * x;
+    }
+  return sum;
+}
+
+__device__ __forceinline__ double warp_total(double sum) {
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
 
@@ -507,16 +540,32 @@ __global__ void __launch_bounds__(kOptThreads) grad_norm_kernel(const __grid_con
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int total = a.chunk_start[a.n];
   double sum = 0.0;
+  unsigned bits = 0;
   for (int chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
     const int k = tensor_of(a.chunk_start, a.n, chunk);
     const long long e0 = (long long) (chunk - a.chunk_start[k]) * kNormChunk;
     const long long left = a.t[k].numel - e0;
     const bool vec = a.vec[k] != 0;
-    if (a.type[k] == FSGS_F32) sum += chunk_squares((const float *) a.t[k].data + e0, vec, left, warp, lane);
-    else if (a.type[k] == FSGS_BF16) sum += chunk_squares((const __nv_bfloat16 *) a.t[k].data + e0, vec, left, warp, lane);
-    else sum += chunk_squares((const __half *) a.t[k].data + e0, vec, left, warp, lane);
+    if (a.type[k] == FSGS_F32) sum += chunk_squares((const float *) a.t[k].data + e0, vec, left, warp, lane, bits);
+    else if (a.type[k] == FSGS_BF16) sum += chunk_squares((const __nv_bfloat16 *) a.t[k].data + e0, vec, left, warp, lane, bits);
+    else sum += chunk_squares((const __half *) a.t[k].data + e0, vec, left, warp, lane, bits);
   }
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  sum = warp_total(sum);
+  // a warp's 1024 elements of a chunk lose 2^-140 at most; again in double where that may be above 2^-28 of the sum, and
+  // where the sum has overflowed (or holds a NaN, which stays)
+  const double least = kLost * (double) ((total - 1 - (int) blockIdx.x) / (int) gridDim.x + 1);
+  if (__any_sync(0xffffffffu, bits != 0) && !(sum >= least && sum < INFINITY)) {
+    sum = 0.0;
+    for (int chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
+      const int k = tensor_of(a.chunk_start, a.n, chunk);
+      const long long e0 = (long long) (chunk - a.chunk_start[k]) * kNormChunk;
+      const long long left = a.t[k].numel - e0;
+      if (a.type[k] == FSGS_F32) sum += warp_squares((const float *) a.t[k].data + e0, left, warp, lane);
+      else if (a.type[k] == FSGS_BF16) sum += warp_squares((const __nv_bfloat16 *) a.t[k].data + e0, left, warp, lane);
+      else sum += warp_squares((const __half *) a.t[k].data + e0, left, warp, lane);
+    }
+    sum = warp_total(sum);
+  }
   if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
   if (threadIdx.x != 0) return;

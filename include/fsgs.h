@@ -149,7 +149,8 @@ int fsgs_adamw_multi(int n_tensors, const fsgs_adamw_tensor *tensors /* host */,
 size_t fsgs_adamw_workspace_bytes(void);
 
 /* out[0] = sqrt(sum of the squares of all elements of all tensors), out[1] = min(1, max_norm / (out[0] + 1e-6)), or 0
- * where the norm is not finite: the grad_scale of fsgs_adamw_multi.  Summed in a fixed order: the same gradients give
+ * where the norm is not finite: the grad_scale of fsgs_adamw_multi.  Right over the whole range of the types, where
+ * squares leave that of float32 too.  Summed in a fixed order: the same gradients give
  * the same bits.  workspace: 16-byte aligned, needs no preparation; calls that may run at the same time need workspaces
  * of their own. */
 typedef struct fsgs_norm_tensor {

@@ -679,3 +679,39 @@ def test_numbers_put_on_the_device_between_steps_are_refused():
     opt.step()
     group["eps"] = float(group["eps"])
     _check_step(opt, before, params, grads)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_norm_over_the_whole_range_of_the_type(dtype):
+    """Gradients whose squares leave the range of float32 on either side, alone, in all tensors, and beside zeros and beside
+    others: 4 e relative on the norm and 1 e for its own rounding, half a denormal where it is one.  The factor: 4 e more,
+    or half a denormal, or (above 2^126) the inverse's half denormal of 2^-150 times the limit."""
+    from fsgs.optim import grad_norm
+    gen = torch.Generator().manual_seed(4)
+    lo, hi = (2.0 ** -24, 6e4) if dtype == torch.float16 else (1e-45, 3e38) if dtype == torch.float32 else (1e-40, 3e38)
+    sizes = (1, 7, 300, 8192, 50_001)
+    for amount in (lo, 1e-38, 1e-30, 1e-23, 1e-20, 1e-18, 1e-16, 1.0, 1e15, 6e18, 1e19, 1e25, 1e36, hi):
+        if not lo <= amount <= hi:
+            continue
+        for others in (None, 0.0, 1e-25, 1e-12):
+            ts = []
+            for k, n in enumerate(sizes):
+                x = (torch.rand(n + 1, generator=gen) + 0.5).double() * amount
+                if others is not None:
+                    x = torch.where(torch.rand(n + 1, generator=gen) < 1e-3, x, others)
+                ts.append(x.clamp(max=float(torch.finfo(dtype).max)).to(dtype).cuda()[k % 2:n + k % 2])
+            want = math.sqrt(sum(float((t.double() ** 2).sum()) for t in ts))
+            norm, factor = (float(t) for t in grad_norm(ts, max_norm=0.25))
+            if want > 3.4e38:
+                assert norm == math.inf and factor == 0.0
+                continue
+            assert abs(norm - want) <= 5 * E * want + 2.0 ** -150, (amount, others, norm, want)
+            limit = min(1.0, 0.25 / (want + 1e-6))
+            assert abs(factor - limit) <= 9 * E * limit + 2.0 ** -150 * 1.25, (amount, others, factor, limit)
+            assert float(grad_norm([t for t in ts] * 2, max_norm=0.25)[0]) > norm or want == 0.0
+    assert float(grad_norm([torch.zeros(70_000, dtype=dtype, device="cuda"), -torch.zeros(9, dtype=dtype, device="cuda")])[0]) == 0.0
+    for bad in (math.inf, -math.inf, math.nan):
+        t = torch.full((9000,), 1e-30 if dtype != torch.float16 else 1e-7, dtype=dtype, device="cuda")
+        t[7777] = bad
+        norm, factor = grad_norm([t], max_norm=1.0)
+        assert not math.isfinite(float(norm)) and float(factor) == 0.0
