@@ -381,3 +381,19 @@ def test_the_gradient_added_to_counts_as_modified():
         plain = torch.zeros(50, 2, device="cuda")
         balance_value_and_grad(w, idx, 5, grad=plain)
     assert torch.equal(plain, into)
+
+
+@pytest.mark.parametrize("N", [1, 1024])
+def test_the_loss_of_terms_that_round_the_same_way(N):
+    """A term of 1 and seven of a little over half a unit behind it, all shares a power of two: added one after another in
+    float32 every addition rounds up, 7 e in all.  Asked for are 3 e of the sum (a share, a product, one addition) and e for
+    the loss itself."""
+    from fsgs.loss import balance_loss, balance_value_and_grad
+    for order in (slice(None), slice(None, None, -1)):
+        w = torch.tensor([1.0] + [1.01 * E] * 7).expand(N, 8).contiguous()
+        idx = torch.arange(8).expand(N, 8).contiguous()
+        if order.step:
+            w = w.flip(1)
+        want = float(w.double().sum()) / N
+        for loss in (balance_value_and_grad(w.cuda(), idx.cuda(), 8)[0], balance_loss(w.cuda(), idx.cuda(), 8)[0]):
+            assert abs(float(loss) - want) <= 4 * E * want
