@@ -277,10 +277,21 @@ void written(const Plan &plan) {
   }
 }
 
-// step(plan, groups, state, max_norm, (norm workspace, its bytes, norm out, workspace, its bytes), grad_scale, gate): on the
-// parameters' device and its current stream; addresses as integers, 0 for none; max_norm None: no norm
+// The optimiser's own tensors, [(tensor, stream that it was made on)]: the allocator keeps them until this stream is done
+// with them, should the optimiser be let go of meanwhile.
+void keep_for(const c10::cuda::CUDAStream &stream, PyObject *own) {
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(own); ++i) {
+    PyObject *pair = PyTuple_GET_ITEM(own, i);
+    if ((cudaStream_t) PyLong_AsVoidPtr(PyTuple_GET_ITEM(pair, 1)) != stream.stream())
+      THPVariable_Unpack(PyTuple_GET_ITEM(pair, 0)).record_stream(stream.unwrap());
+  }
+}
+
+// step(plan, groups, state, max_norm, (norm workspace, its bytes, norm out, workspace, its bytes), own, grad_scale, gate): on
+// the parameters' device and its current stream; addresses as integers, 0 for none; max_norm None: no norm
 PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 7 || !PyList_Check(args[1]) || !PyDict_Check(args[2]) || !PyTuple_Check(args[4]) || PyTuple_GET_SIZE(args[4]) != 5)
+  if (n != 8 || !PyList_Check(args[1]) || !PyDict_Check(args[2]) || !PyTuple_Check(args[4]) || PyTuple_GET_SIZE(args[4]) != 5 ||
+      !PyTuple_Check(args[5]))
     return refuse("fsgs_host.step: wrong arguments");
   Plan *plan = (Plan *) PyCapsule_GetPointer(args[0], "fsgs.plan");
   if (!plan) return nullptr;
@@ -290,15 +301,17 @@ PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   void *norm_ws = (void *) word(0), *ws = (void *) word(3);
   const size_t norm_bytes = word(1), bytes = word(4);
   float *norm_out = clip ? (float *) word(2) : nullptr;
-  const float *grad_scale = (const float *) (uintptr_t) PyLong_AsUnsignedLongLong(args[5]);
-  const float *gate = (const float *) (uintptr_t) PyLong_AsUnsignedLongLong(args[6]);
+  const float *grad_scale = (const float *) (uintptr_t) PyLong_AsUnsignedLongLong(args[6]);
+  const float *gate = (const float *) (uintptr_t) PyLong_AsUnsignedLongLong(args[7]);
   if (PyErr_Occurred()) return nullptr;
   try {
     int rc = walk(*plan, args[1], args[2]);
     if (rc != 0) return PyLong_FromLong(rc);
     written(*plan);
     const c10::cuda::CUDAGuard guard(plan->device);
-    const auto stream = (fsgs_stream_t) c10::cuda::getCurrentCUDAStream(plan->device.index()).stream();
+    const auto current = c10::cuda::getCurrentCUDAStream(plan->device.index());
+    const auto stream = (fsgs_stream_t) current.stream();
+    keep_for(current, args[5]);
     if (norm_out) {
       rc = lib.norm((int) plan->norm.size(), plan->norm.data(), max_norm, norm_ws, norm_bytes, norm_out, stream);
       grad_scale = norm_out + 1;

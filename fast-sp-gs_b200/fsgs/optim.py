@@ -439,17 +439,20 @@ class AdamW(torch.optim.Optimizer):
         if gate is not None:
             _need(gate.device == device, "AdamW: gate and grad_scale are on the parameters' device")
             where = gate.data_ptr()
-        return _lib.host().step(plan.handle, self.param_groups, self.state, clip, self._words, scale, where)
+        return _lib.host().step(plan.handle, self.param_groups, self.state, clip, self._words, self._own, scale, where)
 
     def _workspaces(self, device):
         """Created once and never replaced on the same device: a captured step goes on using them."""
         _need(not torch.cuda.is_current_stream_capturing(),
               "AdamW: take a step, or call init_state(), before a step is captured")
         space = lambda n: torch.empty(int(n), dtype=torch.uint8, device=device)  # noqa: E731
+        stream = torch.cuda.current_stream(device).cuda_stream
         if self._work is None or self._work[0] != device:
             self._work, self._norm = (device, space(lib().fsgs_adamw_workspace_bytes())), None
+            self._own = ((self._work[1], stream),)
         if self.max_grad_norm is not None and self._norm is None:
             self._norm = (torch.zeros(2, device=device), space(lib().fsgs_grad_norm_workspace_bytes()))
+            self._own += tuple((t, stream) for t in self._norm)
         work, norm = self._work[1], self._norm
         self._words = (norm[1].data_ptr(), norm[1].numel(), norm[0].data_ptr()) if norm is not None else (0, 0, 0)
         self._words += (work.data_ptr(), work.numel())

@@ -715,3 +715,32 @@ def test_norm_over_the_whole_range_of_the_type(dtype):
         t[7777] = bad
         norm, factor = grad_norm([t], max_norm=1.0)
         assert not math.isfinite(float(norm)) and float(factor) == 0.0
+
+
+def test_an_optimiser_let_go_of_while_its_step_runs():
+    """Made on one stream, stepped on another that is busy, dropped: the memory that it brought along is not handed out again
+    before that step is done."""
+    import gc
+    from fsgs.optim import AdamW
+    params, grads = _make((700,), torch.float32, torch.float32)
+    params[0].grad = grads[0]
+    opt = AdamW(params, max_grad_norm=1.0)
+    opt.step()
+    torch.cuda.synchronize()
+    own = [opt._work[1], *opt._norm]
+    places, sizes = {t.untyped_storage().data_ptr() for t in own}, [t.untyped_storage().nbytes() for t in own]
+    state = dict(opt.state)                        # the parameters' states are the caller's here
+    stream = torch.cuda.Stream()
+    busy, done = torch.cuda.Event(), torch.cuda.Event()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(1_000_000_000)           # half a second
+        busy.record()
+        opt.step()
+        done.record()
+    del own, opt
+    gc.collect()
+    handed_out = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(30)]
+    waiting = not busy.query()
+    assert waiting and not places & {t.data_ptr() for t in handed_out}
+    done.synchronize()
+    assert float(state[params[0]]["step"]) == 2
