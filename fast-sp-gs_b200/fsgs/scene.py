@@ -290,7 +290,11 @@ class DynamicScene:
         if self.dense_optimizer is not None:
             # a view whose tile lists overflowed (on any rank) left -inf in the mask: the masked Adam above passed no
             # row, and the dense parameters' Adam is gated by the same element (mask values are >= 0 otherwise)
-            self.dense_optimizer.step_gated(b.extra[:1] + 1.0)
+            gate = b.extra[:1] + 1.0
+            if isinstance(self.dense_optimizer, AdamW):
+                self.dense_optimizer.step(gate)   # looks for hooks itself: no wrapper to go round
+            else:
+                self.dense_optimizer.step_gated(gate)
         self._drop_grads()
         return eng
 

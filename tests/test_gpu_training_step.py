@@ -101,3 +101,20 @@ def test_balance_needs_kernel_weights():
     surf = wl.surfels(100, seed=5, log_scale_mean=-3.2)
     with pytest.raises(ValueError):
         DynamicScene(surf, wl.superpoints(surf["means"], M=8, seed=1)["centres"], K=2, device="cuda", balance=1.0)
+
+
+def test_hooks_and_schedules_of_the_dense_optimiser():
+    """What a user hangs on the scene's AdamW runs with its steps: step hooks, and a schedule that counts them."""
+    import warnings
+    scene, _ = _scene(adamw=dict(lr=1e-3))
+    opt, seen = scene.dense_optimizer, []
+    opt.register_step_pre_hook(lambda o, args, kwargs: seen.append("pre"))
+    opt.register_step_post_hook(lambda o, args, kwargs: seen.append("post"))
+    schedule = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.5)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")             # a schedule stepped before its optimiser warns
+        for k in range(2):
+            scene.train_views([], (W, H))
+            schedule.step()
+            assert seen == ["pre", "post"] * (k + 1) and opt.param_groups[0]["lr"] == 1e-3 * 0.5 ** (k + 1)
+    assert float(opt.state[scene.sp_radius]["step"]) == 2
