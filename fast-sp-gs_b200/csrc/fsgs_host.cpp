@@ -11,6 +11,8 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -98,6 +100,12 @@ void free_plan(PyObject *capsule) {
 
 PyObject *refuse(const char *what) {
   PyErr_SetString(PyExc_RuntimeError, what);
+  return nullptr;
+}
+
+// The exception that is being handled, as the Python error that torch's own calls raise for it (out of memory among them).
+PyObject *failed() {
+  torch::translate_exception_to_python(std::current_exception());
   return nullptr;
 }
 
@@ -198,9 +206,9 @@ PyObject *make_plan(PyObject *, PyObject *args) {
     try {
       if (i == 0 && THPVariable_Check(param)) plan->device = THPVariable_Unpack(param).device();
       plan->entries.push_back(entry_of(param, group, state, master, bits, (fsgs_adamw_tensor *) row, plan->device));
-    } catch (const std::exception &e) {
+    } catch (...) {
       Py_DECREF(capsule);
-      return refuse(e.what());
+      return failed();
     }
     const Entry &e = plan->entries.back();
     plan->place.emplace(param, plan->entries.size() - 1);
@@ -208,9 +216,9 @@ PyObject *make_plan(PyObject *, PyObject *args) {
   }
   try {
     need_apart(plan->entries);
-  } catch (const std::exception &e) {
+  } catch (...) {
     Py_DECREF(capsule);
-    return refuse(e.what());
+    return failed();
   }
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(launches); ++i) {
     Launch l;
@@ -321,8 +329,8 @@ PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t n) {
       rc = lib.adamw(l.n, l.table, l.param_type, l.grad_type, l.bits, l.b1, l.b2, l.eps, grad_scale, gate, ws, bytes, stream);
     }
     return PyLong_FromLong(rc);
-  } catch (const std::exception &e) {
-    return refuse(e.what());
+  } catch (...) {
+    return failed();
   }
 }
 
@@ -371,8 +379,8 @@ PyObject *norm_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const int rc = lib.norm((int) count, table.data(), max_norm, ws.data_ptr(), (size_t) bytes, out.data_ptr<float>(), stream_of(out));
     need(rc == 0, "fsgs_grad_norm", std::string(lib.status_string(rc)) + " (status " + std::to_string(rc) + ")");
     return tuple_of({out.select(0, 0), out.select(0, 1)});
-  } catch (const std::exception &e) {
-    return refuse(e.what());
+  } catch (...) {
+    return failed();
   }
 }
 
@@ -566,8 +574,8 @@ PyObject *balance_pairs(PyObject *, PyObject *const *args, Py_ssize_t n) {
     pairs(idx.size(0), idx.size(1), c, w.data_ptr<float>(), weight, nullptr, loss.data_ptr<float>(), grad.data_ptr<float>(), add);
     if (add) written(grad);
     return tuple_of({loss, grad, c.counts.narrow(0, 0, M)});
-  } catch (const std::exception &e) {
-    return refuse(e.what());
+  } catch (...) {
+    return failed();
   }
 }
 
@@ -594,8 +602,8 @@ PyObject *balance_table(PyObject *, PyObject *const *args, Py_ssize_t n) {
     Tensor grad = at::empty(t.sizes(), t.options().requires_grad(false));
     table_pass(t, type, m, c, weight, nullptr, loss.data_ptr<float>(), grad.data_ptr());
     return tuple_of({loss, grad, c.counts.narrow(0, 0, t.size(1))});
-  } catch (const std::exception &e) {
-    return refuse(e.what());
+  } catch (...) {
+    return failed();
   }
 }
 

@@ -397,3 +397,22 @@ def test_the_loss_of_terms_that_round_the_same_way(N):
         want = float(w.double().sum()) / N
         for loss in (balance_value_and_grad(w.cuda(), idx.cuda(), 8)[0], balance_loss(w.cuda(), idx.cuda(), 8)[0]):
             assert abs(float(loss) - want) <= 4 * E * want
+
+
+def test_running_out_of_memory_is_torchs_error():
+    """Seen as ``torch.cuda.OutOfMemoryError`` by who catches it to try a smaller call, and the next call works."""
+    from fsgs.loss import balance_loss, balance_value_and_grad, table_balance_loss, table_balance_value_and_grad
+    from fsgs.optim import grad_norm
+    one = torch.zeros(1, 1, device="cuda")
+    w, idx = one.expand(2 ** 27, 8), one.long().expand(2 ** 27, 8)       # 4 and 8 GB where they are laid out
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction(2 ** 30 / total)
+    try:
+        for call in (lambda: balance_value_and_grad(w, idx, 3), lambda: balance_loss(w.detach().requires_grad_(), idx, 3),
+                     lambda: table_balance_loss(w, idx), lambda: table_balance_value_and_grad(w, idx), lambda: grad_norm([w])):
+            with pytest.raises(torch.cuda.OutOfMemoryError):
+                call()
+        assert float(balance_value_and_grad(w[:4].contiguous() + 1, idx[:4].contiguous(), 1)[0]) == 8.0
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
