@@ -10,7 +10,9 @@
 // second moment of a block spans the square of its gradients' range.  A positive s never rounds to zero (it takes the
 // smallest value): an element whose s were lost while its m survived would step by m / eps.  The scale is a float32 and
 // not a power of two: moments that shrink or grow together keep their 8-bit values and move the scale, where a scale
-// in powers of two would round b2 = 0.999 back to where it came from for ever.
+// in powers of two would round b2 = 0.999 back to where it came from for ever.  What moves against its block does get rounded
+// back: a byte changes only where sqrt(b2 + (1 - b2) (g/s)^2) leaves 1 by half a step of the format, h = 1/32 to 1/16, so s
+// stays while |g| < s sqrt(((1 + h)^2 - b2) / (1 - b2)), 8 to 11 s for b2 = 0.999, and never falls.
 //
 // The update itself is done in float32 with the roundings of the written formula, one per operation, no contraction of
 // the moments' sums: a moment next to a border between two 8-bit values then falls on the side on which the formula

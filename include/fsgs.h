@@ -115,7 +115,9 @@ int fsgs_adam_masked_multi_fmask(int n_tensors, const fsgs_adam_tensor *tensors 
  * with one scale per FSGS_ADAMW_BLOCK consecutive elements (exp_avg_scale / exp_avg_sq_scale,
  * [ceil(numel / FSGS_ADAMW_BLOCK)]): value = byte * scale, scale = largest magnitude of the block / 448; a positive
  * sqrt(v) is held as no less than the smallest positive byte; a block whose largest magnitude is below 2^-110 is held
- * as zeros.  A gradient that is not finite spoils its element (32 bits) or its block (8 bits).
+ * as zeros.  Rounding is to nearest: a value that a step moves by less than half a step of the format keeps its byte, and
+ * changes with its block's scale alone (b2 = 0.999: sqrt(v) does not fall, and rises where |g'| is over 8 - 11 times it).
+ * A gradient that is not finite spoils its element (32 bits) or its block (8 bits).
  * param_type: FSGS_F32, FSGS_BF16 or FSGS_F16; grad_type: FSGS_F32 or the same as param_type.  master (16-bit
  * parameters; for all tensors of a call or for none): the float32 parameter that is updated, param receives it rounded.
  * grad_scale (device, optional): c; gate (device, optional).  A call with *gate <= 0, or with *grad_scale <= 0 or not

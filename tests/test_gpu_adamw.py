@@ -744,3 +744,63 @@ def test_an_optimiser_let_go_of_while_its_step_runs():
     assert waiting and not places & {t.data_ptr() for t in handed_out}
     done.synchronize()
     assert float(state[params[0]]["step"]) == 2
+
+
+def test_eight_bit_second_moments_over_many_steps():
+    """Constant gradients per element beside a twin with 32 bits, the block's largest element holding its own.  A value
+    (8 + k) 2^j of the format has half a step of h = 1 / (2 (8 + k)) above it (1 / (2 k) where it is k smallest steps), so
+    s = sqrt(v) rises as long as sqrt(b2 + (1 - b2) (g / s)^2) >= 1 + h and rests at
+    g / s < sqrt(((1 + h)^2 - b2) / (1 - b2)); it never falls, as sqrt(b2) = 0.9995 is within half a step of 1; and when the
+    largest element grows, all grow with it (a step takes 0.8 % of their share at most, less than 1/32).  Float32 adds 2e-5."""
+    from fsgs.optim import AdamW
+    b2, lr = 0.999, 1e-3
+    first = torch.tensor([0.9 * 2.0 ** -(i % 17) * (1 - (i // 17) / 40) for i in range(B)], device="cuda")
+    first[0] = 1.0
+    params = [torch.nn.Parameter(torch.zeros(B, device="cuda")) for _ in range(2)]
+    eight, whole = opts = [AdamW([p], lr=lr, betas=(0.9, b2), weight_decay=0.0, eps=1e-12, state_bits=bits)
+                           for p, bits in zip(params, (8, 32))]
+
+    def run(g, steps):
+        before = [p.detach().clone() for p in params]
+        for _ in range(steps):
+            before = [p.detach().clone() for p in params]
+            for p, o in zip(params, opts):
+                p.grad = g
+                o.step()
+        st = eight.state[params[0]]
+        held = (st["exp_avg_sq_root"].double() * st["exp_avg_sq_root_scale"].double())
+        return (held, whole.state[params[1]]["exp_avg_sq"].double().sqrt(), st["exp_avg_sq_root"].double(),
+                [(b - p.detach()).double() for b, p in zip(before, params)])
+
+    def half_step(code):
+        low = 2.0 ** -6                                    # the smallest normal value; steps of 2^-9 below it
+        _, e = torch.frexp(code)
+        return torch.where(code >= low, torch.ldexp(torch.ones_like(code), e - 5), 2.0 ** -10) / code
+
+    held, true, codes, _ = run(first, 50)
+    fine = codes >= 2.0 ** -6
+    assert bool(fine.any()) and bool((~fine).any())
+    off = (held / true - 1).abs()
+    assert float(off[fine].max()) <= 1 / 16 + 1e-3 and float(off.max()) <= 1.0 + 1e-3
+    # gradients that vanish: the bytes stay, where 32 bits go down to 0.999^1500
+    gone = first.clone()
+    gone[1:] = 0
+    held, true, now, _ = run(gone, 3000)
+    assert torch.equal(now, codes) and float((held / true)[1:].min()) > 3
+    # gradients that grow thirty times
+    grown = (first * 30).clamp(max=0.9)
+    grown[0] = 1.0
+    held, true, codes, moved = run(grown, 400)
+    bound = (((1 + half_step(codes)) ** 2 - b2) / (1 - b2)).sqrt()
+    assert float(bound.max()) < 35.4 and float(bound[codes >= 2.0 ** -6].max()) < 11.41
+    ratio = grown.double() / held
+    assert bool((ratio <= bound * (1 + 1e-3)).all()) and float(ratio.max()) > 4
+    # the step: m = g, held as a value of the format, 1/16 off, and bias corrections that have gone to 1 (0.999^3450 = 0.03)
+    assert bool((moved[0] <= lr * bound * (1 + 1 / 16) * 1.03).all()) and float(moved[1][1:].max()) < lr * 2
+    # the largest grows four times: the others' bytes stay and their values go with it
+    loud = grown.clone()
+    loud[0] = 4.0
+    after, true, now, _ = run(loud, 3000)
+    assert torch.equal(now, codes)
+    share = after / held
+    assert float(share.min()) > 3.8 and float(share.max()) < 4.1
