@@ -99,13 +99,16 @@ def balance_value_and_grad(weights, idx, M, mask=None, weight=1.0, grad=None):
 
 
 def table_balance_loss(table, idx, mask=None):
-    """``(loss, counts)`` for a learned association ``table`` [N,M] (float32, bfloat16 or float16 logits; the ``"table"``
-    weighting of ``lbs_weights``) and the superpoints ``idx`` [N,K] int64 that each Gaussian is bound to:
+    """``(loss, counts)`` for a ``table`` [N,M] (float32, bfloat16 or float16 logits) of how each Gaussian is spread over all
+    ``M`` superpoints, and the superpoints ``idx`` [N,K] int64 that it is bound to:
 
         ``loss = M * sum_m (counts_m / sum(counts)) * mean over the Gaussians of softmax(table)_m``
 
     ``balance_loss`` with the probabilities of all superpoints in the place of the K blend weights, differentiable in
-    ``table`` (gradient in its type).  A row of nothing but -infinity adds nothing.  ``mask``, indices outside 0 .. M-1
+    ``table`` (gradient in its type).  It acts on the softmax over the whole row, so it also falls where probability goes to
+    the M - K superpoints that a Gaussian is not bound to.  For the ``"table"`` weighting of ``lbs_weights``, a softmax over
+    the K gathered entries, the balance of what is blended is ``balance_loss(lbs_weights(d2, idx, "table", table=table),
+    idx, M)``, which reaches those entries alone.  A row of nothing but -infinity adds nothing.  ``mask``, indices outside 0 .. M-1
     and ``counts`` as in ``balance_loss``; a captured backward pass too.  The gradient of a table
     of N rows is of the order of a probability times M / N: below 6e-8 a float16 table loses it, so scale the loss."""
     return host().balance_table(table, idx, mask, 1.0, True)

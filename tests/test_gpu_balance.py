@@ -416,3 +416,32 @@ def test_running_out_of_memory_is_torchs_error():
         assert float(balance_value_and_grad(w[:4].contiguous() + 1, idx[:4].contiguous(), 1)[0]) == 8.0
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
+
+
+def test_balance_of_the_table_weighting():
+    """``balance_loss`` on the weights that ``lbs_weights`` blends from a table: its gradient reaches the K entries of each
+    row that are read, and no other; ``table_balance_loss`` acts on the whole row.  A weight is a softmax in float32 of
+    values within 8 of each other (20 e), its adjoint two products and a difference of terms below p |up| (16 e more)."""
+    from fsgs.loss import balance_loss, table_balance_loss
+    from fsgs.scene import lbs_weights
+    gen = torch.Generator().manual_seed(12)
+    N, K, M = 400, 3, 30
+    idx = torch.rand(N, M, generator=gen).argsort(dim=1)[:, :K].contiguous()
+    table = torch.randn(N, M, generator=gen)
+    leaf = table.double().requires_grad_()
+    w = leaf.gather(1, idx).softmax(dim=1)
+    c = torch.bincount(idx.reshape(-1), minlength=M).double()
+    up = M * c[idx] / (N * K * N)
+    (w * up).sum().backward()
+    own = table.cuda().requires_grad_()
+    loss, counts = balance_loss(lbs_weights(None, idx.cuda(), "table", table=own), idx.cuda(), M)
+    loss.backward()
+    want = float((w * up).sum())
+    assert torch.equal(counts.cpu().double(), c) and abs(float(loss) - want) <= 24 * E * want
+    room = torch.zeros(N, M, dtype=torch.float64).scatter_(1, idx, (w * up).detach().sum(dim=1, keepdim=True).expand(N, K))
+    assert bool(((own.grad.cpu().double() - leaf.grad).abs() <= 36 * E * room).all())
+    # what no weight reads changes the loss over the whole row only
+    other = table.clone().scatter_(1, idx, -math.inf)
+    moved = torch.where(other == -math.inf, table, other + 3.0).cuda()
+    assert torch.equal(balance_loss(lbs_weights(None, idx.cuda(), "table", table=moved), idx.cuda(), M)[0], loss.detach())
+    assert not torch.equal(table_balance_loss(moved, idx.cuda())[0], table_balance_loss(own, idx.cuda())[0].detach())
