@@ -143,6 +143,13 @@ class DynamicScene:
             self.motion_buf = dict(sp_q=z(4), sp_t=z(3), sp_dr=z(4), sp_ds=z(2))
         return self.bucket
 
+    def _add_balance(self, world):
+        """Adds the balance term's gradient to that of the blend weights.  The ranks' gradients are summed: each adds its
+        part of the one term."""
+        loss, _, self.superpoint_counts = balance_value_and_grad(
+            self.knn_w, self.knn_idx, self.centres.shape[0], weight=self.balance / world, grad=self.g_knn_w)
+        self.balance_loss = loss * world
+
     def train_views(self, views, size, group=None, distributed=False, views_per_rank=None, exchange="factors"):
         """One iteration over the views this rank owns: for each view forward and backward (``libfsgs`` launches only,
         two C calls per view), the per-Gaussian gradients of the views summed in place in call order; then -- when
@@ -216,10 +223,8 @@ class DynamicScene:
         def after_last_view():
             if self.sp_radius is not None:
                 from .motion import kernel_weights_backward
-                if self.balance:  # the ranks' gradients are summed: each adds its part of the one term
-                    loss, _, self.superpoint_counts = balance_value_and_grad(
-                        self.knn_w, self.knn_idx, self.centres.shape[0], weight=self.balance / world, grad=self.g_knn_w)
-                    self.balance_loss = loss * world
+                if self.balance:
+                    self._add_balance(world)
                 kernel_weights_backward(self.knn_d2, self.knn_idx, self.sp_radius.data,
                                         None if self.sp_weight is None else self.sp_weight.data, self.g_knn_w,
                                         self.knn_idx.superpoint_pairs, b.view_of(self.sp_radius),

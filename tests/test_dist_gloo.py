@@ -100,3 +100,44 @@ def test_single_process_bucket_is_a_noop_reduce():
     assert b.reduce() is None and torch.equal(p.grad, torch.full((4, 2), 3.0)) and b.nbytes() >= 32
     v = torch.tensor([True, False])
     assert reduce_visibility(v) is v
+
+
+def _balance_worker(rank, world, port, out):
+    sys.path.insert(0, os.path.join(ROOT, "fast-sp-gs_b200"))
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    from fsgs import scene as module
+    N, K, M = 40, 3, 8
+    g = torch.Generator().manual_seed(0)
+
+    def on_the_host(weights, idx, points, mask=None, weight=1.0, grad=None):
+        """``balance_value_and_grad`` from its definition."""
+        counts = torch.bincount(idx.reshape(-1), minlength=points)
+        share = points * counts.double()[idx] / (counts.sum() * idx.shape[0])
+        grad += (weight * share).float()
+        return (weight * (share * weights.double()).sum()).float(), grad, counts
+
+    module.balance_value_and_grad = on_the_host
+    s = module.DynamicScene.__new__(module.DynamicScene)
+    s.centres, s.knn_idx = torch.zeros(M, 3), torch.randint(0, M, (N, K), generator=g)
+    s.knn_w, s.balance = torch.softmax(torch.randn(N, K, generator=g), dim=1), 0.3
+    from_views = torch.randn(world, N, K, generator=g)
+    alone = from_views.sum(dim=0)
+    loss, _, counts = on_the_host(s.knn_w, s.knn_idx, M, weight=0.3, grad=alone)   # one rank with all views
+    s.g_knn_w = from_views[rank].clone()
+    s._add_balance(dist.get_world_size())
+    dist.all_reduce(s.g_knn_w)
+    off = 4 * 2.0 ** -24 * (alone.abs() + from_views.abs().sum(dim=0))             # the ranks' sums are rounded apart
+    out[rank] = bool(((s.g_knn_w - alone).abs() <= off).all()) and abs(float(s.balance_loss) - float(loss)) <= 3 * 2.0 ** -24 * float(loss) \
+        and torch.equal(s.superpoint_counts, counts)
+    dist.destroy_process_group()
+
+
+def test_ranks_add_the_balance_term_once():
+    """Every rank adds its part of the balance term in front of the sum over the ranks: what one rank alone adds."""
+    mp.set_start_method("spawn", force=True)
+    with mp.Manager() as m:
+        for world in (2, 3):
+            out = m.dict()
+            mp.spawn(_balance_worker, args=(world, 31500 + (os.getpid() + world) % 2000, out), nprocs=world, join=True)
+            assert dict(out) == {r: True for r in range(world)}
