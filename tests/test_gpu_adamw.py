@@ -804,3 +804,23 @@ def test_eight_bit_second_moments_over_many_steps():
     assert torch.equal(now, codes)
     share = after / held
     assert float(share.min()) > 3.8 and float(share.max()) < 4.1
+
+
+def test_a_state_given_to_two_parameters_is_refused():
+    from fsgs.optim import AdamW
+    params, grads = _make((40, 40, 9), torch.float32, torch.float32)
+    for p, g in zip(params, grads):
+        p.grad = g
+    opt = AdamW(params)
+    opt.step()
+    kept = opt.state[params[1]]
+    frozen = [t.clone() for p in params for t in [p.detach()] + list(opt.state[p].values())]
+    for shared in (opt.state[params[0]], dict(kept, step=opt.state[params[2]]["step"])):
+        opt.state[params[1]] = shared
+        with pytest.raises(RuntimeError, match="share a state"):
+            opt.step()
+    opt.state[params[1]] = kept
+    assert all(torch.equal(a, b) for a, b in zip(frozen, [t for p in params for t in [p.detach()] + list(opt.state[p].values())]))
+    before = _snapshot(opt, params)
+    opt.step()
+    _check_step(opt, before, params, grads)
