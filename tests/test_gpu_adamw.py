@@ -824,3 +824,18 @@ def test_a_state_given_to_two_parameters_is_refused():
     before = _snapshot(opt, params)
     opt.step()
     _check_step(opt, before, params, grads)
+
+
+def test_roots_are_rounded_correctly():
+    """The root of the second moment for a quarter of a million mantissas, read back through the scale of a block in which it
+    is the largest: the float32 nearest to the root of fl(g^2) / 2, times the float32 nearest to 1/448."""
+    from fsgs.optim import AdamW
+    n, gen = 2 ** 18, torch.Generator("cuda").manual_seed(6)
+    g = torch.full((n, B), 2.0 ** -20, device="cuda")              # nothing in a lane leaves the range of the fast root
+    g[:, 8] = 1.0 + torch.randint(0, 2 ** 23, (n,), device="cuda", generator=gen).float() * 2.0 ** -23
+    p = torch.nn.Parameter(torch.zeros(n * B, device="cuda"))
+    p.grad = g.view(-1)
+    opt = AdamW([p], betas=(0.0, 0.5), state_bits=8)
+    opt.step()
+    root = ((g[:, 8] * g[:, 8]).double() / 2).sqrt().float()
+    assert torch.equal(opt.state[p]["exp_avg_sq_root_scale"], root * torch.tensor(1 / 448, dtype=torch.float32, device="cuda"))
