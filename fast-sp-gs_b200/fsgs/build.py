@@ -1,4 +1,5 @@
 """Builds ``libfsgs.so`` (sm_100a) next to the sources.  ``python -m fsgs.build`` or ``fsgs.build.build()``."""
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -14,10 +15,16 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
               "--expt-extended-lambda", "-Xcompiler", "-fPIC"]
 
 
+def _has_torch():
+    """Without torch (a host that uses the C ABI alone) the library is built and the host extension is not."""
+    return importlib.util.find_spec("torch") is not None
+
+
 def _stale():
-    if not os.path.exists(LIB) or not os.path.exists(HOST):
+    built = [LIB] + ([HOST] if _has_torch() else [])
+    if not all(os.path.exists(f) for f in built):
         return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(HOST))
+    t = min(os.path.getmtime(f) for f in built)
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps.append(os.path.join(os.path.dirname(os.path.dirname(PKG)), "include", "fsgs.h"))
     return any(os.path.getmtime(d) > t for d in deps)
@@ -41,8 +48,8 @@ def _host_command():
 
 
 def build(force=False, verbose=False):
-    """Compile every CUDA source for sm_100a and link the shared library, and compile the host extension beside it.  Returns
-    the library path."""
+    """Compile every CUDA source for sm_100a and link the shared library, and, where torch is installed, compile the host
+    extension beside it.  Returns the library path."""
     if not force and not _stale():
         return LIB
     os.makedirs(os.path.dirname(LIB), exist_ok=True)
@@ -52,8 +59,9 @@ def build(force=False, verbose=False):
         cmd = ["nvcc", "-c", os.path.join(CSRC, src), "-o", obj] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else [])
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
         objs.append(obj)
-    cmd = _host_command()
-    procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    if _has_torch():
+        cmd = _host_command()
+        procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     for cmd, p in procs:
         out, _ = p.communicate()
         if verbose or p.returncode:

@@ -209,3 +209,32 @@ def test_pairs_grouped_by_superpoint():
         run = pairs[int(offsets[m]):int(offsets[m + 1])].long()
         assert bool((flat[run] == m).all())                             # each run holds one superpoint's pairs
         assert run.tolist() == sorted(run.tolist())                     # in ascending pair order (stable)
+
+
+def test_the_library_is_built_without_torch(tmp_path):
+    """A host that uses the C ABI alone needs nvcc and no torch: the library is linked, the host extension left out.  (The
+    compilers here are stand-ins that write their output file.)"""
+    import subprocess
+    import sys
+    for name in ("nvcc", "g++"):
+        tool = tmp_path / name
+        tool.write_text(f"#!{sys.executable}\nimport sys\nopen(sys.argv[sys.argv.index('-o') + 1], 'w').close()\n")
+        tool.chmod(0o755)
+    code = ("import importlib.abc, importlib.util, os, sys\n"
+            "class No(importlib.abc.MetaPathFinder):\n"
+            "    def find_spec(self, name, path=None, target=None):\n"
+            "        if name.split('.')[0] == 'torch':\n"
+            "            raise ModuleNotFoundError(name, name=name)\n"
+            "without = sys.argv[1] == 'without'\n"
+            "import fsgs.build as b\n"
+            "if without:\n"
+            "    sys.meta_path.insert(0, No())\n"
+            "    importlib.util.find_spec = lambda name, package=None: None\n"
+            "b.LIB, b.HOST = (os.path.join(sys.argv[2], 'lib', n) for n in ('libfsgs.so', '_fsgs_host.so'))\n"
+            "b.build()\n"
+            "assert os.path.exists(b.LIB) and os.path.exists(b.HOST) == (not without) and not b._stale()\n")
+    env = dict(os.environ, PATH=f"{tmp_path}{os.pathsep}{os.environ['PATH']}", PYTHONPATH=os.path.join(ROOT, "fast-sp-gs_b200"))
+    for which in ("without", "with"):
+        out = tmp_path / which
+        out.mkdir()
+        subprocess.run([sys.executable, "-c", code, which, str(out)], check=True, env=env, timeout=120)
