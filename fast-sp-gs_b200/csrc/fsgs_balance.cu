@@ -636,7 +636,7 @@ extern "C" int fsgs_balance_pairs(int64_t N, int K, int M, const float *weights,
 extern "C" int fsgs_balance_table(int64_t N, int M, int type, const void *table, int64_t row_stride, const uint8_t *mask,
     const int64_t *counts, void *workspace, size_t workspace_bytes, float scale, const float *upstream, float *loss, void *g_table,
     int64_t g_row_stride, fsgs_stream_t stream) {
-  FSGS_REQUIRE(N >= 0 && M > 0 && counts && (table || N == 0) && row_stride >= M && (!g_table || g_row_stride >= M));
+  FSGS_REQUIRE(N >= 0 && M > 0 && (counts || !loss) && (table || N == 0) && row_stride >= M && (!g_table || g_row_stride >= M));
   FSGS_REQUIRE(type == FSGS_F32 || type == FSGS_BF16 || type == FSGS_F16);
   if (!balance_sizes(N, M)) return FSGS_ERR_LIMIT;
   if (!balance_workspace(N, 1, M, FSGS_BALANCE_TABLE, workspace, workspace_bytes)) return FSGS_ERR_WORKSPACE;

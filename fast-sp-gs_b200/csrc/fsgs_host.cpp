@@ -431,13 +431,14 @@ int check_table(const Tensor &table, const Tensor &idx, const std::optional<Tens
 const uint8_t *bytes_of(const std::optional<Tensor> &mask) { return mask ? (const uint8_t *) mask->data_ptr() : nullptr; }
 std::optional<Tensor> dense(const std::optional<Tensor> &mask) { return mask ? std::optional<Tensor>(mask->contiguous()) : mask; }
 struct Counted {
-  Tensor counts, ws;  // counts [M + 4]
+  Tensor counts, ws;  // counts [M + 4], and M more for a copy where one is asked for
+  int64_t M;
 };
 
-Counted count(const char *what, const Tensor &idx, int64_t M, const std::optional<Tensor> &mask, int form) {
+Counted count(const char *what, const Tensor &idx, int64_t M, const std::optional<Tensor> &mask, int form, bool copy = false) {
   const size_t bytes = lib.balance_bytes(idx.size(0), (int) idx.size(1), (int) M, form);
   need(bytes > 0, what, "more than 2^36 pairs or table entries");
-  Counted c{at::empty({M + 4}, idx.options()), at::empty({(int64_t) bytes}, idx.options().dtype(at::kByte))};
+  Counted c{at::empty({M + 4 + (copy ? M : 0)}, idx.options()), at::empty({(int64_t) bytes}, idx.options().dtype(at::kByte)), M};
   const Tensor i = idx.contiguous();
   check(lib.balance_count(i.size(0), (int) i.size(1), (int) M, i.data_ptr<int64_t>(), bytes_of(mask), form,
                           c.counts.data_ptr<int64_t>(), c.ws.data_ptr(), bytes, stream_of(i)),
@@ -447,16 +448,17 @@ Counted count(const char *what, const Tensor &idx, int64_t M, const std::optiona
 
 void pairs(int64_t N, int64_t K, const Counted &c, const float *weights, float scale, const float *upstream, float *loss, float *grad,
     bool accumulate) {
-  check(lib.balance_pairs(N, (int) K, (int) c.counts.numel() - 4, weights, c.counts.data_ptr<int64_t>(), c.ws.data_ptr(),
+  check(lib.balance_pairs(N, (int) K, (int) c.M, weights, c.counts.data_ptr<int64_t>(), c.ws.data_ptr(),
                           (size_t) c.ws.numel(), scale, upstream, loss, grad, accumulate, stream_of(c.ws)),
         "fsgs_balance_pairs");
 }
 
-void table_pass(const Tensor &t, int type, const std::optional<Tensor> &mask, const Counted &c, float scale, const float *upstream,
-    float *loss, void *grad) {
+// counts: for the loss alone
+void table_pass(const Tensor &t, int type, const std::optional<Tensor> &mask, const int64_t *counts, const Tensor &ws, float scale,
+    const float *upstream, float *loss, void *grad) {
   const int64_t N = t.size(0), M = t.size(1);
-  check(lib.balance_table(N, (int) M, type, t.data_ptr(), N > 1 ? t.stride(0) : M, bytes_of(mask), c.counts.data_ptr<int64_t>(),
-                          c.ws.data_ptr(), (size_t) c.ws.numel(), scale, upstream, loss, grad, M, stream_of(c.ws)),
+  check(lib.balance_table(N, (int) M, type, t.data_ptr(), N > 1 ? t.stride(0) : M, bytes_of(mask), counts, ws.data_ptr(),
+                          (size_t) ws.numel(), scale, upstream, loss, grad, M, stream_of(ws)),
         "fsgs_balance_table");
 }
 
@@ -494,18 +496,27 @@ struct PairsLoss : torch::autograd::Function<PairsLoss> {
   static variable_list forward(AutogradContext *ctx, const Tensor &weights, const Tensor &idx, int64_t M, const std::optional<Tensor> &mask) {
     const c10::cuda::CUDAGuard guard(weights.device());
     const Tensor w = weights.contiguous();
-    const Counted c = count(kPairs, idx, M, dense(mask), FSGS_BALANCE_PAIRS);
-    Tensor loss = at::empty({}, w.options().requires_grad(false)), counts = c.counts.narrow(0, 0, M);
+    const Counted c = count(kPairs, idx, M, dense(mask), FSGS_BALANCE_PAIRS, true);
+    Tensor loss = at::empty({}, w.options().requires_grad(false));
     pairs(idx.size(0), idx.size(1), c, w.data_ptr<float>(), 1.0f, nullptr, loss.data_ptr<float>(), nullptr, false);
-    ctx->save_for_backward({c.counts, c.ws});
-    ctx->saved_data["N"] = idx.size(0), ctx->saved_data["K"] = idx.size(1);
+    // the backward pass reads the counts: the caller, who may change what it is given, gets a copy (a part of the same tensor,
+    // so the saved one goes where autograd does not compare versions)
+    Tensor counts = c.counts.narrow(0, M + 4, M);
+    if (cudaMemcpyAsync(counts.data_ptr(), c.counts.data_ptr(), sizeof(int64_t) * (size_t) M, cudaMemcpyDeviceToDevice,
+                        (cudaStream_t) stream_of(c.ws)) != cudaSuccess) {
+      (void) cudaGetLastError();
+      check(FSGS_ERR_LAUNCH, "copy of the counts");
+    }
+    ctx->save_for_backward({c.ws});
+    ctx->saved_data["counts"] = c.counts;
+    ctx->saved_data["N"] = idx.size(0), ctx->saved_data["K"] = idx.size(1), ctx->saved_data["M"] = M;
     ctx->mark_non_differentiable({counts});
     return {loss, counts};
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     if (!g[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    const Counted c{saved[0], saved[1]};
+    const Counted c{ctx->saved_data["counts"].toTensor(), saved[0], ctx->saved_data["M"].toInt()};
     const c10::cuda::CUDAGuard guard(c.ws.device());
     hand_over(kPairs);
     const int64_t N = ctx->saved_data["N"].toInt(), K = ctx->saved_data["K"].toInt();
@@ -522,8 +533,8 @@ struct TableLoss : torch::autograd::Function<TableLoss> {
     const auto m = dense(mask);
     const Counted c = count(kTable, idx, t.size(1), m, FSGS_BALANCE_TABLE);
     Tensor loss = at::empty({}, t.options().dtype(at::kFloat).requires_grad(false)), counts = c.counts.narrow(0, 0, t.size(1));
-    table_pass(t, type_of(t.scalar_type()), m, c, 1.0f, nullptr, loss.data_ptr<float>(), nullptr);
-    ctx->save_for_backward({t, m ? *m : Tensor(), c.counts, c.ws});
+    table_pass(t, type_of(t.scalar_type()), m, c.counts.data_ptr<int64_t>(), c.ws, 1.0f, nullptr, loss.data_ptr<float>(), nullptr);
+    ctx->save_for_backward({t, m ? *m : Tensor(), c.ws});
     ctx->mark_non_differentiable({counts});
     return {loss, counts};
   }
@@ -535,7 +546,7 @@ struct TableLoss : torch::autograd::Function<TableLoss> {
     hand_over(kTable);
     Tensor grad = at::empty(t.sizes(), t.options().requires_grad(false));
     table_pass(t, type_of(t.scalar_type()), saved[1].defined() ? std::optional<Tensor>(saved[1]) : std::nullopt,
-               Counted{saved[2], saved[3]}, 1.0f, g[0].data_ptr<float>(), nullptr, grad.data_ptr());
+               nullptr, saved[2], 1.0f, g[0].data_ptr<float>(), nullptr, grad.data_ptr());
     return {once(grad, g[0]), Tensor(), Tensor()};
   }
 };
@@ -607,7 +618,7 @@ PyObject *balance_table(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Counted c = count(kTable, idx, t.size(1), m, FSGS_BALANCE_TABLE);
     Tensor loss = at::empty({}, t.options().dtype(at::kFloat).requires_grad(false));
     Tensor grad = at::empty(t.sizes(), t.options().requires_grad(false));
-    table_pass(t, type, m, c, weight, nullptr, loss.data_ptr<float>(), grad.data_ptr());
+    table_pass(t, type, m, c.counts.data_ptr<int64_t>(), c.ws, weight, nullptr, loss.data_ptr<float>(), grad.data_ptr());
     return tuple_of({loss, grad, c.counts.narrow(0, 0, t.size(1))});
   } catch (...) {
     return failed();

@@ -607,7 +607,7 @@ int fsgs_lbs_weights_backward(int P, int K, int M, const float *d2, const int64_
  * called any number of times, one after another, with the same counts and workspace.  scale and *upstream (device, optional)
  * multiply the loss and the gradient.  loss (device, one float) and the gradient are both optional.  accumulate: the
  * gradient is added to g_weights.  fsgs_balance_table: rows of M elements of `type`, row_stride / g_row_stride elements
- * apart; g_table has the table's type; its workspace is that of any K.  The order in which blocks finish does not change
+ * apart; g_table has the table's type; its workspace is that of any K; counts are read for the loss alone.  The order in which blocks finish does not change
  * the sums: the same inputs give the same bits.  N K <= 2^36, and N M <= 2^36 in the table form.
  * ---------------------------------------------------------------------------------------------- */
 #define FSGS_BALANCE_PAIRS 0

@@ -445,3 +445,23 @@ def test_balance_of_the_table_weighting():
     moved = torch.where(other == -math.inf, table, other + 3.0).cuda()
     assert torch.equal(balance_loss(lbs_weights(None, idx.cuda(), "table", table=moved), idx.cuda(), M)[0], loss.detach())
     assert not torch.equal(table_balance_loss(moved, idx.cuda())[0], table_balance_loss(own, idx.cuda())[0].detach())
+
+
+def test_the_counts_are_the_callers():
+    """Summed over ranks or steps in place before the backward pass, as counts are: the gradient is of the counts that the
+    loss was formed with."""
+    from fsgs.loss import balance_loss, balance_value_and_grad, table_balance_loss, table_balance_value_and_grad
+    gen = torch.Generator().manual_seed(13)
+    N, K, M = 300, 3, 20
+    idx = _indices(N, K, M, gen).cuda()
+    w, z = torch.rand(N, K, generator=gen).cuda(), torch.randn(N, M, generator=gen).cuda()
+    for x, form, plain in ((w, lambda t: balance_loss(t, idx, M), lambda t: balance_value_and_grad(t, idx, M)),
+                           (z, lambda t: table_balance_loss(t, idx), lambda t: table_balance_value_and_grad(t, idx))):
+        want, grad, counts = plain(x)
+        for change in (lambda c: c.mul_(2), lambda c: c.data.zero_()):
+            leaf = x.clone().requires_grad_()
+            loss, own = form(leaf)
+            assert torch.equal(own, counts)
+            change(own)
+            loss.backward()
+            assert torch.equal(loss.detach(), want) and torch.equal(leaf.grad, grad)
