@@ -25,7 +25,9 @@
 
 namespace fsgs {
 
-constexpr int kBalSharedPoints = 8192;    // superpoints whose histogram or shares are kept in shared memory (32 KB)
+// Superpoints whose histogram or shares are kept in shared memory (32 KB).  Above, a pair is an atomic on a 64-bit count in
+// memory: 2 M x 8 evenly over 8192 superpoints 62 us, over 8193 234 us, and 2.4 ms where a few of them take most pairs.
+constexpr int kBalSharedPoints = 8192;
 constexpr int kCountThreads = 1024;
 constexpr int kPairThreads = 512;
 constexpr int kTableThreads = 256;
@@ -87,7 +89,8 @@ __device__ __forceinline__ T block_total(T v, T *scratch) {  // valid in the fir
 // form the superpoint of every pair is kept as a 16- or 32-bit code (all ones: does not count) for the pass that needs the
 // complete counts, which then reads 2 bytes per pair instead of 8 and no mask, most of it from L2 (the indices are read,
 // and the weights and gradients of that pass streamed, so as not to displace the codes).  In the table form the block that finishes
-// last turns the counts into shares.  Bound by the read of the indices and, beside it, by one shared-memory atomic per pair.
+// last turns the counts into shares.  Bound by instructions, 41 per pair and 70 % of the issue slots at 2 M x 8 with a mask
+// (quotient, mask and code beside the atomic on shared memory), next to the read of the indices at 5.3 TB/s.
 template <typename Code, bool SHARED>
 __global__ void __launch_bounds__(kCountThreads, 2) balance_count_kernel(long long N, int K, int M, const int64_t *__restrict__ idx,
     const uint8_t *__restrict__ mask, int wide, unsigned magic, unsigned long long *__restrict__ counts, BalanceHead *__restrict__ head,
@@ -384,7 +387,9 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // table, and the shares come from the copy that is moved up by s.  What a group holds beside its row belongs to the
 // neighbouring rows; it is read and not used (the first and the last rows read element by element where there is no such
 // neighbour).  exp(z - max) is the hardware's exp2 of (z - max) log2(e); the difference is taken first, because z log2(e)
-// overflows for the type's lowest value, which stands for masked columns in places.  The row stays in registers from its
+// overflows for the type's lowest value, which stands for masked columns in places.  Both are rounded, so an exponential is
+// 2^-23 times the row's range off beside the 2 units of exp2, and the sum's inverse is the approximate one (2 units): loss and
+// gradient stay within 8.1e-8 of 64 bits where separate float32 operations are at 7.6e-8 (300 k x 512).  The row stays in registers from its
 // one read to the write of its gradient; the grid covers the rows and leaves the order to the hardware.
 template <typename T, int G, int PER, int ROWS>
 __global__ void __launch_bounds__(kTableThreads) balance_table_kernel(TableArgs a) {
@@ -543,6 +548,10 @@ static int table_launch(TableArgs &a, cudaStream_t st) {
   const int64_t blocks = (a.N + rows - 1) / rows;
   if (blocks > INT32_MAX) return FSGS_ERR_LIMIT;
   if (blocks == 0) return FSGS_OK;
+  // Rows are loaded beside their mask in calls of a few waves, where waiting for it shows, and only if they count in longer
+  // ones, where what they would read does (us, value and gradient, eager | after the mask; 3 % masked, then half): 20 k x
+  // 333 bf16 24.6 | 25.4, 25.5 | 25.5; 20 k x 512 float32 20.9 | 20.8, 22.3 | 21.3; 60 k x 512 float32 (7500 blocks) 52.0 |
+  // 51.4, 51.6 | 46.7; 300 k x 512 float32 202 | 200, 201 | 179, bf16 174 | 188, 172 | 181.
   a.eager = blocks <= 4096;
   balance_table_kernel<T, G, PER, ROWS><<<(int) blocks, kTableThreads, 0, st>>>(a);
   FSGS_LAUNCH_CHECK();
@@ -553,7 +562,9 @@ static int table_launch(TableArgs &a, cudaStream_t st) {
 // 16 bits, whose rows are instructions rather than bytes, have the next row's loads under way meanwhile.  Measured, value
 // and gradient (us; one row a thread group | two): 300 k x 512 bf16 177 | 171, 400 k x 256 bf16 140 | 123, 1 M x 100 bf16
 // 148 | 155, 2 M x 40 bf16 209 | 189; float32 is bound by memory (300 k x 512: 190 us, 6.5 TB/s) and takes one.  A warp
-// per row reaches to 1024 columns (100 k x 1000: 138 us, a block per row 244), a block per row lies above.
+// per row reaches to 1024 columns (100 k x 1000: 138 us, a block per row 244), a block per row lies above.  Rows of more than
+// 8192 columns do not fit the registers and are read three times: 12 k x 8192 float32 141 us (5.6 TB/s), 12 k x 8200 192,
+// 12 k x 20 000 655 (2.9 TB/s); bf16 150, 151.
 //
 // `reach`: columns from the first group of four to the row's end, M where every row starts on a boundary of four elements.
 template <typename T>
@@ -569,7 +580,7 @@ static int table_pick(TableArgs &a, int reach, cudaStream_t st) {
   if (reach <= 2048) return table_launch<T, 256, 8, 1>(a, st);
   if (reach <= 4096) return table_launch<T, 256, 16, 1>(a, st);
   if (reach <= 8192) return table_launch<T, 256, 32, 1>(a, st);
-  return table_launch<T, 256, 0, 1>(a, st);
+  return table_launch<T, 256, 0, 1>(a, st);  // reads the row three times
 }
 
 static bool balance_sizes(int64_t N, int64_t per_row) { return N <= (1ll << 36) / per_row; }
