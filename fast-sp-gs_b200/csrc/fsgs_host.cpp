@@ -55,11 +55,11 @@ struct StateTensor {
   void *data;
   int64_t numel;
   at::ScalarType type;
-  PyObject *now;   // the tensor that the last walk found
-  // still a dense tensor of that length and type there: the kernels trust all of it
-  bool is(const at::Tensor &x, c10::Device device) const {
-    return x.layout() == at::kStrided && x.device() == device && x.scalar_type() == type && x.numel() == numel && x.is_contiguous() &&
-           x.data_ptr() == data;
+  c10::TensorImpl *now;   // the tensor that the last walk found
+  // still a dense tensor of that length and type there (the address tells the device): the kernels trust all of it
+  bool is(c10::TensorImpl *x) const {
+    return x->has_storage() && x->dtype() == c10::scalarTypeToTypeMeta(type) && x->numel() == numel && x->is_contiguous() &&
+           (const char *) x->unsafe_storage().data() + x->storage_offset() * (int64_t) x->itemsize() == (const char *) data;
   }
 };
 
@@ -114,8 +114,8 @@ void need(bool ok, const char *what, const std::string &message) {
 }
 
 // What a kernel writes counts as modified in place: a graph that has saved it then raises instead of using the new values.
-void written(const at::Tensor &t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+void written(c10::TensorImpl *t) {
+  if (!t->is_inference()) t->bump_version();
 }
 
 // The names of a parameter's state, and where in its table row the address goes.
@@ -152,6 +152,7 @@ Entry entry_of(PyObject *param, Py_ssize_t group, PyObject *state, bool master, 
   row->param = e.data, row->numel = e.numel;
   Slot *slots = bits == 8 ? slots8 : slots32;
   const int n = (bits == 8 ? 6 : 4) - (master ? 0 : 1);
+  e.held.reserve((size_t) n);
   for (int k = 0; k < n; ++k) {
     Slot &s = slots[k];
     if (!s.key) s.key = PyUnicode_InternFromString(s.name);
@@ -166,7 +167,7 @@ Entry entry_of(PyObject *param, Py_ssize_t group, PyObject *state, bool master, 
              " elements on the parameter's device");
     if (s.untyped) row->*s.untyped = x.data_ptr();
     else row->*s.typed = (float *) x.data_ptr();
-    e.held.push_back({s.key, x.data_ptr(), size, kind, v});
+    e.held.push_back({s.key, x.data_ptr(), size, kind, x.unsafeGetTensorImpl()});
   }
   return e;
 }
@@ -177,6 +178,7 @@ Entry entry_of(PyObject *param, Py_ssize_t group, PyObject *state, bool master, 
 void need_apart(const std::vector<Entry> &entries) {
   std::vector<std::pair<const char *, const char *>> spans;
   std::vector<const void *> steps;
+  spans.reserve(entries.size()), steps.reserve(entries.size());
   for (const Entry &e : entries) {
     if (e.numel > 0) spans.emplace_back((const char *) e.data, (const char *) e.data + e.numel * c10::elementSize(e.type));
     steps.push_back(e.held[0].data);
@@ -201,6 +203,8 @@ PyObject *make_plan(PyObject *, PyObject *args) {
   }
   plan->keep = PyTuple_Pack(2, entries, launches);
   plan->params_key = PyUnicode_InternFromString("params");
+  const size_t count = (size_t) PyList_GET_SIZE(entries);
+  plan->entries.reserve(count), plan->norm.reserve(count), plan->place.reserve(count);
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(entries); ++i) {
     PyObject *param, *state;
     Py_ssize_t group;
@@ -263,10 +267,13 @@ int walk(Plan &plan, PyObject *groups, PyObject *state) {
       if (grad.scalar_type() != e.grad_type || grad.layout() != at::kStrided || grad.device() != t.device() || grad.numel() != e.numel)
         return kStale;
       strided = strided || !grad.is_contiguous();
+      PyObject *name, *v;
+      Py_ssize_t at = 0;
+      bool in_order = true;  // a state's tensors mostly stand as they were put there
       for (StateTensor &h : e.held) {
-        PyObject *v = PyDict_GetItem(e.state, h.name);
-        if (!v || !THPVariable_Check(v) || !h.is(THPVariable_Unpack(v), plan.device)) return kStale;
-        h.now = v;
+        in_order = in_order && PyDict_Next(e.state, &at, &name, &v) && name == h.name;
+        if (!in_order) v = PyDict_GetItem(e.state, h.name);
+        if (!v || !THPVariable_Check(v) || !h.is(h.now = THPVariable_Unpack(v).unsafeGetTensorImpl())) return kStale;
       }
       e.row->grad = grad.data_ptr();
       plan.norm[i].data = e.row->grad;
@@ -276,10 +283,13 @@ int walk(Plan &plan, PyObject *groups, PyObject *state) {
   if (i != plan.entries.size()) return kStale;
   PyObject *key, *value;
   Py_ssize_t pos = 0;
-  while (PyDict_Next(state, &pos, &key, &value)) {  // the states are still the parameters' states
-    auto it = plan.place.find(key);
-    if (it == plan.place.end()) continue;
-    if (plan.entries[it->second].state != value) return kStale;
+  for (size_t next = 0; PyDict_Next(state, &pos, &key, &value);) {  // the states are still the parameters' states
+    if (next >= plan.entries.size() || plan.entries[next].param != key) {  // mostly they come in the parameters' order
+      auto it = plan.place.find(key);
+      if (it == plan.place.end()) continue;
+      next = it->second;
+    }
+    if (plan.entries[next++].state != value) return kStale;
     ++found;
   }
   return found != plan.entries.size() ? kStale : strided ? kStrided : 0;
@@ -287,8 +297,8 @@ int walk(Plan &plan, PyObject *groups, PyObject *state) {
 
 void written(const Plan &plan) {
   for (const Entry &e : plan.entries) {
-    written(THPVariable_Unpack(e.param));
-    for (const StateTensor &h : e.held) written(THPVariable_Unpack(h.now));
+    written(THPVariable_Unpack(e.param).unsafeGetTensorImpl());
+    for (const StateTensor &h : e.held) written(h.now);
   }
 }
 
@@ -590,7 +600,7 @@ PyObject *balance_pairs(PyObject *, PyObject *const *args, Py_ssize_t n) {
     Tensor loss = at::empty({}, w.options().requires_grad(false));
     if (!add) grad = at::empty(w.sizes(), w.options().requires_grad(false));
     pairs(idx.size(0), idx.size(1), c, w.data_ptr<float>(), weight, nullptr, loss.data_ptr<float>(), grad.data_ptr<float>(), add);
-    if (add) written(grad);
+    if (add) written(grad.unsafeGetTensorImpl());
     return tuple_of({loss, grad, c.counts.narrow(0, 0, M)});
   } catch (...) {
     return failed();

@@ -169,7 +169,8 @@ class _Plan:
     they are what it was made from."""
 
     def __init__(self, opt):
-        self.settings, self.form = self.current_settings(opt), self.current_form(opt)
+        self.settings, self.form = self.current_settings(opt), (opt.state_bits, opt.master_weights)
+        self.seen = self.plain_settings(opt)
         self.params, self.groups, found, kinds = [], [], [], {}
         for k, group in enumerate(opt.param_groups):
             tail = self.settings[k][2:]
@@ -200,14 +201,18 @@ class _Plan:
         return [(_number(g["lr"]), _number(g["weight_decay"]), *map(_number, g["betas"]), _number(g["eps"]))
                 for g in opt.param_groups]
 
-    @staticmethod
-    def current_form(opt):
-        return opt.state_bits, opt.master_weights
+    def plain_settings(self, opt):
+        """The same as they stand there, None where one of them is no float (a tensor may change where it lies)."""
+        found = [(g["lr"], g["weight_decay"], *g["betas"], g["eps"]) for g in opt.param_groups]
+        return found if all(v.__class__ is float for t in found for v in t) else None
 
     def follow(self, opt):
         """Take over changed learning rates and weight decays; False where betas, eps or the form of the state changed."""
-        if self.current_form(opt) != self.form:
+        if (opt.state_bits, opt.master_weights) != self.form:
             return False
+        if self.seen is not None and self.seen == [(g["lr"], g["weight_decay"], *g["betas"], g["eps"]) for g in opt.param_groups]:
+            return True
+        self.seen = self.plain_settings(opt)
         now = self.current_settings(opt)
         if now != self.settings:
             if [s[2:] for s in now] != [s[2:] for s in self.settings]:
