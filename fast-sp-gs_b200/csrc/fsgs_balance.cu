@@ -16,7 +16,8 @@
 // 6.57 TB/s; device time): 2 M x 8 pairs over 4096 superpoints 59 us, 30 counting (160 MB at 5.3 TB/s; neither the
 // shared-memory atomics nor their flush show: 30.9 and 29.0 us without them) and 27 for loss and gradient (160 MB at 5.9
 // TB/s); 300 k x 3 over 512 12 us in three nodes; table 300 k x 512 float32, value and gradient, 178 us (6.9 TB/s) and 12
-// of counting and closing; bf16 171 us in all (3.7 TB/s, bound by instructions: 28 per column and lane).
+// of counting and closing; bf16 171 us in all (3.7 TB/s, bound by instructions: 28 per column, about 10 of them the row's
+// arithmetic, the others for rows off a boundary of four, partial groups and masked rows).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
