@@ -2,8 +2,8 @@
 //
 // The optimiser step: reads every address, length and type of the parameters, gradients and states anew each step, straight
 // from the tensors, hands them to the C entry points and marks what they write.  In Python the same walk costs 1.2 us per
-// tensor (190 us for a network of 120 tensors whose kernels take 17 us); here 0.08 us.  The balance losses: argument checks, outputs, and the autograd
-// nodes.
+// tensor (190 us for a network of 120 tensors whose kernels take 17 us); here 0.08 us.  The balance losses: argument checks,
+// outputs, and the autograd nodes.
 //
 // A CPython extension compiled against torch's headers; it holds no CUDA code and calls libfsgs.so through the function
 // pointers that bind() gives it.
