@@ -258,8 +258,9 @@ class AdamW(torch.optim.Optimizer):
     A dropped step -- that, or a closed ``gate`` -- leaves parameters, moments and step counts as they were; the decision
     is taken on the device.  Nothing synchronises.  A step can be captured into a CUDA graph once the state exists (after
     a step, or ``init_state()``): the step counts advance with every replay, while learning rates and the other numbers
-    are those of the capture, and gradients are read where they lay then.  Steps of one optimiser have to follow one
-    another on their stream."""
+    are those of the capture, and gradients are read where they lay then; the optimiser, whose states and workspaces a
+    replay uses, has to live as long as the graph.  Steps of one optimiser have to follow one another, on one stream or on
+    streams that wait for each other.  What a step writes counts as modified in place."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
                  master_weights=False, max_grad_norm=None):
